@@ -86,5 +86,36 @@ namespace ILGPU.Algorithms.Hip
             IntPtr stream, void* source, long sourceLength, int sourceType, void* target,
             long targetLength, int targetType, int* order, long orderLength, int transformer,
             long factor);
+
+        [DllImport(LibName)] internal static extern int ilgpu_hip_embedding(
+            IntPtr stream, void* table, long vocabulary, long dimension, long tableStride,
+            int tableType, void* tokens, long count, int tokenType, float* hostScale,
+            void* output, long outStride, int outType);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_embedding_gradient_temp_bytes(
+            long count, long vocabulary, long dimension, out long tempBytes);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_embedding_gradient(
+            IntPtr stream, void* gradOut, long gradOutStride, int gradOutType, void* tokens,
+            long count, int tokenType, float* hostScale, long paddingToken, int accumulate,
+            void* gradTable, long vocabulary, long dimension, long gradTableStride,
+            int gradTableType, void* temp, long tempBytes);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_layer_norm(
+            IntPtr stream, void* input, long rows, long columns, long inStride, int type,
+            void* weight, void* bias, int weightType, float* hostEpsilon, void* output,
+            long outStride, float* mean, float* rstd);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_layer_norm_gradient_temp_bytes(
+            long rows, long columns, out long tempBytes);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_layer_norm_gradient(
+            IntPtr stream, void* gradOut, long gradOutStride, void* input, long inStride,
+            long rows, long columns, int type, void* weight, int weightType, float* mean,
+            float* rstd, void* gradIn, long gradInStride, void* gradWeight, void* gradBias,
+            int accumulate, void* temp, long tempBytes);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_gradient_norm_temp_bytes(
+            long count, out long tempBytes);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_gradient_norm(
+            IntPtr stream, HipTensor* hostTensors, long count, float* norm, void* temp,
+            long tempBytes);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_clip_gradients(
+            IntPtr stream, HipTensor* hostSources, HipTensor* hostTargets, long count,
+            float* norm, float* hostMaxNorm);
     }
 }

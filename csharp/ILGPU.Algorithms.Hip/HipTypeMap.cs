@@ -16,6 +16,8 @@ namespace ILGPU.Algorithms.Hip
         // ilgpu_hip_type: NumericTypes of TypeInformation.ttinclude:94-121, in order.
         public const int I8 = 0, I16 = 1, I32 = 2, I64 = 3, U8 = 4, U16 = 5, U32 = 6, U64 = 7,
             F16 = 8, F32 = 9, F64 = 10;
+        // taken by the operators of HipLanguageModelExtensions only
+        public const int BF16 = 11;
         // ilgpu_hip_op
         public const int OpAdd = 0, OpMax = 1, OpMin = 2;
         // ilgpu_hip_scan_kind: ScanKind.Inclusive / Exclusive (ScanExtensions.cs:27-38)
@@ -34,7 +36,7 @@ namespace ILGPU.Algorithms.Hip
             { typeof(sbyte), I8 }, { typeof(short), I16 }, { typeof(int), I32 },
             { typeof(long), I64 }, { typeof(byte), U8 }, { typeof(ushort), U16 },
             { typeof(uint), U32 }, { typeof(ulong), U64 }, { typeof(Half), F16 },
-            { typeof(float), F32 }, { typeof(double), F64 },
+            { typeof(float), F32 }, { typeof(double), F64 }, { typeof(HipBFloat16), BF16 },
             { typeof(Index1D), I32 }, { typeof(LongIndex1D), I64 },
         };
 

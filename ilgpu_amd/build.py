@@ -4,7 +4,7 @@
 (in parallel) and links them into ``ilgpu_amd/lib/libilgpu_hip_algorithms.so``.
 hipcc cross-compiles, so no GPU is needed.  The shared library is kept in the
 tree (git-ignored) so that it travels with the source to the machine that runs
-it.  The same call builds the C++ host-layer test program and the
+it.  The same call builds the C++ host-layer test programs and the
 micro-benchmarks of ``bench_bounds.hip``.
 
 ``python -m ilgpu_amd.build --variant NAME -D MACRO=VALUE [-D ...] [--units a,b]``
@@ -117,23 +117,24 @@ def build_bounds() -> str:
     return BOUNDS_BIN
 
 
-HOST_TEST_SRC = os.path.join(os.path.dirname(HERE), "tests", "cpp",
-                             "host_api_tests.cpp")
-HOST_TEST_BIN = os.path.join(os.path.dirname(HERE), "tests", "cpp",
-                             "host_api_tests")
+CPP_TESTS = os.path.join(os.path.dirname(HERE), "tests", "cpp")
+HOST_TEST_SRC = os.path.join(CPP_TESTS, "host_api_tests.cpp")
+HOST_TEST_BIN = os.path.join(CPP_TESTS, "host_api_tests")
+OPERATOR_TEST_SRC = os.path.join(CPP_TESTS, "operator_tests.cpp")
+OPERATOR_TEST_BIN = os.path.join(CPP_TESTS, "operator_tests")
 
 
-def build_host_example() -> str:
-    """Compiles the C++ host-layer test program against the built library."""
+def build_host_example(source: str = HOST_TEST_SRC, binary: str = HOST_TEST_BIN) -> str:
+    """Compiles a C++ host-layer test program against the built library."""
     cmd = [HIPCC, "-x", "c++", "-std=c++17", "-O2", "-D__HIP_PLATFORM_AMD__",
-           "-I/opt/rocm/include", HOST_TEST_SRC, "-o", HOST_TEST_BIN,
+           "-I/opt/rocm/include", source, "-o", binary,
            "-L" + LIB_DIR, "-lilgpu_hip_algorithms",
            "-L/opt/rocm/lib", "-lamdhip64",
            "-Wl,-rpath,$ORIGIN/../../ilgpu_amd/lib", "-Wl,-rpath,/opt/rocm/lib"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"host test build failed:\n{proc.stderr}")
-    return HOST_TEST_BIN
+    return binary
 
 
 if __name__ == "__main__":
@@ -149,4 +150,5 @@ if __name__ == "__main__":
     else:
         print(build())
         print(build_host_example())
+        print(build_host_example(OPERATOR_TEST_SRC, OPERATOR_TEST_BIN))
         print(build_bounds())

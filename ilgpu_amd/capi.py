@@ -29,7 +29,7 @@ SUCCESS, ERROR_NULL_VIEW, ERROR_OUT_OF_RANGE, ERROR_NOT_SUPPORTED, \
     ERROR_UNALIGNED_TEMP, ERROR_RUNTIME, ERROR_STATIC_LIMIT = range(7)
 SCAN_STATIC_MAX_BYTES = 1 << 30
 # ilgpu_hip_type
-I8, I16, I32, I64, U8, U16, U32, U64, F16, F32, F64 = range(11)
+I8, I16, I32, I64, U8, U16, U32, U64, F16, F32, F64, BF16 = range(12)
 # ilgpu_hip_op / scan kind / flags / value source / locator
 OP_ADD, OP_MAX, OP_MIN = 0, 1, 2
 SCAN_INCLUSIVE, SCAN_EXCLUSIVE = 0, 1
@@ -53,14 +53,23 @@ EXPORTS = [
     "ilgpu_hip_unique_temp_bytes", "ilgpu_hip_unique", "ilgpu_hip_initialize",
     "ilgpu_hip_sequence", "ilgpu_hip_reorder",
     "ilgpu_hip_transform", "ilgpu_hip_reorder_transform",
+    "ilgpu_hip_embedding", "ilgpu_hip_embedding_gradient_temp_bytes",
+    "ilgpu_hip_embedding_gradient", "ilgpu_hip_layer_norm",
+    "ilgpu_hip_layer_norm_gradient_temp_bytes", "ilgpu_hip_layer_norm_gradient",
+    "ilgpu_hip_gradient_norm_temp_bytes", "ilgpu_hip_gradient_norm",
+    "ilgpu_hip_clip_gradients",
 ]
+
+# numpy has no bfloat16: a dtype of its own that holds the 16 bits, so that a
+# DeviceArray of them is not one of uint16.  ``a.view(np.uint16)`` gives the bits.
+bfloat16 = np.dtype([("bfloat16", np.uint16)])
 
 _NP_TO_TYPE = {
     np.dtype(np.int8): I8, np.dtype(np.int16): I16, np.dtype(np.int32): I32,
     np.dtype(np.int64): I64, np.dtype(np.uint8): U8, np.dtype(np.uint16): U16,
     np.dtype(np.uint32): U32, np.dtype(np.uint64): U64,
     np.dtype(np.float16): F16, np.dtype(np.float32): F32,
-    np.dtype(np.float64): F64,
+    np.dtype(np.float64): F64, bfloat16: BF16,
 }
 
 
@@ -158,6 +167,20 @@ def lib() -> ctypes.CDLL:
         L.ilgpu_hip_reduce.argtypes = [vp, vp, i64, i64, i32, i32, vp, i64, vp, i64]
         L.ilgpu_hip_histogram.argtypes = [vp, vp, i64, i64, i32, vp, i64, i32,
                                           i32, vp]
+        pf = ctypes.POINTER(ctypes.c_float)
+        L.ilgpu_hip_embedding.argtypes = [vp, vp, i64, i64, i64, i32, vp, i64, i32, pf, vp, i64,
+                                          i32]
+        L.ilgpu_hip_embedding_gradient_temp_bytes.argtypes = [i64, i64, i64, p64]
+        L.ilgpu_hip_embedding_gradient.argtypes = [
+            vp, vp, i64, i32, vp, i64, i32, pf, i64, i32, vp, i64, i64, i64, i32, vp, i64]
+        L.ilgpu_hip_layer_norm.argtypes = [vp, vp, i64, i64, i64, i32, vp, vp, i32, pf, vp, i64,
+                                           vp, vp]
+        L.ilgpu_hip_layer_norm_gradient_temp_bytes.argtypes = [i64, i64, p64]
+        L.ilgpu_hip_layer_norm_gradient.argtypes = [
+            vp, vp, i64, vp, i64, i64, i64, i32, vp, i32, vp, vp, vp, i64, vp, vp, i32, vp, i64]
+        L.ilgpu_hip_gradient_norm_temp_bytes.argtypes = [i64, p64]
+        L.ilgpu_hip_gradient_norm.argtypes = [vp, vp, i64, vp, vp, i64]
+        L.ilgpu_hip_clip_gradients.argtypes = [vp, vp, vp, i64, vp, pf]
         for name in EXPORTS:
             if name.endswith(("_bytes", "_keys", "_pairs", "_scan", "_reduce",
                               "_histogram")):
@@ -212,6 +235,16 @@ class DeviceArray:
         return cls(a.size, a.dtype, _bytes=host.to("cuda:0"))
 
     @classmethod
+    def from_tensor(cls, t) -> "DeviceArray":
+        """The elements of a contiguous torch tensor on the GPU, in place: the
+        tensor's own memory, kept alive by this array."""
+        if not t.is_cuda or not t.is_contiguous():
+            raise ValueError("a contiguous tensor on the GPU is needed")
+        import torch
+        return cls(t.numel(), _torch_dtype(t.dtype),
+                   _bytes=t.detach().view(-1).view(torch.uint8))
+
+    @classmethod
     def zeros(cls, length: int, dtype) -> "DeviceArray":
         out = cls(length, dtype)
         out.bytes.zero_()
@@ -251,6 +284,92 @@ class DeviceArray:
         s = self.dtype.itemsize
         return DeviceArray(length, self.dtype,
                            _bytes=self.bytes[offset * s:(offset + length) * s])
+
+
+_torch_to_np = None
+
+
+def _torch_dtype(dtype) -> np.dtype:
+    global _torch_to_np
+    if _torch_to_np is None:
+        import torch
+        _torch_to_np = {
+            torch.int8: np.dtype(np.int8), torch.int16: np.dtype(np.int16),
+            torch.int32: np.dtype(np.int32), torch.int64: np.dtype(np.int64),
+            torch.uint8: np.dtype(np.uint8), torch.float16: np.dtype(np.float16),
+            torch.float32: np.dtype(np.float32), torch.float64: np.dtype(np.float64),
+            torch.bfloat16: bfloat16,
+        }
+    if dtype not in _torch_to_np:
+        raise NotSupportedError(ERROR_NOT_SUPPORTED, f"torch type {dtype}")
+    return _torch_to_np[dtype]
+
+
+class DeviceMatrix:
+    """``rows`` x ``columns`` elements of a DeviceArray: element (r, c) is element
+    ``r * row_stride + c`` of it.  A row stride of 0 (one row for all) is for
+    matrices that are only read."""
+
+    def __init__(self, base: DeviceArray, rows: int, columns: int,
+                 row_stride: Optional[int] = None):
+        self.base = base
+        self.rows, self.columns = int(rows), int(columns)
+        self.row_stride = self.columns if row_stride is None else int(row_stride)
+        self.dtype, self.type_code = base.dtype, base.type_code
+        if min(self.rows, self.columns, self.row_stride) < 0 or (
+                self.rows > 0
+                and (self.rows - 1) * self.row_stride + self.columns > base.length):
+            raise ArgumentOutOfRangeError(ERROR_OUT_OF_RANGE, "matrix")
+
+    @classmethod
+    def from_tensor(cls, t) -> "DeviceMatrix":
+        """The last dimension of a torch tensor on the GPU as columns and all others
+        as rows, in place.  The columns have to lie side by side and the rows at one
+        stride (0 where a tensor was expanded)."""
+        import torch
+        if not t.is_cuda or t.dim() < 1:
+            raise ValueError("a tensor on the GPU with at least one dimension is needed")
+        t = t.detach()
+        t = t.view(-1, t.shape[-1]) if t.numel() else t.reshape(t.numel(), t.shape[-1])
+        rows, columns = t.shape
+        if columns > 1 and rows > 0 and t.stride(1) != 1:
+            raise ValueError("the elements of a row have to lie side by side")
+        stride = t.stride(0) if rows > 1 else columns
+        length = (rows - 1) * stride + columns if rows else 0
+        flat = torch.as_strided(t, (length,), (1,)) if length else t.reshape(-1)
+        return cls(DeviceArray.from_tensor(flat), rows, columns, stride)
+
+    @property
+    def ptr(self) -> int:
+        return self.base.ptr if self.rows > 0 else 0
+
+
+class _Tensor(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("length", ctypes.c_int64),
+                ("type", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class TensorList:
+    """A list of DeviceArrays as the calls over many tensors take it; it keeps the
+    arrays, and can be used for any number of calls."""
+
+    def __init__(self, arrays):
+        self.arrays = [_dense(a) for a in arrays]
+        self.table = (_Tensor * max(1, len(self.arrays)))(
+            *((a.ptr, a.length, a.type_code, 0) for a in self.arrays))
+
+    def __len__(self) -> int:
+        return len(self.arrays)
+
+
+def _tensor_list(tensors) -> "TensorList":
+    return tensors if isinstance(tensors, TensorList) else TensorList(tensors)
+
+
+def _dense(a: DeviceArray) -> DeviceArray:
+    if a.stride != 1:
+        raise NotSupportedError(ERROR_NOT_SUPPORTED, "a dense view is needed")
+    return a
 
 
 def temp_buffer(nbytes: int) -> DeviceArray:
@@ -490,3 +609,157 @@ def reorder_transform(source: DeviceArray, target: DeviceArray,
         _stream_ptr(stream), source.ptr, source.length, source.type_code,
         target.ptr, target.length, target.type_code, order.ptr, order.length,
         transformer, factor))
+
+
+# ---- operators of language models ----------------------------------------------
+def _scratch(nbytes: int, stream) -> DeviceArray:
+    """A temp of the call's own.  On another stream than torch's current one it is
+    taken from that stream's memory: what is freed there waits for that stream."""
+    if stream is None:
+        return temp_buffer(nbytes)
+    import torch
+    pointer = _stream_ptr(stream)
+    with torch.cuda.stream(torch.cuda.ExternalStream(pointer) if pointer
+                           else torch.cuda.default_stream()):
+        return temp_buffer(nbytes)
+
+
+def _float(value) -> ctypes.c_float:
+    return ctypes.byref(ctypes.c_float(value))
+
+
+def _need(condition: bool, what: str) -> None:
+    if not condition:
+        raise ArgumentOutOfRangeError(ERROR_OUT_OF_RANGE, what)
+
+
+def _column_vector(a: Optional[DeviceArray], length: int, what: str):
+    if a is None:
+        return None
+    _need(_dense(a).length == length, what)
+    return a.ptr
+
+
+def _statistic(a: Optional[DeviceArray], rows: int, what: str):
+    if a is None:
+        return None
+    if a.type_code != F32:
+        raise NotSupportedError(ERROR_NOT_SUPPORTED, f"{what} is float32")
+    _need(_dense(a).length >= rows, what)
+    return a.ptr
+
+
+def embedding(table: DeviceMatrix, tokens: DeviceArray, out: DeviceMatrix, *,
+              scale: float = 1.0, stream=None) -> None:
+    """out[i] = scale * table[tokens[i]]; tokens outside the table (int32 or int64,
+    -1 for padding) give rows of zeros."""
+    _need(out.rows == _dense(tokens).length and out.columns == table.columns, "out")
+    check((_lib or lib()).ilgpu_hip_embedding(
+        _stream_ptr(stream), table.ptr, table.rows, table.columns, table.row_stride,
+        table.type_code, tokens.ptr, tokens.length, tokens.type_code, _float(scale), out.ptr,
+        out.row_stride, out.type_code))
+
+
+def embedding_gradient_temp_bytes(count: int, vocabulary: int, dimension: int) -> int:
+    return _query(lib().ilgpu_hip_embedding_gradient_temp_bytes, count, vocabulary, dimension)
+
+
+def embedding_gradient(grad_out: DeviceMatrix, tokens: DeviceArray, grad_table: DeviceMatrix,
+                       temp: Optional[DeviceArray] = None, *, scale: float = 1.0,
+                       padding_token: int = -1, accumulate: bool = False,
+                       stream=None) -> None:
+    """grad_table[v] = scale * sum of grad_out[i] over the positions i of token v, zeros
+    where there is none; with accumulate the sums are added to what is there.
+    padding_token and tokens outside the table contribute nothing."""
+    _need(grad_out.rows == _dense(tokens).length, "grad_out")
+    _need(grad_out.columns == grad_table.columns, "grad_table")
+    if temp is None:
+        temp = _scratch(embedding_gradient_temp_bytes(
+            tokens.length, grad_table.rows, grad_table.columns), stream)
+    check((_lib or lib()).ilgpu_hip_embedding_gradient(
+        _stream_ptr(stream), grad_out.ptr, grad_out.row_stride, grad_out.type_code, tokens.ptr,
+        tokens.length, tokens.type_code, _float(scale), padding_token, 1 if accumulate else 0,
+        grad_table.ptr, grad_table.rows, grad_table.columns, grad_table.row_stride,
+        grad_table.type_code, temp.ptr, temp.nbytes))
+
+
+def layer_norm(inp: DeviceMatrix, out: DeviceMatrix, weight: Optional[DeviceArray] = None,
+               bias: Optional[DeviceArray] = None, *, epsilon: float = 1e-5,
+               mean: Optional[DeviceArray] = None, rstd: Optional[DeviceArray] = None,
+               stream=None) -> None:
+    """Every row of inp less its mean, over its deviation, times weight, plus bias; mean
+    and rstd (float32) receive what the gradient needs of the rows."""
+    _need(out.rows == inp.rows and out.columns == inp.columns, "out")
+    some = weight if weight is not None else bias
+    weight_type = inp.type_code if some is None else some.type_code
+    if out.type_code != inp.type_code or (bias is not None and bias.type_code != weight_type):
+        raise NotSupportedError(ERROR_NOT_SUPPORTED, "types differ")
+    check((_lib or lib()).ilgpu_hip_layer_norm(
+        _stream_ptr(stream), inp.ptr, inp.rows, inp.columns, inp.row_stride, inp.type_code,
+        _column_vector(weight, inp.columns, "weight"), _column_vector(bias, inp.columns, "bias"),
+        weight_type, _float(epsilon), out.ptr, out.row_stride,
+        _statistic(mean, inp.rows, "mean"), _statistic(rstd, inp.rows, "rstd")))
+
+
+def layer_norm_gradient_temp_bytes(rows: int, columns: int) -> int:
+    return _query(lib().ilgpu_hip_layer_norm_gradient_temp_bytes, rows, columns)
+
+
+def layer_norm_gradient(grad_out: DeviceMatrix, inp: DeviceMatrix,
+                        weight: Optional[DeviceArray], mean: DeviceArray, rstd: DeviceArray,
+                        grad_in: Optional[DeviceMatrix] = None,
+                        grad_weight: Optional[DeviceArray] = None,
+                        grad_bias: Optional[DeviceArray] = None,
+                        temp: Optional[DeviceArray] = None, *, accumulate: bool = False,
+                        stream=None) -> None:
+    """The gradients of layer_norm from the mean and rstd it left; those passed as None
+    are not computed.  With accumulate grad_weight and grad_bias are added to."""
+    _need(grad_out.rows == inp.rows and grad_out.columns == inp.columns, "grad_out")
+    if grad_in is not None:
+        _need(grad_in.rows == inp.rows and grad_in.columns == inp.columns, "grad_in")
+    vectors = [a for a in (weight, grad_weight, grad_bias) if a is not None]
+    weight_type = vectors[0].type_code if vectors else inp.type_code
+    if grad_out.type_code != inp.type_code or (
+            grad_in is not None and grad_in.type_code != inp.type_code) or any(
+            a.type_code != weight_type for a in vectors):
+        raise NotSupportedError(ERROR_NOT_SUPPORTED, "types differ")
+    if temp is None:
+        temp = _scratch(layer_norm_gradient_temp_bytes(inp.rows, inp.columns), stream)
+    check((_lib or lib()).ilgpu_hip_layer_norm_gradient(
+        _stream_ptr(stream), grad_out.ptr, grad_out.row_stride, inp.ptr, inp.row_stride,
+        inp.rows, inp.columns, inp.type_code, _column_vector(weight, inp.columns, "weight"),
+        weight_type, _statistic(mean, inp.rows, "mean"), _statistic(rstd, inp.rows, "rstd"),
+        None if grad_in is None else grad_in.ptr,
+        0 if grad_in is None else grad_in.row_stride,
+        _column_vector(grad_weight, inp.columns, "grad_weight"),
+        _column_vector(grad_bias, inp.columns, "grad_bias"), 1 if accumulate else 0,
+        temp.ptr, temp.nbytes))
+
+
+def gradient_norm_temp_bytes(count: int) -> int:
+    return _query(lib().ilgpu_hip_gradient_norm_temp_bytes, count)
+
+
+def gradient_norm(gradients, norm: DeviceArray, temp: Optional[DeviceArray] = None, *,
+                  stream=None) -> None:
+    """norm[0] (float32, on the device) = the root of the sum of the squares of all
+    elements of a TensorList, or of a list of DeviceArrays."""
+    gradients = _tensor_list(gradients)
+    if temp is None:
+        temp = _scratch(gradient_norm_temp_bytes(len(gradients)), stream)
+    check((_lib or lib()).ilgpu_hip_gradient_norm(
+        _stream_ptr(stream), gradients.table, len(gradients), _statistic(norm, 1, "norm"),
+        temp.ptr, temp.nbytes))
+
+
+def clip_gradients(gradients, norm: DeviceArray, max_norm: float, targets=None, *,
+                   stream=None) -> None:
+    """Scales all gradients by max_norm / norm[0] where norm[0] (on the device) is finite
+    and larger than max_norm, in place or into targets."""
+    gradients = _tensor_list(gradients)
+    if targets is not None:
+        targets = _tensor_list(targets)
+        _need(len(targets) == len(gradients), "targets")
+    check((_lib or lib()).ilgpu_hip_clip_gradients(
+        _stream_ptr(stream), gradients.table, None if targets is None else targets.table,
+        len(gradients), _statistic(norm, 1, "norm"), _float(max_norm)))

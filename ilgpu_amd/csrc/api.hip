@@ -8,6 +8,7 @@
 #include <string>
 #include <vector>
 
+#include "elements.hpp"
 #include "kernels.hpp"
 
 namespace ilgpu_hip {
@@ -135,6 +136,37 @@ inline bool scan_reduce_type(int32_t t) {
 inline bool valid_op(int32_t op) {
   return op == ILGPU_HIP_OP_ADD || op == ILGPU_HIP_OP_MAX ||
          op == ILGPU_HIP_OP_MIN;
+}
+
+// A rows x columns matrix that a call reads (written = false) or writes.
+inline int32_t check_matrix(const void* data, int64_t rows, int64_t columns, int64_t stride,
+                            int elem_bytes, bool written) {
+  if (columns == 0 || (rows > 0 && data == nullptr)) return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (rows < 0 || columns < 0 || stride < (written && rows > 1 ? columns : 0))
+    return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  if (rows > INT32_MAX || columns > INT32_MAX || stride > INT32_MAX)
+    return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  if (!aligned_to(data, elem_bytes)) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  return ILGPU_HIP_SUCCESS;
+}
+
+// The list of a norm or of a clip.
+inline int32_t check_tensors(const ilgpu_hip_tensor* tensors, int64_t count) {
+  if (count < 0) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  if (count > INT32_MAX) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  if (count > 0 && tensors == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  int64_t total = 0;
+  for (int64_t k = 0; k < count; ++k) {
+    const int eb = operator_elem_size(tensors[k].type);
+    if (eb < 0) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+    if (tensors[k].length < 0) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+    if (tensors[k].length == 0) continue;
+    if (tensors[k].data == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+    if (!aligned_to(tensors[k].data, eb)) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+    if (tensors[k].length > (INT64_C(1) << 40) - total) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+    total += tensors[k].length;
+  }
+  return ILGPU_HIP_SUCCESS;
 }
 
 }  // namespace
@@ -578,6 +610,180 @@ int32_t ilgpu_hip_reorder_transform(ilgpu_hip_stream_t stream,
   TransformArgs a{source, 1, source_type, target, 1, target_type, order,
                   order_length, transformer, factor};
   return launch_transform(static_cast<hipStream_t>(stream), a);
+}
+
+/* ---- embedding ----------------------------------------------------------- */
+
+static int32_t check_tokens(const void* tokens, int64_t count, int32_t token_type) {
+  if (token_type != ILGPU_HIP_I32 && token_type != ILGPU_HIP_I64)
+    return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  if (count < 0) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  if (count > INT32_MAX) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  if (count > 0 && tokens == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (!aligned_to(tokens, elem_size(token_type))) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  return ILGPU_HIP_SUCCESS;
+}
+
+int32_t ilgpu_hip_embedding(ilgpu_hip_stream_t stream, const void* table,
+                            int64_t vocabulary, int64_t dimension,
+                            int64_t table_stride, int32_t table_type,
+                            const void* tokens, int64_t count,
+                            int32_t token_type, const float* scale, void* out,
+                            int64_t out_stride, int32_t out_type) {
+  const int tb = operator_elem_size(table_type), ob = operator_elem_size(out_type);
+  if (tb < 0 || ob < 0) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  int32_t rc = check_tokens(tokens, count, token_type);
+  if (rc == ILGPU_HIP_SUCCESS)
+    rc = check_matrix(table, vocabulary, dimension, table_stride, tb, false);
+  if (rc == ILGPU_HIP_SUCCESS) rc = check_matrix(out, count, dimension, out_stride, ob, true);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  const EmbeddingArgs a{table, vocabulary, dimension, table_stride, table_type, tokens, count,
+                        token_type, scale != nullptr ? *scale : 1.0f, out, out_stride, out_type};
+  return launch_embedding(static_cast<hipStream_t>(stream), a);
+}
+
+int32_t ilgpu_hip_embedding_gradient_temp_bytes(int64_t count, int64_t vocabulary,
+                                                int64_t dimension, int64_t* temp_bytes) {
+  if (temp_bytes == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (count < 0 || vocabulary < 0 || dimension < 1) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  if (count > radix_sort_max_length() || vocabulary > INT32_MAX || dimension > INT32_MAX)
+    return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  *temp_bytes = embedding_gradient_temp_bytes(count, vocabulary, dimension);
+  return ILGPU_HIP_SUCCESS;
+}
+
+int32_t ilgpu_hip_embedding_gradient(
+    ilgpu_hip_stream_t stream, const void* grad_out, int64_t grad_out_stride,
+    int32_t grad_out_type, const void* tokens, int64_t count,
+    int32_t token_type, const float* scale, int64_t padding_token,
+    int32_t accumulate, void* grad_table, int64_t vocabulary,
+    int64_t dimension, int64_t grad_table_stride, int32_t grad_table_type,
+    void* temp, int64_t temp_bytes) {
+  const int gb = operator_elem_size(grad_out_type), wb = operator_elem_size(grad_table_type);
+  if (gb < 0 || wb < 0) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  int32_t rc = check_tokens(tokens, count, token_type);
+  if (rc == ILGPU_HIP_SUCCESS && count > radix_sort_max_length())
+    rc = ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  if (rc == ILGPU_HIP_SUCCESS)
+    rc = check_matrix(grad_out, count, dimension, grad_out_stride, gb, false);
+  if (rc == ILGPU_HIP_SUCCESS)
+    rc = check_matrix(grad_table, vocabulary, dimension, grad_table_stride, wb, true);
+  if (rc == ILGPU_HIP_SUCCESS)
+    rc = check_temp(temp, temp_bytes, embedding_gradient_temp_bytes(count, vocabulary, dimension));
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  const EmbeddingGradientArgs a{grad_out, grad_out_stride, grad_out_type, tokens, count,
+                                token_type, scale != nullptr ? *scale : 1.0f, padding_token,
+                                accumulate != 0 ? 1 : 0, grad_table, vocabulary, dimension,
+                                grad_table_stride, grad_table_type, temp};
+  return launch_embedding_gradient(static_cast<hipStream_t>(stream), a);
+}
+
+/* ---- layer norm ------------------------------------------------------------ */
+
+static int32_t check_norm_types(int32_t type, int32_t weight_type) {
+  if (operator_elem_size(type) < 0 || (weight_type != type && weight_type != ILGPU_HIP_F32))
+    return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  return ILGPU_HIP_SUCCESS;
+}
+
+int32_t ilgpu_hip_layer_norm(ilgpu_hip_stream_t stream, const void* in,
+                             int64_t rows, int64_t columns, int64_t in_stride,
+                             int32_t type, const void* weight,
+                             const void* bias, int32_t weight_type,
+                             const float* epsilon, void* out,
+                             int64_t out_stride, float* mean, float* rstd) {
+  int32_t rc = check_norm_types(type, weight_type);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  const int eb = operator_elem_size(type), wb = operator_elem_size(weight_type);
+  if (epsilon == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  rc = check_matrix(in, rows, columns, in_stride, eb, false);
+  if (rc == ILGPU_HIP_SUCCESS) rc = check_matrix(out, rows, columns, out_stride, eb, true);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  if (!(*epsilon >= 0.0f && *epsilon <= 3.402823466e+38f)) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  if (!aligned_to(weight, wb) || !aligned_to(bias, wb) || !aligned_to(mean, 4) ||
+      !aligned_to(rstd, 4))
+    return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  const LayerNormArgs a{in, rows, columns, in_stride, type, weight, bias, weight_type,
+                        *epsilon, out, out_stride, mean, rstd};
+  return launch_layer_norm(static_cast<hipStream_t>(stream), a);
+}
+
+int32_t ilgpu_hip_layer_norm_gradient_temp_bytes(int64_t rows, int64_t columns,
+                                                 int64_t* temp_bytes) {
+  if (temp_bytes == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (rows < 0 || columns < 1) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  if (rows > INT32_MAX || columns > INT32_MAX) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  *temp_bytes = layer_norm_gradient_temp_bytes(rows, columns);
+  return ILGPU_HIP_SUCCESS;
+}
+
+int32_t ilgpu_hip_layer_norm_gradient(
+    ilgpu_hip_stream_t stream, const void* grad_out, int64_t grad_out_stride,
+    const void* in, int64_t in_stride, int64_t rows, int64_t columns,
+    int32_t type, const void* weight, int32_t weight_type, const float* mean,
+    const float* rstd, void* grad_in, int64_t grad_in_stride,
+    void* grad_weight, void* grad_bias, int32_t accumulate, void* temp,
+    int64_t temp_bytes) {
+  int32_t rc = check_norm_types(type, weight_type);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  const int eb = operator_elem_size(type), wb = operator_elem_size(weight_type);
+  rc = check_matrix(grad_out, rows, columns, grad_out_stride, eb, false);
+  if (rc == ILGPU_HIP_SUCCESS) rc = check_matrix(in, rows, columns, in_stride, eb, false);
+  if (rc == ILGPU_HIP_SUCCESS && grad_in != nullptr)
+    rc = check_matrix(grad_in, rows, columns, grad_in_stride, eb, true);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  if (rows > 0 && (mean == nullptr || rstd == nullptr)) return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (rows > 0 && grad_in == nullptr && grad_weight == nullptr && grad_bias == nullptr)
+    return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (!aligned_to(weight, wb) || !aligned_to(grad_weight, wb) || !aligned_to(grad_bias, wb) ||
+      !aligned_to(mean, 4) || !aligned_to(rstd, 4))
+    return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  rc = check_temp(temp, temp_bytes, layer_norm_gradient_temp_bytes(rows, columns));
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  const LayerNormGradientArgs a{grad_out, grad_out_stride, in, in_stride, rows, columns, type,
+                                weight, weight_type, mean, rstd, grad_in, grad_in_stride,
+                                grad_weight, grad_bias, accumulate != 0 ? 1 : 0, temp};
+  return launch_layer_norm_gradient(static_cast<hipStream_t>(stream), a);
+}
+
+/* ---- gradient norm and clipping ---------------------------------------------- */
+
+int32_t ilgpu_hip_gradient_norm_temp_bytes(int64_t count, int64_t* temp_bytes) {
+  if (temp_bytes == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (count < 0) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  if (count > INT32_MAX) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  *temp_bytes = gradient_norm_temp_bytes(count);
+  return ILGPU_HIP_SUCCESS;
+}
+
+int32_t ilgpu_hip_gradient_norm(ilgpu_hip_stream_t stream,
+                                const ilgpu_hip_tensor* tensors, int64_t count,
+                                float* norm, void* temp, int64_t temp_bytes) {
+  int32_t rc = check_tensors(tensors, count);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  if (norm == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (!aligned_to(norm, 4)) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  rc = check_temp(temp, temp_bytes, gradient_norm_temp_bytes(count));
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  return launch_gradient_norm(static_cast<hipStream_t>(stream), tensors, count, norm, temp);
+}
+
+int32_t ilgpu_hip_clip_gradients(ilgpu_hip_stream_t stream,
+                                 const ilgpu_hip_tensor* sources,
+                                 const ilgpu_hip_tensor* targets, int64_t count,
+                                 const float* norm, const float* max_norm) {
+  int32_t rc = check_tensors(sources, count);
+  if (rc == ILGPU_HIP_SUCCESS && targets != nullptr) rc = check_tensors(targets, count);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  for (int64_t k = 0; targets != nullptr && k < count; ++k) {
+    if (targets[k].type != sources[k].type) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+    if (targets[k].length != sources[k].length) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  }
+  if (norm == nullptr || max_norm == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (!aligned_to(norm, 4)) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  if (!(*max_norm >= 0.0f)) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  return launch_clip_gradients(static_cast<hipStream_t>(stream), sources, targets, count, norm,
+                               *max_norm);
 }
 
 }  // extern "C"

@@ -91,6 +91,10 @@ ILGPU_TYPE_CODE(float, ILGPU_HIP_F32);   ILGPU_TYPE_CODE(double, ILGPU_HIP_F64);
 // IEEE binary16 carried as raw bits (System.Half / ILGPU.Half).
 struct Half { uint16_t bits; };
 template <> struct TypeCode<Half> { static constexpr int32_t value = ILGPU_HIP_F16; };
+// The upper half of a float, carried as raw bits; only the operators of language
+// models take it (the primitives throw NotSupportedException).
+struct BFloat16 { uint16_t bits; };
+template <> struct TypeCode<BFloat16> { static constexpr int32_t value = ILGPU_HIP_BF16; };
 
 // ---- strides and views -------------------------------------------------------
 namespace Stride1D {
@@ -149,6 +153,29 @@ template <typename T, typename TStride = Stride1D::Dense> class ArrayView1D {
   ArrayView<T> base_;
   int64_t extent_ = 0;
   TStride stride_{};
+};
+
+// Rows x columns elements of a view: element (r, c) is element r * rowStride + c of it
+// (a row stride of 0, one row for all, only where the matrix is read).
+template <typename T> class MatrixView {
+ public:
+  MatrixView() = default;
+  MatrixView(ArrayView<T> base, int64_t rows, int64_t columns, int64_t rowStride)
+      : base_(base), rows_(rows), columns_(columns), rowStride_(rowStride) {
+    if (rows < 0 || columns < 0 || rowStride < 0 ||
+        (rows > 0 && (columns > base.Length() ||
+                      (rowStride > 0 && rows - 1 > (base.Length() - columns) / rowStride))))
+      throw ArgumentOutOfRangeException("base");
+  }
+  MatrixView(ArrayView<T> base, int64_t rows, int64_t columns)
+      : MatrixView(base, rows, columns, columns) {}
+  int64_t Rows() const { return rows_; }
+  int64_t Columns() const { return columns_; }
+  int64_t RowStride() const { return rowStride_; }
+  T* LoadEffectiveAddressAsPtr() const { return base_.LoadEffectiveAddressAsPtr(); }
+ private:
+  ArrayView<T> base_;
+  int64_t rows_ = 0, columns_ = 0, rowStride_ = 0;
 };
 
 // ---- accelerator, stream, buffers ---------------------------------------------
@@ -1041,6 +1068,156 @@ void ReorderTransform(Accelerator& accelerator, AcceleratorStream& stream,
                       ArrayView<Index1D> reorderView, TTransformer transformer) {
   CreateReorderTransformer<TSource, TTarget, TTransformer>(accelerator)(
       stream, source, target, reorderView, transformer);
+}
+
+// ---- operators of language models (no counterpart in the reference) -------------------
+// The checks that the C ABI cannot make (it sees no view lengths); everything else is
+// checked there.
+inline void CheckLength(bool fits, const char* name) {
+  if (!fits) throw ArgumentOutOfRangeException(name);
+}
+
+// output[i] = scale * table[tokens[i]]; a token outside the table gives a row of zeros.
+template <typename T, typename TOutput, typename TToken>
+void Embedding(Accelerator&, AcceleratorStream& stream, MatrixView<T> table,
+               ArrayView<TToken> tokens, MatrixView<TOutput> output, float scale = 1.0f) {
+  CheckLength(output.Rows() == tokens.Length() && output.Columns() == table.Columns(), "output");
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_embedding(stream.StreamPtr(), table.LoadEffectiveAddressAsPtr(), table.Rows(),
+                          table.Columns(), table.RowStride(), TypeCode<T>::value,
+                          tokens.LoadEffectiveAddressAsPtr(), tokens.Length(),
+                          TypeCode<TToken>::value, &scale, output.LoadEffectiveAddressAsPtr(),
+                          output.RowStride(), TypeCode<TOutput>::value),
+      "table");
+}
+
+// In 32-bit ints.
+inline int64_t ComputeEmbeddingGradientTempStorageSize(Accelerator&, int64_t count,
+                                                       int64_t vocabulary, int64_t dimension) {
+  int64_t bytes = 0;
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_embedding_gradient_temp_bytes(count, vocabulary, dimension, &bytes), "count");
+  return (bytes + 3) / 4;
+}
+// gradTable[v] = scale * sum of gradOutput[i] over the positions i of token v, or, with
+// accumulate, added to what is there.
+template <typename TGrad, typename T, typename TToken>
+void EmbeddingGradient(Accelerator&, AcceleratorStream& stream, MatrixView<TGrad> gradOutput,
+                       ArrayView<TToken> tokens, MatrixView<T> gradTable, ArrayView<int32_t> temp,
+                       float scale = 1.0f, int64_t paddingToken = -1, bool accumulate = false) {
+  CheckLength(gradOutput.Rows() == tokens.Length(), "gradOutput");
+  CheckLength(gradOutput.Columns() == gradTable.Columns(), "gradTable");
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_embedding_gradient(
+          stream.StreamPtr(), gradOutput.LoadEffectiveAddressAsPtr(), gradOutput.RowStride(),
+          TypeCode<TGrad>::value, tokens.LoadEffectiveAddressAsPtr(), tokens.Length(),
+          TypeCode<TToken>::value, &scale, paddingToken, accumulate ? 1 : 0,
+          gradTable.LoadEffectiveAddressAsPtr(), gradTable.Rows(), gradTable.Columns(),
+          gradTable.RowStride(), TypeCode<T>::value, temp.LoadEffectiveAddressAsPtr(),
+          temp.Length() * 4),
+      "temp");
+}
+
+// Layer norm of every row.  weight, bias, mean and rstd may be views without a buffer:
+// 1, 0, not wanted.
+template <typename T, typename TWeight>
+void LayerNorm(Accelerator&, AcceleratorStream& stream, MatrixView<T> input, MatrixView<T> output,
+               ArrayView<TWeight> weight, ArrayView<TWeight> bias, float epsilon,
+               ArrayView<float> mean = {}, ArrayView<float> rstd = {}) {
+  CheckLength(output.Rows() == input.Rows() && output.Columns() == input.Columns(), "output");
+  CheckLength(!weight.IsValid() || weight.Length() == input.Columns(), "weight");
+  CheckLength(!bias.IsValid() || bias.Length() == input.Columns(), "bias");
+  CheckLength(!mean.IsValid() || mean.Length() >= input.Rows(), "mean");
+  CheckLength(!rstd.IsValid() || rstd.Length() >= input.Rows(), "rstd");
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_layer_norm(stream.StreamPtr(), input.LoadEffectiveAddressAsPtr(), input.Rows(),
+                           input.Columns(), input.RowStride(), TypeCode<T>::value,
+                           weight.LoadEffectiveAddressAsPtr(), bias.LoadEffectiveAddressAsPtr(),
+                           TypeCode<TWeight>::value, &epsilon,
+                           output.LoadEffectiveAddressAsPtr(), output.RowStride(),
+                           mean.LoadEffectiveAddressAsPtr(), rstd.LoadEffectiveAddressAsPtr()),
+      "input");
+}
+
+inline int64_t ComputeLayerNormGradientTempStorageSize(Accelerator&, int64_t rows,
+                                                       int64_t columns) {
+  int64_t bytes = 0;
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_layer_norm_gradient_temp_bytes(rows, columns, &bytes), "rows");
+  return (bytes + 3) / 4;
+}
+// Its gradients; gradInput, gradWeight and gradBias may be views without a buffer: not
+// wanted.
+template <typename T, typename TWeight>
+void LayerNormGradient(Accelerator&, AcceleratorStream& stream, MatrixView<T> gradOutput,
+                       MatrixView<T> input, ArrayView<TWeight> weight, ArrayView<float> mean,
+                       ArrayView<float> rstd, MatrixView<T> gradInput,
+                       ArrayView<TWeight> gradWeight, ArrayView<TWeight> gradBias,
+                       ArrayView<int32_t> temp, bool accumulate = false) {
+  CheckLength(gradOutput.Rows() == input.Rows() && gradOutput.Columns() == input.Columns(),
+              "gradOutput");
+  CheckLength(gradInput.LoadEffectiveAddressAsPtr() == nullptr ||
+                  (gradInput.Rows() == input.Rows() && gradInput.Columns() == input.Columns()),
+              "gradInput");
+  CheckLength(!weight.IsValid() || weight.Length() == input.Columns(), "weight");
+  CheckLength(!gradWeight.IsValid() || gradWeight.Length() == input.Columns(), "gradWeight");
+  CheckLength(!gradBias.IsValid() || gradBias.Length() == input.Columns(), "gradBias");
+  CheckLength(mean.Length() >= input.Rows(), "mean");
+  CheckLength(rstd.Length() >= input.Rows(), "rstd");
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_layer_norm_gradient(
+          stream.StreamPtr(), gradOutput.LoadEffectiveAddressAsPtr(), gradOutput.RowStride(),
+          input.LoadEffectiveAddressAsPtr(), input.RowStride(), input.Rows(), input.Columns(),
+          TypeCode<T>::value, weight.LoadEffectiveAddressAsPtr(), TypeCode<TWeight>::value,
+          mean.LoadEffectiveAddressAsPtr(), rstd.LoadEffectiveAddressAsPtr(),
+          gradInput.LoadEffectiveAddressAsPtr(), gradInput.RowStride(),
+          gradWeight.LoadEffectiveAddressAsPtr(), gradBias.LoadEffectiveAddressAsPtr(),
+          accumulate ? 1 : 0, temp.LoadEffectiveAddressAsPtr(), temp.Length() * 4),
+      "temp");
+}
+
+// A list of views of any of the three types for the calls over many tensors.
+class TensorList {
+ public:
+  template <typename T> void Add(ArrayView<T> view) {
+    tensors_.push_back({view.LoadEffectiveAddressAsPtr(), view.Length(), TypeCode<T>::value, 0});
+  }
+  int64_t Count() const { return (int64_t)tensors_.size(); }
+  const ilgpu_hip_tensor* Data() const { return tensors_.data(); }
+ private:
+  std::vector<ilgpu_hip_tensor> tensors_;
+};
+
+inline int64_t ComputeGradientNormTempStorageSize(Accelerator&, int64_t count) {
+  int64_t bytes = 0;
+  HipAlgorithmsException::ThrowIfFailed(ilgpu_hip_gradient_norm_temp_bytes(count, &bytes),
+                                        "count");
+  return (bytes + 3) / 4;
+}
+// norm[0] = the root of the sum of the squares of all elements.
+inline void GradientNorm(Accelerator&, AcceleratorStream& stream, const TensorList& gradients,
+                         ArrayView<float> norm, ArrayView<int32_t> temp) {
+  if (!norm.IsValid()) throw ArgumentNullException("norm");
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_gradient_norm(stream.StreamPtr(), gradients.Data(), gradients.Count(),
+                              norm.LoadEffectiveAddressAsPtr(), temp.LoadEffectiveAddressAsPtr(),
+                              temp.Length() * 4),
+      "temp");
+}
+// gradients *= maxNorm / norm[0] where that is finite and norm[0] the larger, in place or
+// into targets.
+inline void ClipGradients(Accelerator&, AcceleratorStream& stream, const TensorList& gradients,
+                          const TensorList& targets, ArrayView<float> norm, float maxNorm) {
+  CheckLength(targets.Count() == gradients.Count(), "targets");
+  if (!norm.IsValid()) throw ArgumentNullException("norm");
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_clip_gradients(stream.StreamPtr(), gradients.Data(), targets.Data(),
+                               gradients.Count(), norm.LoadEffectiveAddressAsPtr(), &maxNorm),
+      "gradients");
+}
+inline void ClipGradients(Accelerator& accelerator, AcceleratorStream& stream,
+                          const TensorList& gradients, ArrayView<float> norm, float maxNorm) {
+  ClipGradients(accelerator, stream, gradients, gradients, norm, maxNorm);
 }
 
 }  // namespace Algorithms

@@ -3,10 +3,11 @@
  *
  * Hand-written gfx950 (MI355X, CDNA4) implementation of the data-parallel
  * primitives of ILGPU.Algorithms: radix sort (keys, key/value pairs), inclusive
- * and exclusive scan, reduction and histogram.  The entry points below are
- * what a P/Invoke layer behind ILGPU's existing C# surface binds; each one
- * names the reference interface it stands in for (paths relative to the ILGPU
- * source tree).
+ * and exclusive scan, reduction and histogram; and operators of language models
+ * built beside them (embedding, layer norm, gradient norm and clipping).  The
+ * entry points below are what a P/Invoke layer behind ILGPU's existing C#
+ * surface binds; each primitive names the reference interface it stands in for
+ * (paths relative to the ILGPU source tree).
  *
  * Conventions
  *  - Every pointer named keys/values/in/out/bins/overflow/temp is a DEVICE
@@ -60,11 +61,14 @@ typedef enum ilgpu_hip_status {
                                          scratch serves (ilgpu_hip_scan_static) */
 } ilgpu_hip_status;
 
-/* Element types: NumericTypes of TypeInformation.ttinclude:94-121. */
+/* Element types: NumericTypes of TypeInformation.ttinclude:94-121.  BF16 (the
+ * upper half of a float32) has no counterpart there; only the operators at the
+ * end of this header take it, the primitives answer NOT_SUPPORTED. */
 typedef enum ilgpu_hip_type {
   ILGPU_HIP_I8 = 0, ILGPU_HIP_I16 = 1, ILGPU_HIP_I32 = 2, ILGPU_HIP_I64 = 3,
   ILGPU_HIP_U8 = 4, ILGPU_HIP_U16 = 5, ILGPU_HIP_U32 = 6, ILGPU_HIP_U64 = 7,
-  ILGPU_HIP_F16 = 8, ILGPU_HIP_F32 = 9, ILGPU_HIP_F64 = 10
+  ILGPU_HIP_F16 = 8, ILGPU_HIP_F32 = 9, ILGPU_HIP_F64 = 10,
+  ILGPU_HIP_BF16 = 11
 } ilgpu_hip_type;
 
 /* Scan/reduce functors: Add/Max/Min of ScanReduceOperations.tt:20-27. */
@@ -427,6 +431,120 @@ int32_t ilgpu_hip_reorder_transform(ilgpu_hip_stream_t stream,
                                     int64_t target_length, int32_t target_type,
                                     const int32_t *order, int64_t order_length,
                                     int32_t transformer, int64_t factor);
+
+/* ---- operators of language models -------------------------------------------
+ * No counterpart in the reference.  They follow the conventions above, and:
+ *  - A matrix is given by its first element, its rows and columns and its row
+ *    stride in elements; element (r, c) is at base[r * row_stride + c].  The
+ *    row stride of a matrix that is read may be anything from 0 (one row for
+ *    all); that of a matrix that is written is at least its columns
+ *    (ILGPU_HIP_ERROR_OUT_OF_RANGE otherwise).  Any element-aligned base and any
+ *    stride will do; rows need no alignment of their own.
+ *  - Types are ILGPU_HIP_F32, F16 and BF16 (others: ILGPU_HIP_ERROR_NOT_SUPPORTED).
+ *    All arithmetic is in float32 or wider; each result is rounded to its type
+ *    once, to nearest even.
+ *  - No rows, no tokens, no tensors are valid inputs: the call does what the
+ *    formula says for an empty sum.  A null pointer is ILGPU_HIP_ERROR_NULL_VIEW
+ *    where there is something to read or write; zero columns always are.
+ *  - Single numbers (scale, epsilon, max_norm) are HOST pointers, read before
+ *    the call returns.
+ *  - Results do not depend on the order in which blocks run: the same call on
+ *    the same inputs gives the same bits.
+ */
+
+/* Embedding: out[i] = scale * table[tokens[i]] for every i < count, rows of
+ * `dimension` elements.  tokens: int32 or int64 (token_type).  A token outside
+ * [0, vocabulary) gives a row of zeros and is never used as an address.
+ * scale: NULL means 1.  Any of the three types for the table and for out. */
+int32_t ilgpu_hip_embedding(ilgpu_hip_stream_t stream, const void *table,
+                            int64_t vocabulary, int64_t dimension,
+                            int64_t table_stride, int32_t table_type,
+                            const void *tokens, int64_t count,
+                            int32_t token_type, const float *scale, void *out,
+                            int64_t out_stride, int32_t out_type);
+
+/* Its gradient: grad_table[v] (+)= scale * sum of grad_out[i] over the positions
+ * i with tokens[i] == v, added up in float32.  Every row of
+ * grad_table is written, with zeros where no position has its token; with
+ * accumulate != 0 the sums are added to what is there instead, and other rows
+ * are left alone.  Tokens outside [0, vocabulary) and padding_token (pass -1
+ * for none) contribute nothing.  grad_table must not overlap grad_out or
+ * tokens.  On a device whose LDS fails ilgpu_hip_sort_check_device:
+ * ILGPU_HIP_ERROR_NOT_SUPPORTED, like a sort. */
+int32_t ilgpu_hip_embedding_gradient_temp_bytes(int64_t count,
+                                                int64_t vocabulary,
+                                                int64_t dimension,
+                                                int64_t *temp_bytes);
+int32_t ilgpu_hip_embedding_gradient(
+    ilgpu_hip_stream_t stream, const void *grad_out, int64_t grad_out_stride,
+    int32_t grad_out_type, const void *tokens, int64_t count,
+    int32_t token_type, const float *scale, int64_t padding_token,
+    int32_t accumulate, void *grad_table, int64_t vocabulary,
+    int64_t dimension, int64_t grad_table_stride, int32_t grad_table_type,
+    void *temp, int64_t temp_bytes);
+
+/* Layer norm of every row: out = (in - m) * r * weight + bias with m the row's
+ * mean, r = 1 / sqrt(v + epsilon) and v the mean of (in - m)^2.  weight and bias
+ * (`columns` elements of weight_type, which is `type` or F32) may be NULL: 1 and
+ * 0.  mean and rstd (float32, one per row) receive m and r and may be NULL.
+ * in and out have the same type; out may be in itself (same base and stride).
+ * epsilon: finite and not negative. */
+int32_t ilgpu_hip_layer_norm(ilgpu_hip_stream_t stream, const void *in,
+                             int64_t rows, int64_t columns, int64_t in_stride,
+                             int32_t type, const void *weight,
+                             const void *bias, int32_t weight_type,
+                             const float *epsilon, void *out,
+                             int64_t out_stride, float *mean, float *rstd);
+
+/* Its gradients from mean and rstd as the forward call left them: with
+ * h = (in - mean) * rstd and g = weight * grad_out,
+ *   grad_in     = rstd * (g - mean of g - h * mean of g * h)   (means over the row)
+ *   grad_weight = sum over the rows of grad_out * h
+ *   grad_bias   = sum over the rows of grad_out
+ * weight may be NULL (1).  Each of grad_in, grad_weight and grad_bias may be NULL
+ * and is not computed then; not all of them.  grad_in may be grad_out itself or in
+ * itself (same base and stride).  With accumulate != 0 grad_weight and grad_bias
+ * are added to what is there.  No rows leave sums of zero. */
+int32_t ilgpu_hip_layer_norm_gradient_temp_bytes(int64_t rows, int64_t columns,
+                                                 int64_t *temp_bytes);
+int32_t ilgpu_hip_layer_norm_gradient(
+    ilgpu_hip_stream_t stream, const void *grad_out, int64_t grad_out_stride,
+    const void *in, int64_t in_stride, int64_t rows, int64_t columns,
+    int32_t type, const void *weight, int32_t weight_type, const float *mean,
+    const float *rstd, void *grad_in, int64_t grad_in_stride,
+    void *grad_weight, void *grad_bias, int32_t accumulate, void *temp,
+    int64_t temp_bytes);
+
+/* One array of a list: `length` dense elements of `type` at `data`.  The list
+ * itself is HOST memory, read before the call returns. */
+typedef struct ilgpu_hip_tensor {
+  void *data;
+  int64_t length;
+  int32_t type;
+  int32_t reserved; /* 0 */
+} ilgpu_hip_tensor;
+
+/* norm[0] = the root of the sum of the squares of all elements of all tensors,
+ * added up in float64.  At most 2^40 elements and INT32_MAX tensors (beyond:
+ * ILGPU_HIP_ERROR_NOT_SUPPORTED); tensors of length 0 are skipped. */
+int32_t ilgpu_hip_gradient_norm_temp_bytes(int64_t count, int64_t *temp_bytes);
+int32_t ilgpu_hip_gradient_norm(ilgpu_hip_stream_t stream,
+                                const ilgpu_hip_tensor *tensors, int64_t count,
+                                float *norm, void *temp, int64_t temp_bytes);
+
+/* targets[k] = factor * sources[k], element for element, with
+ * factor = max_norm / norm[0] where norm[0] is finite and larger than max_norm,
+ * 1 otherwise: an infinite or NaN norm leaves the values as they are, and norm[0]
+ * tells.  norm is DEVICE memory (ilgpu_hip_gradient_norm's, or combined over
+ * processes); nothing waits for it on the host.  targets[k] has the length and
+ * type of sources[k] and is the same array or does not overlap any source; targets
+ * NULL: in place.  Tensors that a factor of 1 leaves as they are in place are not
+ * touched.  max_norm: not negative, not NaN. */
+int32_t ilgpu_hip_clip_gradients(ilgpu_hip_stream_t stream,
+                                 const ilgpu_hip_tensor *sources,
+                                 const ilgpu_hip_tensor *targets,
+                                 int64_t count, const float *norm,
+                                 const float *max_norm);
 
 #ifdef __cplusplus
 }
