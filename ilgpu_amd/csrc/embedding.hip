@@ -73,9 +73,154 @@ __global__ __launch_bounds__(kBlock) void token_keys_kernel(
   }
 }
 
+// The same order for a moderate number of tokens in one launch instead of a sort's
+// several: block g of `1 << log2` gathers the positions of the tokens that are g modulo
+// the number of blocks.  Every block reads all tokens (from its XCD's L2) and counts
+// those of the blocks before it, so it knows where its own begin without a word from
+// them.  Sixteen waves take a stretch of the input each, and count their tokens by
+// (wave, token); the counts' prefix sums are the places.  Lanes of one LDS atomic are
+// served in lane order (check_sort_device), so the order is the same in every call; it is
+// not that of the positions, which no sum needs.
+constexpr int kGroupBlock = 1024;
+constexpr int kGroupWaves = kGroupBlock / kWaveSize;
+constexpr int kGroupMinLog2 = 8;          // blocks: one per compute unit
+constexpr int kGroupMaxLog2 = 10;
+constexpr int kGroupRows = 1024;          // most tokens a block gathers
+constexpr int kGroupList = 512;           // positions a wave remembers; beyond it reads again
+constexpr int64_t kGroupMaxCount = 1 << 18;
+
+inline int group_log2(int64_t vocabulary) {
+  int log2 = kGroupMinLog2;
+  while (log2 < kGroupMaxLog2 && ((int64_t)kGroupRows << log2) < vocabulary) ++log2;
+  return log2;
+}
+inline bool takes_groups(int64_t count, int64_t vocabulary) {
+  return count <= kGroupMaxCount && vocabulary <= ((int64_t)kGroupRows << kGroupMaxLog2);
+}
+
+template <typename TT>
+__global__ __launch_bounds__(kGroupBlock) void group_tokens_kernel(
+    const TT* __restrict__ tokens, int64_t count, int64_t vocabulary, int64_t padding_token,
+    int log2, int rows, uint32_t* __restrict__ keys, uint32_t* __restrict__ order,
+    uint64_t* __restrict__ met, uint32_t* __restrict__ crossings) {
+  extern __shared__ uint32_t group_lds[];
+  __shared__ uint32_t wave_rows[kGroupWaves], wave_below[kGroupWaves];
+  const uint32_t group = blockIdx.x, groups = gridDim.x;
+  const int wave = threadIdx.x / kWaveSize, lane = threadIdx.x & (kWaveSize - 1);
+  uint32_t* const counters = group_lds + wave * rows;
+  uint32_t* const list = group_lds + kGroupWaves * rows + wave * kGroupList;
+  if (group == 0 && threadIdx.x == 0) crossings[0] = 0;
+  for (int i = threadIdx.x; i < kGroupWaves * rows; i += kGroupBlock) group_lds[i] = 0;
+  __syncthreads();
+
+  constexpr int V = 4, U = 4;  // tokens a load, loads in flight
+  constexpr int64_t kStep = (int64_t)kWaveSize * V * U;
+  const int64_t stretch = (count + kGroupWaves * kStep - 1) / (kGroupWaves * kStep) * kStep;
+  const int64_t begin = wave * stretch;
+  const int64_t end = begin + stretch < count ? begin + stretch : count;
+  uint32_t below = 0, listed = 0;
+
+  // Calls f(position, token, own) for every position of the stretch, 64 lanes at a time.
+  auto scan = [&](auto f) {
+    for (int64_t base = begin; base < end; base += kStep) {
+      TT t[U][V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = base + (u * kWaveSize + lane) * V;
+        if (at + V <= end) {
+          const auto r = *reinterpret_cast<const typename Pack<TT, V>::type*>(tokens + at);
+#pragma unroll
+          for (int k = 0; k < V; ++k) t[u][k] = r[k];
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; ++k) t[u][k] = at + k < end ? tokens[at + k] : (TT)-1;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const int64_t token = (int64_t)t[u][k];
+          f((uint32_t)(base + (u * kWaveSize + lane) * V + k), (uint32_t)token,
+            (uint64_t)token < (uint64_t)vocabulary && token != padding_token);
+        }
+    }
+  };
+
+  scan([&](uint32_t at, uint32_t token, bool counts) {
+    const uint32_t of = token & (groups - 1);
+    below += counts && of < group ? 1 : 0;
+    const bool own = counts && of == group;
+    const uint64_t owns = __ballot(own);
+    if (owns != 0) {
+      if (own) {
+        atomicAdd(&counters[token >> log2], 1u);
+        const uint32_t place = listed + mbcnt(owns);
+        if (place < kGroupList) list[place] = at;
+      }
+      listed += __popcll(owns);
+    }
+  });
+  for (int off = kWaveSize / 2; off > 0; off >>= 1) below += __shfl_xor(below, off, kWaveSize);
+  if (lane == 0) wave_below[wave] = below;
+  __syncthreads();
+
+  // Places: by token, then by wave.
+  uint32_t total = 0;
+  if ((int)threadIdx.x < rows) {
+    for (int w = 0; w < kGroupWaves; ++w) total += group_lds[w * rows + threadIdx.x];
+  }
+  const uint64_t any = __ballot(total > 0);
+  if (lane == 0 && wave * kWaveSize < rows) met[(int64_t)wave * groups + group] = any;
+  uint32_t before = total;
+  for (int off = 1; off < kWaveSize; off <<= 1) {
+    const uint32_t other = __shfl_up(before, off, kWaveSize);
+    if (lane >= off) before += other;
+  }
+  if (lane == kWaveSize - 1) wave_rows[wave] = before;
+  __syncthreads();
+  uint32_t place = before - total, all_own = 0, all_below = 0;
+  for (int w = 0; w < kGroupWaves; ++w) {
+    if (w < wave) place += wave_rows[w];
+    all_own += wave_rows[w];
+    all_below += wave_below[w];
+  }
+  place += all_below;
+  if ((int)threadIdx.x < rows) {
+    for (int w = 0; w < kGroupWaves; ++w) {
+      const uint32_t here = group_lds[w * rows + threadIdx.x];
+      group_lds[w * rows + threadIdx.x] = place;
+      place += here;
+    }
+  }
+  __syncthreads();
+
+  if (listed <= kGroupList) {
+    for (uint32_t j = lane; j < listed; j += kWaveSize) {
+      const uint32_t at = list[j], token = (uint32_t)tokens[at];
+      const uint32_t to = atomicAdd(&counters[token >> log2], 1u);
+      keys[to] = token;
+      order[to] = at;
+    }
+  } else {
+    scan([&](uint32_t at, uint32_t token, bool counts) {
+      if (counts && (token & (groups - 1)) == group) {
+        const uint32_t to = atomicAdd(&counters[token >> log2], 1u);
+        keys[to] = token;
+        order[to] = at;
+      }
+    });
+  }
+  if (group == groups - 1)
+    for (int64_t i = (int64_t)all_below + all_own + threadIdx.x; i < count; i += kGroupBlock)
+      keys[i] = (uint32_t)vocabulary;
+}
+
 struct Sums {
   const uint32_t* keys;
   const uint32_t* order;
+  const uint64_t* met;   // bit (v >> group_log2) & 63 of word (v >> group_log2 >> 6, v modulo the
+  int group_log2;        // groups): row v has a token; nullptr where the keys are sorted
   uint32_t* crossings;   // [0]: their number; then the chunks in which a run begins that
                          // goes on into the next
   float* parts;          // per chunk the part of a run from before it, then as many of
@@ -105,22 +250,26 @@ __device__ __forceinline__ void finish_row(TW* to, float (&sum)[W], int64_t colu
 
 constexpr int kClearRows = 16;  // per block
 
-// Whether a row has a token: its key is among the sorted ones.
-__device__ __forceinline__ bool is_met(const uint32_t* keys, int64_t count, int64_t row) {
-  int64_t low = 0, high = count;
+// Whether a row has a token: by its bit, or its key is among the sorted ones.
+__device__ __forceinline__ bool is_met(const Sums& s, int64_t row) {
+  if (s.met != nullptr) {
+    const uint32_t of = (uint32_t)row & ((1u << s.group_log2) - 1), local = (uint32_t)(row >> s.group_log2);
+    return (s.met[((uint64_t)(local >> 6) << s.group_log2) + of] >> (local & 63)) & 1;
+  }
+  int64_t low = 0, high = s.count;
   while (low < high) {
     const int64_t middle = (low + high) >> 1;
-    if ((int64_t)keys[middle] < row) low = middle + 1;
+    if ((int64_t)s.keys[middle] < row) low = middle + 1;
     else high = middle;
   }
-  return low < count && (int64_t)keys[low] == row;
+  return low < s.count && (int64_t)s.keys[low] == row;
 }
 
 template <typename TW>
 __device__ __forceinline__ void clear_rows(const Sums& s, TW* __restrict__ table, int64_t first) {
   constexpr int W = 16 / sizeof(TW);
   const int64_t mine = first + (threadIdx.x & (kClearRows - 1));
-  const bool met = mine >= s.vocabulary || is_met(s.keys, s.count, mine);
+  const bool met = mine >= s.vocabulary || is_met(s, mine);
   uint32_t unmet = ~(uint32_t)__ballot(met) & ((1u << kClearRows) - 1);
   float zeros[W];
 #pragma unroll
@@ -259,19 +408,24 @@ __global__ __launch_bounds__(kJoinBlock) void join_runs_kernel(Sums s, TW* __res
 }
 
 struct GradientTemp {
-  int64_t keys, order, crossings, parts, sort, bytes;  // offsets
+  int64_t keys, order, met, crossings, parts, sort, bytes;  // offsets
   int64_t chunks, part_stride;
 };
-GradientTemp gradient_temp(int64_t count, int64_t dimension) {
+GradientTemp gradient_temp(int64_t count, int64_t vocabulary, int64_t dimension) {
   GradientTemp t;
+  const bool groups = takes_groups(count, vocabulary);
   t.chunks = div_up(count, kChunk);
   t.part_stride = align_up(dimension, 8);
   t.keys = 0;
   t.order = align_up(count * 4, 256);
-  t.crossings = t.order + align_up(count * 4, 256);
+  t.met = t.order + align_up(count * 4, 256);
+  t.crossings =
+      t.met + (groups ? (div_up(vocabulary, (int64_t)64 << group_log2(vocabulary)) * 8)
+                            << group_log2(vocabulary)
+                      : 0);
   t.parts = t.crossings + align_up((t.chunks + 1) * 4, 256);
   t.sort = t.parts + align_up(2 * t.chunks * t.part_stride * 4, 256);
-  t.bytes = t.sort + (count > 0 ? radix_sort_temp_bytes(count, 4, 4) : 0) + 256;
+  t.bytes = t.sort + (count > 0 && !groups ? radix_sort_temp_bytes(count, 4, 4) : 0) + 256;
   return t;
 }
 
@@ -301,8 +455,8 @@ int32_t launch_embedding(hipStream_t stream, const EmbeddingArgs& a) {
   });
 }
 
-int64_t embedding_gradient_temp_bytes(int64_t count, int64_t, int64_t dimension) {
-  return gradient_temp(count, dimension).bytes;
+int64_t embedding_gradient_temp_bytes(int64_t count, int64_t vocabulary, int64_t dimension) {
+  return gradient_temp(count, vocabulary, dimension).bytes;
 }
 
 int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArgs& a) {
@@ -311,12 +465,30 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
     const int32_t rc = check_sort_device(stream);  // before anything is launched
     if (rc != ILGPU_HIP_SUCCESS) return rc;
   }
-  const GradientTemp t = gradient_temp(a.count, a.dimension);
+  const GradientTemp t = gradient_temp(a.count, a.vocabulary, a.dimension);
   char* base = reinterpret_cast<char*>(align_up((int64_t)(uintptr_t)a.temp, 256));
   uint32_t* keys = reinterpret_cast<uint32_t*>(base + t.keys);
   uint32_t* order = reinterpret_cast<uint32_t*>(base + t.order);
   uint32_t* crossings = reinterpret_cast<uint32_t*>(base + t.crossings);
-  if (a.count > 0) {
+  const bool groups = a.count > 0 && takes_groups(a.count, a.vocabulary);
+  if (groups) {
+    const int32_t rc = with_token_type(a.token_type, [&](auto tt) -> int32_t {
+      using TT = decltype(tt);
+      const int log2 = group_log2(a.vocabulary);
+      const int rows = (int)div_up(a.vocabulary, (int64_t)1 << log2);
+      {
+        ProfileScope scope(stream, "embedding_group_tokens");
+        hipLaunchKernelGGL((group_tokens_kernel<TT>), dim3(1u << log2), dim3(kGroupBlock),
+                           (unsigned)(kGroupWaves * (rows + kGroupList) * 4), stream,
+                           static_cast<const TT*>(a.tokens), a.count, a.vocabulary,
+                           a.padding_token, log2, rows, keys, order,
+                           reinterpret_cast<uint64_t*>(base + t.met), crossings);
+      }
+      ILGPU_HIP_CHECK(hipGetLastError());
+      return ILGPU_HIP_SUCCESS;
+    });
+    if (rc != ILGPU_HIP_SUCCESS) return rc;
+  } else if (a.count > 0) {
     const int32_t rc = with_token_type(a.token_type, [&](auto tt) -> int32_t {
       using TT = decltype(tt);
       const int64_t blocks = div_up(a.count, kBlock);
@@ -351,7 +523,9 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
       const int64_t sum_blocks = div_up(t.chunks * slices, kBlock >> log2);
       int64_t clear_blocks = a.accumulate ? 0 : div_up(a.vocabulary, kClearRows);
       if (clear_blocks > kMaxBlocks) clear_blocks = kMaxBlocks;
-      const Sums s{keys, order, crossings, reinterpret_cast<float*>(base + t.parts), a.count,
+      const Sums s{keys, order,
+                   groups ? reinterpret_cast<const uint64_t*>(base + t.met) : nullptr,
+                   group_log2(a.vocabulary), crossings, reinterpret_cast<float*>(base + t.parts), a.count,
                    t.chunks, t.part_stride, a.vocabulary, a.dimension, a.grad_out_stride,
                    a.table_stride, a.scale, a.accumulate, (uint32_t)sum_blocks,
                    (uint32_t)clear_blocks, (uint32_t)slices, (uint32_t)join_slices, log2};
