@@ -54,20 +54,24 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(
 // (keys: their tokens, order: the positions; positions that count nowhere come last
 // under the key `vocabulary`).  Chunks of kChunk positions of that order are added up
 // by a wave each, whatever tokens they hold, so a token that fills half of the input
-// takes no longer than the rest: a run of one token inside a chunk goes straight into
-// the table, the parts of a run that crosses chunks go into `parts` and are joined by
-// a second kernel.  Rows of no token are cleared by further blocks of the first.
-constexpr int kChunk = 32;
+// takes no longer than the rest: a run of one token goes straight into the table where
+// it ends before the next chunk does, parts of longer ones go into `parts` and are joined
+// by a second kernel.  Rows of no token are cleared by further blocks of both.
+constexpr int kChunk = 32, kShortChunk = 8;
+// Few and narrow rows fill the chip only in short chunks.
+inline int chunk_length(int64_t count, int64_t dimension) {
+  return div_up(count, kChunk) * div_up(dimension, 256) < 1024 ? kShortChunk : kChunk;
+}
 
 // Sort keys of the positions: their tokens, `vocabulary` for those that count nowhere.
 template <typename TT>
 __global__ __launch_bounds__(kBlock) void token_keys_kernel(
-    const TT* __restrict__ tokens, int64_t count, int64_t vocabulary, int64_t padding_token,
-    uint32_t* __restrict__ keys, uint32_t* __restrict__ crossings) {
+    const TT* __restrict__ tokens, int64_t count, int64_t padded, int64_t vocabulary,
+    int64_t padding_token, uint32_t* __restrict__ keys, uint32_t* __restrict__ crossings) {
   if (blockIdx.x == 0 && threadIdx.x == 0) crossings[0] = 0;
-  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < count;
+  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < padded;
        i += (int64_t)gridDim.x * kBlock) {
-    const int64_t token = (int64_t)tokens[i];
+    const int64_t token = i < count ? (int64_t)tokens[i] : -1;
     const bool counts = (uint64_t)token < (uint64_t)vocabulary && token != padding_token;
     keys[i] = (uint32_t)(counts ? token : vocabulary);
   }
@@ -77,32 +81,41 @@ __global__ __launch_bounds__(kBlock) void token_keys_kernel(
 // several: block g of `1 << log2` gathers the positions of the tokens that are g modulo
 // the number of blocks.  Every block reads all tokens (from its XCD's L2) and counts
 // those of the blocks before it, so it knows where its own begin without a word from
-// them.  Sixteen waves take a stretch of the input each, and count their tokens by
-// (wave, token); the counts' prefix sums are the places.  Lanes of one LDS atomic are
-// served in lane order (check_sort_device), so the order is the same in every call; it is
-// not that of the positions, which no sum needs.
+// them.  Sixteen waves take a stretch of the input each, keep the positions of their tokens
+// and count them by (wave, token); the counts' prefix sums are the places.  Lanes of one LDS
+// atomic are served in lane order (check_sort_device), so the order is the same in every
+// call; it is not that of the positions, which no sum needs.  Bound by the vector units
+// (some ten operations a token in every block): 65536 tokens 10 us, 16 where one token is 6 %
+// of them and its block counts and places 3800.
 constexpr int kGroupBlock = 1024;
 constexpr int kGroupWaves = kGroupBlock / kWaveSize;
 constexpr int kGroupMinLog2 = 8;          // blocks: one per compute unit
 constexpr int kGroupMaxLog2 = 10;
 constexpr int kGroupRows = 1024;          // most tokens a block gathers
-constexpr int kGroupList = 512;           // positions a wave remembers; beyond it reads again
-constexpr int64_t kGroupMaxCount = 1 << 18;
+constexpr int kGroupList = 1024;          // places a wave remembers; beyond it reads again
+constexpr int kGroupCountLog2 = 17;       // most tokens in all: place and row share a word
+static_assert(((uint64_t)kGroupRows << kGroupCountLog2) <= (1ull << 32), "a word");
 
 inline int group_log2(int64_t vocabulary) {
   int log2 = kGroupMinLog2;
   while (log2 < kGroupMaxLog2 && ((int64_t)kGroupRows << log2) < vocabulary) ++log2;
   return log2;
 }
+// Each block reads all tokens: with 256 blocks (up to 2^18 table rows) ahead of the sort up
+// to 2^17 tokens, with more blocks up to as much fewer.  (Whole gradient into 131072 x 64, us,
+// groups / sort: 8192 tokens 23 / 53, 32768 39 / 88, 131072 65 / 102, of 1000 rows 67 / 70; 2^18
+// tokens, which overflow the waves' lists, 162 / 116.)
 inline bool takes_groups(int64_t count, int64_t vocabulary) {
-  return count <= kGroupMaxCount && vocabulary <= ((int64_t)kGroupRows << kGroupMaxLog2);
+  const int log2 = group_log2(vocabulary);
+  return vocabulary <= ((int64_t)kGroupRows << log2) &&
+         count <= ((int64_t)1 << (kGroupCountLog2 + kGroupMinLog2 - log2));
 }
 
 template <typename TT>
 __global__ __launch_bounds__(kGroupBlock) void group_tokens_kernel(
-    const TT* __restrict__ tokens, int64_t count, int64_t vocabulary, int64_t padding_token,
-    int log2, int rows, uint32_t* __restrict__ keys, uint32_t* __restrict__ order,
-    uint64_t* __restrict__ met, uint32_t* __restrict__ crossings) {
+    const TT* __restrict__ tokens, int64_t count, int64_t padded, int64_t vocabulary,
+    int64_t padding_token, int log2, int rows, uint32_t* __restrict__ keys,
+    uint32_t* __restrict__ order, uint64_t* __restrict__ met, uint32_t* __restrict__ crossings) {
   extern __shared__ uint32_t group_lds[];
   __shared__ uint32_t wave_rows[kGroupWaves], wave_below[kGroupWaves];
   const uint32_t group = blockIdx.x, groups = gridDim.x;
@@ -118,50 +131,73 @@ __global__ __launch_bounds__(kGroupBlock) void group_tokens_kernel(
   const int64_t stretch = (count + kGroupWaves * kStep - 1) / (kGroupWaves * kStep) * kStep;
   const int64_t begin = wave * stretch;
   const int64_t end = begin + stretch < count ? begin + stretch : count;
+  const uint32_t limit = (uint32_t)vocabulary, mask = groups - 1;
+  // (A padding token outside the table is none.)
+  const uint32_t padding = (uint64_t)padding_token < (uint64_t)vocabulary ? (uint32_t)padding_token
+                                                                          : 0xffffffffu;
   uint32_t below = 0, listed = 0;
 
-  // Calls f(position, token, own) for every position of the stretch, 64 lanes at a time.
-  auto scan = [&](auto f) {
+  // Calls f(position, token, its block or none) for every position of the stretch, 64 lanes
+  // at a time.
+  const auto scan = [&](auto f) {
     for (int64_t base = begin; base < end; base += kStep) {
       TT t[U][V];
+      const TT* from = tokens + base + lane * V;
+      if (base + kStep <= end) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t at = base + (u * kWaveSize + lane) * V;
-        if (at + V <= end) {
-          const auto r = *reinterpret_cast<const typename Pack<TT, V>::type*>(tokens + at);
+        for (int u = 0; u < U; ++u) {
+          const auto r = *reinterpret_cast<const typename Pack<TT, V>::type*>(from + u * kWaveSize * V);
 #pragma unroll
           for (int k = 0; k < V; ++k) t[u][k] = r[k];
-        } else {
-#pragma unroll
-          for (int k = 0; k < V; ++k) t[u][k] = at + k < end ? tokens[at + k] : (TT)-1;
         }
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            t[u][k] = base + (u * kWaveSize + lane) * V + k < end ? from[u * kWaveSize * V + k] : (TT)-1;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const int64_t token = (int64_t)t[u][k];
-          f((uint32_t)(base + (u * kWaveSize + lane) * V + k), (uint32_t)token,
-            (uint64_t)token < (uint64_t)vocabulary && token != padding_token);
+          const uint32_t token = (uint32_t)t[u][k];
+          bool counts = token < limit && token != padding;
+          if constexpr (sizeof(TT) == 8) counts = counts && (uint64_t)t[u][k] >> 32 == 0;
+          f((uint32_t)base + (u * kWaveSize + lane) * V + k, token, counts ? token & mask : ~0u);
         }
     }
   };
 
-  scan([&](uint32_t at, uint32_t token, bool counts) {
-    const uint32_t of = token & (groups - 1);
-    below += counts && of < group ? 1 : 0;
-    const bool own = counts && of == group;
-    const uint64_t owns = __ballot(own);
+  // One add for all lanes whose row is that of the first lane (a frequent token's, mostly:
+  // 64 adds to one counter take as many cycles), one for each other lane; the counter
+  // before the add and the lanes in front, or nothing.
+  const auto count_row = [&](uint32_t row) {
+    const uint64_t same = __builtin_amdgcn_ballot_w64(row == __builtin_amdgcn_readfirstlane(row));
+    const bool mine = (same >> lane) & 1;
+    const uint32_t before = mine ? mbcnt(same) : 0;
+    uint32_t at = 0;
+    if (before == 0) at = atomicAdd(&counters[row], mine ? (uint32_t)__popcll(same) : 1u);
+    const uint32_t first = __builtin_amdgcn_readfirstlane(at);
+    return mine ? first + before : at;
+  };
+
+  scan([&](uint32_t at, uint32_t token, uint32_t of) {
+    below += __popcll(__builtin_amdgcn_ballot_w64(of < group));
+    const uint64_t owns = __builtin_amdgcn_ballot_w64(of == group);
     if (owns != 0) {
-      if (own) {
-        atomicAdd(&counters[token >> log2], 1u);
-        const uint32_t place = listed + mbcnt(owns);
-        if (place < kGroupList) list[place] = at;
-      }
+      const uint32_t place = listed + mbcnt(owns);
+      if (of == group && place < kGroupList) list[place] = (token >> log2) << kGroupCountLog2 | at;
       listed += __popcll(owns);
     }
   });
-  for (int off = kWaveSize / 2; off > 0; off >>= 1) below += __shfl_xor(below, off, kWaveSize);
+  if (listed <= kGroupList) {
+    for (uint32_t j = lane; j < listed; j += kWaveSize) count_row(list[j] >> kGroupCountLog2);
+  } else {
+    scan([&](uint32_t, uint32_t token, uint32_t of) {
+      if (of == group) count_row(token >> log2);
+    });
+  }
   if (lane == 0) wave_below[wave] = below;
   __syncthreads();
 
@@ -197,28 +233,26 @@ __global__ __launch_bounds__(kGroupBlock) void group_tokens_kernel(
 
   if (listed <= kGroupList) {
     for (uint32_t j = lane; j < listed; j += kWaveSize) {
-      const uint32_t at = list[j], token = (uint32_t)tokens[at];
-      const uint32_t to = atomicAdd(&counters[token >> log2], 1u);
-      keys[to] = token;
-      order[to] = at;
+      const uint32_t row = list[j] >> kGroupCountLog2;
+      const uint32_t to = count_row(row);
+      keys[to] = row << log2 | group;
+      order[to] = list[j] & ((1u << kGroupCountLog2) - 1);
     }
   } else {
-    scan([&](uint32_t at, uint32_t token, bool counts) {
-      if (counts && (token & (groups - 1)) == group) {
-        const uint32_t to = atomicAdd(&counters[token >> log2], 1u);
+    scan([&](uint32_t at, uint32_t token, uint32_t of) {
+      if (of == group) {
+        const uint32_t to = count_row(token >> log2);
         keys[to] = token;
         order[to] = at;
       }
     });
   }
   if (group == groups - 1)
-    for (int64_t i = (int64_t)all_below + all_own + threadIdx.x; i < count; i += kGroupBlock)
+    for (int64_t i = (int64_t)all_below + all_own + threadIdx.x; i < padded; i += kGroupBlock)
       keys[i] = (uint32_t)vocabulary;
 }
 
 struct Sums {
-  const uint32_t* keys;
-  const uint32_t* order;
   const uint64_t* met;   // bit (v >> group_log2) & 63 of word (v >> group_log2 >> 6, v modulo the
   int group_log2;        // groups): row v has a token; nullptr where the keys are sorted
   uint32_t* crossings;   // [0]: their number; then the chunks in which a run begins that
@@ -226,32 +260,47 @@ struct Sums {
   float* parts;          // per chunk the part of a run from before it, then as many of
                          // runs that go on behind it
   int64_t count, chunks, part_stride;
+  int64_t chunk;         // positions in one
   int64_t vocabulary, dimension;
   int64_t grad_stride, table_stride;
   float scale;
   int32_t accumulate;
-  uint32_t sum_blocks;   // further blocks clear rows
-  uint32_t clear_blocks;
-  uint32_t slices;       // column slices of a row
+  uint32_t slices;       // column slices of a row, in the sums and in the join
   uint32_t join_slices;
+  uint32_t sum_blocks;   // blocks of the sums and of the join; further ones clear rows,
+  uint32_t join_blocks;  // those from early_rows on beside the join
+  int64_t early_rows;
+  int32_t clear_rows;    // rows a block clears, lanes that share one
+  int32_t clear_lanes_log2;
   int lanes_log2;        // lanes that share a row
 };
 
+// A thread's columns of a row, which begin at its `own`-th of W sums (0, or what the last
+// columns of a row leave over), into the table.
 template <typename TW, int W>
-__device__ __forceinline__ void finish_row(TW* to, float (&sum)[W], int64_t columns, float scale,
+__device__ __forceinline__ void finish_row(TW* to, const float (&sum)[W], int own, float scale,
                                            int32_t accumulate) {
-  if (columns <= 0) return;
-  float old[W];
-  load_floats<TW, W>(old, to, accumulate ? columns : 0);
+  float v[W];
+  if (own == 0) {
+    if (accumulate) {
+      load_floats<TW, W>(v, to, W);
 #pragma unroll
-  for (int k = 0; k < W; ++k) sum[k] = sum[k] * scale + old[k];
-  store_floats<TW, W>(to, sum, columns);
+      for (int k = 0; k < W; ++k) v[k] = sum[k] * scale + v[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[k] = sum[k] * scale;
+    }
+    store_floats<TW, W>(to, v, W);
+  } else {
+#pragma unroll
+    for (int k = 0; k < W; ++k)
+      if (k >= own) to[k] = (TW)(sum[k] * scale + (accumulate ? (float)to[k] : 0.0f));
+  }
 }
 
-constexpr int kClearRows = 16;  // per block
-
 // Whether a row has a token: by its bit, or its key is among the sorted ones.
-__device__ __forceinline__ bool is_met(const Sums& s, int64_t row) {
+__device__ __forceinline__ bool is_met(const Sums& s, const uint32_t* __restrict__ keys,
+                                       int64_t row) {
   if (s.met != nullptr) {
     const uint32_t of = (uint32_t)row & ((1u << s.group_log2) - 1), local = (uint32_t)(row >> s.group_log2);
     return (s.met[((uint64_t)(local >> 6) << s.group_log2) + of] >> (local & 63)) & 1;
@@ -259,41 +308,58 @@ __device__ __forceinline__ bool is_met(const Sums& s, int64_t row) {
   int64_t low = 0, high = s.count;
   while (low < high) {
     const int64_t middle = (low + high) >> 1;
-    if ((int64_t)s.keys[middle] < row) low = middle + 1;
+    if ((int64_t)keys[middle] < row) low = middle + 1;
     else high = middle;
   }
-  return low < s.count && (int64_t)s.keys[low] == row;
+  return low < s.count && (int64_t)keys[low] == row;
 }
 
+// Clears the rows of no token in [begin, end): zeros, past the caches that the rows in use
+// are in (8192 tokens into 50021 x 1024: 47.5 us, 54.7 with plain stores).  A block clears
+// 8 KB, as many rows at a time as its threads cover; with longer stretches a block, more
+// places are written at once (65536 tokens into 131072 x 2048: 259 us, 271 with 16 KB, 275
+// with 32 KB), shorter ones are too many blocks (8192 into 50021 x 1024: 42.0, 44.5 with
+// 4 KB).
+constexpr int64_t kClearBytes = 8192;
 template <typename TW>
-__device__ __forceinline__ void clear_rows(const Sums& s, TW* __restrict__ table, int64_t first) {
+__device__ __forceinline__ void clear_rows(const Sums& s, const uint32_t* __restrict__ keys,
+                                           TW* __restrict__ table, int64_t begin, int64_t end,
+                                           uint32_t block, uint32_t blocks) {
   constexpr int W = 16 / sizeof(TW);
-  const int64_t mine = first + (threadIdx.x & (kClearRows - 1));
-  const bool met = mine >= s.vocabulary || is_met(s, mine);
-  uint32_t unmet = ~(uint32_t)__ballot(met) & ((1u << kClearRows) - 1);
-  float zeros[W];
-#pragma unroll
-  for (int k = 0; k < W; ++k) zeros[k] = 0.0f;
-  for (; unmet != 0; unmet &= unmet - 1) {
-    TW* row = table + (first + __builtin_ctz(unmet)) * s.table_stride;
-    for (int64_t c = (int64_t)threadIdx.x * W; c < s.dimension; c += kBlock * W)
-      store_floats<TW, W>(row + c, zeros, s.dimension - c);
+  const int log2 = s.clear_lanes_log2;
+  const typename Pack<TW, W>::vec zeros = {};
+  for (int64_t first = begin + (int64_t)block * s.clear_rows; first < end;
+       first += (int64_t)blocks * s.clear_rows) {
+    for (int64_t r = first + (threadIdx.x >> log2); r < first + s.clear_rows && r < end;
+         r += kBlock >> log2) {
+      if (is_met(s, keys, r)) continue;
+      TW* row = table + r * s.table_stride;
+      for (int64_t c = (int64_t)(threadIdx.x & ((1u << log2) - 1)) * W; c < s.dimension;
+           c += (int64_t)W << log2) {
+        if (c + W <= s.dimension) {
+          __builtin_nontemporal_store(zeros, reinterpret_cast<typename Pack<TW, W>::type*>(row + c));
+        } else {
+          for (int64_t k = c; k < s.dimension; ++k) row[k] = (TW)0.0f;
+        }
+      }
+    }
   }
 }
 
-template <typename TG, typename TW, bool WHOLE_WAVE>
-__global__ __launch_bounds__(kBlock) void embedding_gradient_kernel(
-    Sums s, const TG* __restrict__ grad_out, TW* __restrict__ table) {
-  constexpr int W = Width<TG, TW>::value;
-  constexpr int U = 8;  // rows in flight
-  if (blockIdx.x >= s.sum_blocks) {
-    for (int64_t first = (int64_t)(blockIdx.x - s.sum_blocks) * kClearRows; first < s.vocabulary;
-         first += (int64_t)s.clear_blocks * kClearRows)
-      clear_rows(s, table, first);
-    return;
-  }
+constexpr int64_t kLateBytes = 32 << 20;
+
+// What becomes of a run's sum: a part of it is left for the join, it is the row, or it is
+// the business of the chunk before.
+enum class Run { kPart, kOwn, kOther };
+
+template <typename TG, typename TW, int W, int CHUNK, bool WHOLE_WAVE>
+__device__ __forceinline__ void sum_chunk(const Sums& s, const uint32_t* __restrict__ keys,
+                                          const uint32_t* __restrict__ order, uint32_t group,
+                                          const TG* __restrict__ grad_out,
+                                          TW* __restrict__ table) {
+  using P = typename Pack<TG, W>::type;
+    constexpr int U = WHOLE_WAVE && CHUNK > 8 ? 16 : 8;  // rows in flight
   const int log2 = WHOLE_WAVE ? 6 : s.lanes_log2;
-  const uint32_t group = (blockIdx.x << (8 - log2)) + (threadIdx.x >> log2);
   uint32_t chunk = group / s.slices;
   uint32_t slice = group - chunk * s.slices;
   if (WHOLE_WAVE) {
@@ -302,77 +368,147 @@ __global__ __launch_bounds__(kBlock) void embedding_gradient_kernel(
   }
   if (chunk >= s.chunks) return;
   const uint32_t lane = threadIdx.x & ((1u << log2) - 1);
-  const int64_t c = (((int64_t)slice << log2) + lane) * W;
-  const int64_t columns = s.dimension - c;
+  // The last thread of a row begins early enough for whole loads and leaves the columns of
+  // the one before it alone; a thread beyond does the same for none (W >= dimension: see
+  // the launch).
+  const int64_t first = (((int64_t)slice << log2) + lane) * W;
+  const int64_t c = first + W <= s.dimension ? first : s.dimension - W;
+  const int own = (int)(first - c < W ? first - c : W);
   const uint32_t none = (uint32_t)s.vocabulary;
-  const int64_t p0 = (int64_t)chunk * kChunk;
-  const uint32_t before = p0 > 0 ? s.keys[p0 - 1] : none;
-  float* const head = s.parts + (int64_t)chunk * s.part_stride + c;
+  const int64_t p0 = (int64_t)chunk * CHUNK;
+  float* const head = s.parts + (int64_t)chunk * s.part_stride + first;
   float* const tail = head + s.chunks * s.part_stride;
+  const auto store_part = [&](float* to, const float (&v)[W]) {
+    if (own == 0) {
+      store_floats<float, W>(to, v, W);
+    } else {
+#pragma unroll
+      for (int k = 0; k < W; ++k)
+        if (k >= own) to[k - own] = v[k];
+    }
+  };
 
-  uint32_t run = s.keys[p0];
-  bool began = run != before;  // the run began in this chunk
+  // The keys and positions of this chunk and of the next one, which a short run may reach:
+  // one per lane where a whole wave shares a row.
+  uint32_t lane_key = 0, lane_order = 0;
+  if (WHOLE_WAVE) {
+    static_assert(2 * CHUNK <= kWaveSize, "a chunk and the next in a wave's lanes");
+    lane_key = lane < 2 * CHUNK ? keys[p0 + lane] : none;
+    lane_order = lane < 2 * CHUNK ? order[p0 + lane] : 0;
+  }
+  const auto key_of = [&](int u) -> uint32_t {
+    return WHOLE_WAVE ? __builtin_amdgcn_readlane(lane_key, u) : keys[p0 + u];
+  };
+  const auto order_of = [&](int u) -> uint32_t {
+    return WHOLE_WAVE ? __builtin_amdgcn_readlane(lane_order, u) : order[p0 + u];
+  };
+
+  uint32_t run = key_of(0);
+  if (run == none) return;
+  const uint32_t some = order_of(0);
+  Run what = Run::kOwn;
+  if (p0 > 0 && run == keys[p0 - 1])
+    what = (p0 > CHUNK && run == keys[p0 - CHUNK - 1]) || run == keys[p0 + CHUNK] ? Run::kPart
+                                                                                    : Run::kOther;
+  const uint32_t other = what == Run::kOther ? run : none;
   float sum[W];
 #pragma unroll
   for (int k = 0; k < W; ++k) sum[k] = 0.0f;
-  for (int u0 = 0; u0 < kChunk && run != none; u0 += U) {
+  bool extended = false;
+  for (int u0 = 0;; u0 += U) {
+    if (u0 == CHUNK) {
+      const bool goes_on = keys[p0 + CHUNK] == run;
+      if (what == Run::kOwn && goes_on && keys[p0 + 2 * CHUNK] != run) {
+        extended = true;
+      } else {
+        if (what == Run::kOwn && !goes_on)
+          finish_row<TW, W>(table + run * s.table_stride + c, sum, own, s.scale, s.accumulate);
+        else if (what != Run::kOther)
+          store_part(what == Run::kOwn ? tail : head, sum);
+        if (what == Run::kOwn && goes_on && slice == 0 && lane == 0)
+          s.crossings[1 + atomicAdd(s.crossings, 1u)] = chunk;
+        return;
+      }
+    }
+    if (u0 == 2 * CHUNK) {
+      finish_row<TW, W>(table + run * s.table_stride + c, sum, own, s.scale, s.accumulate);
+      return;
+    }
+    // Loads first, without a branch: positions that are not wanted read one that is.
     uint32_t key[U];
-    float v[U][W];
+    typename Pack<TG, W>::vec v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t p = p0 + u0 + u;
-      key[u] = p < s.count ? s.keys[p] : none;
-      load_floats<TG, W>(v[u], grad_out + (key[u] != none ? s.order[p] * s.grad_stride : 0) + c,
-                         key[u] != none ? columns : 0);
+      key[u] = key_of(u0 + u);
+      if (extended && key[u] != run) key[u] = none;
+      const bool wanted = key[u] != none && key[u] != other;
+      const uint32_t at = wanted ? order_of(u0 + u) : some;
+      v[u] = *reinterpret_cast<const P*>(grad_out + at * s.grad_stride + c);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (key[u] != run) {
         // The run ends here.
-        if (began) finish_row<TW, W>(table + run * s.table_stride + c, sum, columns, s.scale,
-                                     s.accumulate);
-        else if (columns > 0) store_floats<float, W>(head, sum, W);
+        if (what == Run::kOwn)
+          finish_row<TW, W>(table + run * s.table_stride + c, sum, own, s.scale, s.accumulate);
+        else if (what == Run::kPart)
+          store_part(head, sum);
+        if (key[u] == none) return;
 #pragma unroll
         for (int k = 0; k < W; ++k) sum[k] = 0.0f;
         run = key[u];
-        began = true;
+        what = Run::kOwn;
       }
+      // (Of a run that is another chunk's the sum is never used.)
 #pragma unroll
-      for (int k = 0; k < W; ++k) sum[k] += v[u][k];
+      for (int k = 0; k < W; ++k) sum[k] += (float)v[u][k];
     }
   }
-  if (run == none) return;
-  const int64_t next = p0 + kChunk;
-  const bool goes_on = next < s.count && s.keys[next] == run;
-  if (began && !goes_on) {
-    finish_row<TW, W>(table + run * s.table_stride + c, sum, columns, s.scale, s.accumulate);
-    return;
-  }
-  if (columns > 0) store_floats<float, W>(began ? tail : head, sum, W);
-  if (began && slice == 0 && lane == 0) s.crossings[1 + atomicAdd(s.crossings, 1u)] = chunk;
 }
 
-// Joins the parts of the runs that cross chunks: the waves of a block take every 16th
-// part, and their sums are added in the order of the waves.
-constexpr int kJoinBlock = 1024;
+template <typename TG, typename TW, int W, int CHUNK, bool WHOLE_WAVE>
+__global__ __launch_bounds__(kBlock) void embedding_gradient_kernel(
+    Sums s, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ order,
+    const TG* __restrict__ grad_out, TW* __restrict__ table) {
+  if (blockIdx.x >= s.sum_blocks) {
+    clear_rows(s, keys, table, 0, s.early_rows, blockIdx.x - s.sum_blocks,
+               gridDim.x - s.sum_blocks);
+    return;
+  }
+  const int log2 = WHOLE_WAVE ? 6 : s.lanes_log2;
+  sum_chunk<TG, TW, W, CHUNK, WHOLE_WAVE>(s, keys, order, (blockIdx.x << (8 - log2)) + (threadIdx.x >> log2),
+                                   grad_out, table);
+}
+
+// Joins the parts of the long runs: the waves of a block take every fourth part, and
+// their sums are added in the order of the waves.  The blocks behind clear rows.
+constexpr int kJoinBlock = kBlock;
+constexpr int kJoinBlocks = 2048;
 constexpr int kJoinWaves = kJoinBlock / kWaveSize;
+
 template <typename TW>
-__global__ __launch_bounds__(kJoinBlock) void join_runs_kernel(Sums s, TW* __restrict__ table) {
+__global__ __launch_bounds__(kJoinBlock) void join_runs_kernel(
+    Sums s, const uint32_t* __restrict__ keys, TW* __restrict__ table) {
   constexpr int W = 4;
+  if (blockIdx.x >= s.join_blocks) {
+    clear_rows(s, keys, table, s.early_rows, s.vocabulary, blockIdx.x - s.join_blocks,
+               gridDim.x - s.join_blocks);
+    return;
+  }
   __shared__ float lds[kJoinWaves][kWaveSize * W];
   const uint32_t slices = s.join_slices;
   const int wave = threadIdx.x / kWaveSize, lane = threadIdx.x & (kWaveSize - 1);
   const uint32_t items = s.crossings[0] * slices;
-  for (uint32_t item = blockIdx.x; item < items; item += gridDim.x) {
+  for (uint32_t item = blockIdx.x; item < items; item += s.join_blocks) {
     const int64_t chunk = s.crossings[1 + item / slices];
     const int64_t c = ((int64_t)(item % slices) * kWaveSize + lane) * W;
-    const int64_t columns = s.dimension - c;
-    const uint32_t run = s.keys[chunk * kChunk + kChunk - 1];
+    const int64_t columns = s.dimension - c;  // a part's row is padded to whole loads
+    const uint32_t run = keys[chunk * s.chunk + s.chunk - 1];
     // Chunks behind it that begin inside the run.
     int64_t more = 0;
     for (;;) {
-      const int64_t p = (chunk + 1 + more + lane) * kChunk;
-      const uint64_t inside = __ballot(p < s.count && s.keys[p < s.count ? p : 0] == run);
+      const int64_t p = (chunk + 1 + more + lane) * s.chunk;
+      const uint64_t inside = __ballot(p < s.count && keys[p < s.count ? p : 0] == run);
       if (inside == ~0ull) {
         more += kWaveSize;
         continue;
@@ -401,7 +537,17 @@ __global__ __launch_bounds__(kJoinBlock) void join_runs_kernel(Sums s, TW* __res
       for (int w = 1; w < kJoinWaves; ++w)
 #pragma unroll
         for (int k = 0; k < W; ++k) sum[k] += lds[w][lane * W + k];
-      finish_row<TW, W>(table + run * s.table_stride + c, sum, columns, s.scale, s.accumulate);
+      TW* to = table + run * s.table_stride + c;
+      if (columns >= W) {
+        finish_row<TW, W>(to, sum, 0, s.scale, s.accumulate);
+      } else {
+#pragma unroll
+        for (int k = 0; k < W; ++k)
+          if (k < columns) {
+            const float one[1] = {sum[k]};
+            finish_row<TW, 1>(to + k, one, 0, s.scale, s.accumulate);
+          }
+      }
     }
     __syncthreads();
   }
@@ -409,16 +555,19 @@ __global__ __launch_bounds__(kJoinBlock) void join_runs_kernel(Sums s, TW* __res
 
 struct GradientTemp {
   int64_t keys, order, met, crossings, parts, sort, bytes;  // offsets
-  int64_t chunks, part_stride;
+  int64_t chunk, chunks, part_stride;
+  int64_t padded;  // length of keys and order: whole chunks and the reach of the last one
 };
 GradientTemp gradient_temp(int64_t count, int64_t vocabulary, int64_t dimension) {
   GradientTemp t;
   const bool groups = takes_groups(count, vocabulary);
-  t.chunks = div_up(count, kChunk);
+  t.chunk = chunk_length(count, dimension);
+  t.chunks = div_up(count, t.chunk);
   t.part_stride = align_up(dimension, 8);
   t.keys = 0;
-  t.order = align_up(count * 4, 256);
-  t.met = t.order + align_up(count * 4, 256);
+  t.padded = (t.chunks + 2) * t.chunk;
+  t.order = align_up(t.padded * 4, 256);
+  t.met = t.order + align_up(t.padded * 4, 256);
   t.crossings =
       t.met + (groups ? (div_up(vocabulary, (int64_t)64 << group_log2(vocabulary)) * 8)
                             << group_log2(vocabulary)
@@ -480,7 +629,7 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
         ProfileScope scope(stream, "embedding_group_tokens");
         hipLaunchKernelGGL((group_tokens_kernel<TT>), dim3(1u << log2), dim3(kGroupBlock),
                            (unsigned)(kGroupWaves * (rows + kGroupList) * 4), stream,
-                           static_cast<const TT*>(a.tokens), a.count, a.vocabulary,
+                           static_cast<const TT*>(a.tokens), a.count, t.padded, a.vocabulary,
                            a.padding_token, log2, rows, keys, order,
                            reinterpret_cast<uint64_t*>(base + t.met), crossings);
       }
@@ -491,13 +640,13 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
   } else if (a.count > 0) {
     const int32_t rc = with_token_type(a.token_type, [&](auto tt) -> int32_t {
       using TT = decltype(tt);
-      const int64_t blocks = div_up(a.count, kBlock);
+      const int64_t blocks = div_up(t.padded, kBlock);
       {
         ProfileScope scope(stream, "embedding_token_keys");
         hipLaunchKernelGGL((token_keys_kernel<TT>),
                            dim3((unsigned)(blocks < kMaxBlocks ? blocks : kMaxBlocks)),
                            dim3(kBlock), 0, stream, static_cast<const TT*>(a.tokens), a.count,
-                           a.vocabulary, a.padding_token, keys, crossings);
+                           t.padded, a.vocabulary, a.padding_token, keys, crossings);
       }
       ILGPU_HIP_CHECK(hipGetLastError());
       return ILGPU_HIP_SUCCESS;
@@ -512,7 +661,8 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
     return with_type(a.table_type, [&](auto tw) -> int32_t {
       using TG = decltype(tg);
       using TW = decltype(tw);
-      constexpr int W = Width<TG, TW>::value;
+      constexpr int kWide = Width<TG, TW>::value;
+      const int W = a.dimension >= kWide ? kWide : 1;  // a thread's columns
       TW* table = static_cast<TW*>(a.grad_table);
       const int all_log2 = lanes_log2(a.dimension, W);
       const int log2 = all_log2 < 6 ? all_log2 : 6;
@@ -521,27 +671,49 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
       // (That many chunks and slices have parts of 2^42 bytes: no device holds such a temp.)
       if (t.chunks * join_slices > INT32_MAX) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
       const int64_t sum_blocks = div_up(t.chunks * slices, kBlock >> log2);
-      int64_t clear_blocks = a.accumulate ? 0 : div_up(a.vocabulary, kClearRows);
-      if (clear_blocks > kMaxBlocks) clear_blocks = kMaxBlocks;
-      const Sums s{keys, order,
-                   groups ? reinterpret_cast<const uint64_t*>(base + t.met) : nullptr,
+      // Rows cleared beside the join are as many as it has time for while it waits for its
+      // own reads; those before them keep the memory busy while the sums wait for theirs
+      // (8192 tokens into 50021 x 1024: 43.6 us, 46.9 with all of them beside the sums, 56.9
+      // with all beside the join).
+      const int64_t late = kLateBytes / ((int64_t)sizeof(TW) * a.dimension);
+      const int64_t row_bytes = (int64_t)sizeof(TW) * a.dimension;
+      const int clear_log2 = lanes_log2(a.dimension, 16 / sizeof(TW));
+      int64_t clear_rows = kBlock >> clear_log2;
+      while (2 * clear_rows * row_bytes <= kClearBytes) clear_rows *= 2;
+      const int64_t early_rows =
+          a.accumulate || a.vocabulary <= late ? 0 : (a.vocabulary - late) / clear_rows * clear_rows;
+      const auto clear_blocks = [&](int64_t rows) {
+        const int64_t blocks = div_up(rows, clear_rows);
+        return blocks < kMaxBlocks ? blocks : kMaxBlocks;
+      };
+      const int64_t early_blocks = clear_blocks(early_rows);
+      const int64_t late_blocks = a.accumulate ? 0 : clear_blocks(a.vocabulary - early_rows);
+      const int64_t items = t.chunks > 2 ? (t.chunks - 2) * join_slices : 0;
+      const int64_t join_blocks = items < kJoinBlocks ? items : kJoinBlocks;
+      const Sums s{groups ? reinterpret_cast<const uint64_t*>(base + t.met) : nullptr,
                    group_log2(a.vocabulary), crossings, reinterpret_cast<float*>(base + t.parts), a.count,
-                   t.chunks, t.part_stride, a.vocabulary, a.dimension, a.grad_out_stride,
-                   a.table_stride, a.scale, a.accumulate, (uint32_t)sum_blocks,
-                   (uint32_t)clear_blocks, (uint32_t)slices, (uint32_t)join_slices, log2};
-      if (sum_blocks + clear_blocks > 0) {
+                   t.chunks, t.part_stride, t.chunk, a.vocabulary, a.dimension, a.grad_out_stride,
+                   a.table_stride, a.scale, a.accumulate, (uint32_t)slices,
+                   (uint32_t)join_slices, (uint32_t)sum_blocks, (uint32_t)join_blocks,
+                   early_rows, (int32_t)clear_rows, clear_log2, log2};
+      if (sum_blocks + early_blocks > 0) {
         ProfileScope scope(stream, "embedding_gradient");
-        auto kernel = log2 == 6 ? embedding_gradient_kernel<TG, TW, true>
-                                : embedding_gradient_kernel<TG, TW, false>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(sum_blocks + clear_blocks)), dim3(kBlock), 0,
-                           stream, s, static_cast<const TG*>(a.grad_out), table);
+        const auto kernel_of = [&](auto chunk) {
+          constexpr int C = decltype(chunk)::value;
+          return W == 1      ? embedding_gradient_kernel<TG, TW, 1, C, false>
+                 : log2 == 6 ? embedding_gradient_kernel<TG, TW, kWide, C, true>
+                             : embedding_gradient_kernel<TG, TW, kWide, C, false>;
+        };
+        auto kernel = t.chunk == kChunk ? kernel_of(std::integral_constant<int, kChunk>())
+                                        : kernel_of(std::integral_constant<int, kShortChunk>());
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(sum_blocks + early_blocks)), dim3(kBlock), 0,
+                           stream, s, keys, order, static_cast<const TG*>(a.grad_out), table);
       }
       ILGPU_HIP_CHECK(hipGetLastError());
-      if (t.chunks > 1) {
-        const int64_t items = (t.chunks - 1) * join_slices;
-        ProfileScope scope(stream, "embedding_join_runs");
-        hipLaunchKernelGGL((join_runs_kernel<TW>), dim3((unsigned)(items < 512 ? items : 512)),
-                           dim3(kJoinBlock), 0, stream, s, table);
+      if (join_blocks + late_blocks > 0) {
+        ProfileScope scope(stream, "embedding_gradient_rest");
+        hipLaunchKernelGGL((join_runs_kernel<TW>), dim3((unsigned)(join_blocks + late_blocks)),
+                           dim3(kJoinBlock), 0, stream, s, keys, table);
       }
       ILGPU_HIP_CHECK(hipGetLastError());
       return ILGPU_HIP_SUCCESS;

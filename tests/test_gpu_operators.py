@@ -195,7 +195,9 @@ def test_embedding_gradient(n, vocabulary, dimension, grad_type, table_type):
 
 
 @pytest.mark.parametrize("n,vocabulary", [(20_000, 32_003), (70_001, 1000), (150_000, 250_007),
-                                          (300_000, 70_000), (40_000, 1_500_000)])
+                                          (300_000, 70_000), (40_000, 1_500_000),
+                                          (20_000, 500_009), (30_000, 1_048_576),
+                                          (131_072, 50_000), (131_073, 50_000), (65_537, 300_000)])
 def test_embedding_gradient_of_many_tokens(n, vocabulary):
     import torch
     g = _rng(n, vocabulary)
@@ -209,7 +211,7 @@ def test_embedding_gradient_of_many_tokens(n, vocabulary):
 
 @pytest.mark.parametrize("distribution", ["one", "two", "alternating", "runs", "all_outside",
                                           "ascending", "mostly_one"])
-@pytest.mark.parametrize("n", [31, 1000, 30_000])
+@pytest.mark.parametrize("n", [31, 64, 1000, 1024, 30_000, 120_001])
 def test_embedding_gradient_of_skewed_tokens(n, distribution):
     import torch
     vocabulary = 513
