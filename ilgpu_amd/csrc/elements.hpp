@@ -58,6 +58,15 @@ __device__ __forceinline__ void store_floats(T* p, const float (&v)[N], int64_t 
   }
 }
 
+// x * scale as it is rounded to T next.  (Of a product that is rounded to half the compiler
+// makes a fused one with an addend of +0, which turns -0 into +0; the empty statement keeps
+// the two apart.)
+template <typename T> __device__ __forceinline__ float product_for(float x, float scale) {
+  float v = x * scale;
+  if constexpr (std::is_same<T, half_t>::value) asm("" : "+v"(v));
+  return v;
+}
+
 // Calls f(T()) with the element type of a validated type code.
 template <typename F> int32_t with_type(int32_t type, F f) {
   switch (type) {
