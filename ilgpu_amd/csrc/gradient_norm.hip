@@ -12,8 +12,8 @@ namespace ilgpu_hip {
 namespace {
 
 constexpr int kBlock = 256;
-constexpr int kTensors = 128;            // per launch
-constexpr int64_t kChunk = 16384;        // elements
+constexpr int kTensors = 120;            // per launch
+constexpr int64_t kChunkBytes = 32768;
 constexpr int kBlocksPerCu = 8;
 
 struct TensorTable {
@@ -21,7 +21,7 @@ struct TensorTable {
   void* target[kTensors];
   int64_t length[kTensors];
   uint32_t chunks_end[kTensors];         // chunks of this and all tensors before it
-  uint8_t type[kTensors];
+  int32_t type[kTensors];                // (words: a scalar load of its own each)
   int32_t count;
 };
 static_assert(sizeof(TensorTable) <= 4000, "kernel arguments");
@@ -34,12 +34,13 @@ int64_t fill_table(TensorTable& table, const ilgpu_hip_tensor* sources,
   int64_t chunks = 0;
   for (; next < count && used < kTensors; ++next) {
     if (sources[next].length == 0) continue;
-    chunks += div_up(sources[next].length, kChunk);  // at most 2^26 and one per tensor
+    // (At most 2^27 and one per tensor.)
+    chunks += div_up(sources[next].length * operator_elem_size(sources[next].type), kChunkBytes);
     table.source[used] = sources[next].data;
     table.target[used] = targets != nullptr ? targets[next].data : sources[next].data;
     table.length[used] = sources[next].length;
     table.chunks_end[used] = (uint32_t)chunks;
-    table.type[used] = (uint8_t)sources[next].type;
+    table.type[used] = sources[next].type;
     ++used;
   }
   table.count = used;
@@ -67,17 +68,45 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
   return sum;
 }
 
-template <typename T>
-__device__ __forceinline__ double chunk_squares(const T* p, int64_t count) {
-  constexpr int W = 16 / sizeof(T);
-  double sum = 0.0;
-  for (int64_t i = (int64_t)threadIdx.x * W; i < count; i += kBlock * W) {
-    float v[W];
-    load_floats<T, W>(v, p + i, count - i);
-#pragma unroll
-    for (int k = 0; k < W; ++k) sum += (double)v[k] * (double)v[k];
+// Calls f(tensor, T(), first element, elements) for a chunk.
+template <typename F>
+__device__ __forceinline__ void with_chunk(const TensorTable& table, uint32_t chunk, F f) {
+  const int t = tensor_of(table, chunk);
+  const int64_t in = chunk - (t > 0 ? table.chunks_end[t - 1] : 0);
+  const auto call = [&](auto type) {
+    constexpr int64_t kElements = kChunkBytes / sizeof(type);
+    const int64_t left = table.length[t] - in * kElements;
+    f(t, type, in * kElements, left < kElements ? left : kElements);
+  };
+  switch (table.type[t]) {
+    case ILGPU_HIP_F32: call(float()); break;
+    case ILGPU_HIP_F16: call(half_t()); break;
+    default: call(bfloat_t()); break;
   }
-  return sum;
+}
+
+// Calls f(loaded vector, its index) for the whole vectors of `count` elements, several loads
+// in flight, and g(element index) for the elements that are left.
+template <typename T, typename F, typename G>
+__device__ __forceinline__ void for_elements(const T* p, int64_t count, F f, G g) {
+  constexpr int W = 16 / sizeof(T), U = 8;
+  using P = typename Pack<T, W>::type;
+  const int vectors = (int)(count / W);
+  int i = threadIdx.x;
+  for (; i + (U - 1) * kBlock < vectors; i += U * kBlock) {
+    typename Pack<T, W>::vec v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      v[u] = __builtin_nontemporal_load(reinterpret_cast<const P*>(p + (int64_t)(i + u * kBlock) * W));
+#pragma unroll
+    for (int u = 0; u < U; ++u) f(v[u], (int64_t)(i + u * kBlock) * W);
+  }
+  for (; i < vectors; i += kBlock) {
+    const typename Pack<T, W>::vec v = *reinterpret_cast<const P*>(p + (int64_t)i * W);
+    f(v, (int64_t)i * W);
+  }
+  const int64_t rest = (int64_t)vectors * W + threadIdx.x;
+  if (rest < count) g(rest);
 }
 
 __global__ __launch_bounds__(kBlock) void square_sums_kernel(TensorTable table,
@@ -86,21 +115,18 @@ __global__ __launch_bounds__(kBlock) void square_sums_kernel(TensorTable table,
   const uint32_t chunks = table.chunks_end[table.count - 1];
   double sum = 0.0;
   for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-    const int t = tensor_of(table, chunk);
-    const int64_t from = (int64_t)(chunk - (t > 0 ? table.chunks_end[t - 1] : 0)) * kChunk;
-    const int64_t left = table.length[t] - from;
-    const int64_t count = left < kChunk ? left : kChunk;
-    switch (table.type[t]) {
-      case ILGPU_HIP_F32:
-        sum += chunk_squares(static_cast<const float*>(table.source[t]) + from, count);
-        break;
-      case ILGPU_HIP_F16:
-        sum += chunk_squares(static_cast<const half_t*>(table.source[t]) + from, count);
-        break;
-      default:
-        sum += chunk_squares(static_cast<const bfloat_t*>(table.source[t]) + from, count);
-        break;
-    }
+    with_chunk(table, chunk, [&](int t, auto type, int64_t from, int64_t count) {
+      using T = decltype(type);
+      constexpr int W = 16 / sizeof(T);
+      const T* p = static_cast<const T*>(table.source[t]) + from;
+      for_elements<T>(
+          p, count,
+          [&](const typename Pack<T, W>::vec& v, int64_t) {
+#pragma unroll
+            for (int k = 0; k < W; ++k) sum += (double)(float)v[k] * (double)(float)v[k];
+          },
+          [&](int64_t i) { sum += (double)(float)p[i] * (double)(float)p[i]; });
+    });
   }
   sum = block_sum(sum, lds);
   if (threadIdx.x == 0) partials[blockIdx.x] = sum;
@@ -115,20 +141,6 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(const double* __restrict__
   if (threadIdx.x == 0) norm[0] = (float)sqrt(sum);
 }
 
-// source and target may be the same array.
-template <typename T>
-__device__ __forceinline__ void scale_chunk(const T* source, T* target, int64_t count,
-                                            float factor) {
-  constexpr int W = 16 / sizeof(T);
-  for (int64_t i = (int64_t)threadIdx.x * W; i < count; i += kBlock * W) {
-    float v[W];
-    load_floats<T, W>(v, source + i, count - i);
-#pragma unroll
-    for (int k = 0; k < W; ++k) v[k] *= factor;
-    store_floats<T, W>(target + i, v, count - i);
-  }
-}
-
 __global__ __launch_bounds__(kBlock) void clip_kernel(TensorTable table,
                                                       const float* __restrict__ norm,
                                                       float max_norm) {
@@ -138,25 +150,22 @@ __global__ __launch_bounds__(kBlock) void clip_kernel(TensorTable table,
   const float factor = clipped ? max_norm / n : 1.0f;
   const uint32_t chunks = table.chunks_end[table.count - 1];
   for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-    const int t = tensor_of(table, chunk);
-    if (!clipped && table.source[t] == table.target[t]) continue;
-    const int64_t from = (int64_t)(chunk - (t > 0 ? table.chunks_end[t - 1] : 0)) * kChunk;
-    const int64_t left = table.length[t] - from;
-    const int64_t count = left < kChunk ? left : kChunk;
-    switch (table.type[t]) {
-      case ILGPU_HIP_F32:
-        scale_chunk(static_cast<const float*>(table.source[t]) + from,
-                    static_cast<float*>(table.target[t]) + from, count, factor);
-        break;
-      case ILGPU_HIP_F16:
-        scale_chunk(static_cast<const half_t*>(table.source[t]) + from,
-                    static_cast<half_t*>(table.target[t]) + from, count, factor);
-        break;
-      default:
-        scale_chunk(static_cast<const bfloat_t*>(table.source[t]) + from,
-                    static_cast<bfloat_t*>(table.target[t]) + from, count, factor);
-        break;
-    }
+    with_chunk(table, chunk, [&](int t, auto type, int64_t from, int64_t count) {
+      using T = decltype(type);
+      constexpr int W = 16 / sizeof(T);
+      if (!clipped && table.source[t] == table.target[t]) return;
+      const T* source = static_cast<const T*>(table.source[t]) + from;
+      T* target = static_cast<T*>(table.target[t]) + from;  // perhaps the source
+      for_elements<T>(
+          source, count,
+          [&](const typename Pack<T, W>::vec& v, int64_t at) {
+            typename Pack<T, W>::vec r;
+#pragma unroll
+            for (int k = 0; k < W; ++k) r[k] = (T)product_for<T>((float)v[k], factor);
+            __builtin_nontemporal_store(r, reinterpret_cast<typename Pack<T, W>::type*>(target + at));
+          },
+          [&](int64_t at) { target[at] = (T)product_for<T>((float)source[at], factor); });
+    });
   }
 }
 

@@ -606,7 +606,7 @@ SIZES = {
     "none": [], "empty": [0, 0], "one": [1], "few": [5, 0, 3, 1000, 7],
     "chunks": [16384, 16383, 16385, 65536, 1], "large": [3_000_017, 12],
     "many": [1 + 37 * k % 4001 for k in range(300)],
-    "full_table": [3] * 128, "beyond_a_table": [40_000] * 129, "large_many": [70_001] * 260,
+    "full_table": [3] * 120, "beyond_a_table": [40_000] * 121, "tables": [9_000] * 240, "large_many": [70_001] * 260,
 }
 
 
