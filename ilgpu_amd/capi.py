@@ -219,6 +219,7 @@ class DeviceArray:
     def __init__(self, length: int, dtype, *, _bytes=None):
         import torch
         self.dtype = np.dtype(dtype)
+        self._type_code = _NP_TO_TYPE.get(self.dtype)
         self.length = int(length)
         nbytes = self.length * self.dtype.itemsize
         self.bytes = _bytes if _bytes is not None else torch.empty(
@@ -260,7 +261,7 @@ class DeviceArray:
 
     @property
     def type_code(self) -> int:
-        return _NP_TO_TYPE[self.dtype]
+        return self._type_code if self._type_code is not None else _NP_TO_TYPE[self.dtype]
 
     def numpy(self) -> np.ndarray:
         if self.length == 0:
@@ -320,6 +321,7 @@ class DeviceMatrix:
                 self.rows > 0
                 and (self.rows - 1) * self.row_stride + self.columns > base.length):
             raise ArgumentOutOfRangeError(ERROR_OUT_OF_RANGE, "matrix")
+        self.ptr = base.ptr if self.rows > 0 else 0
 
     @classmethod
     def from_tensor(cls, t) -> "DeviceMatrix":
@@ -338,10 +340,6 @@ class DeviceMatrix:
         length = (rows - 1) * stride + columns if rows else 0
         flat = torch.as_strided(t, (length,), (1,)) if length else t.reshape(-1)
         return cls(DeviceArray.from_tensor(flat), rows, columns, stride)
-
-    @property
-    def ptr(self) -> int:
-        return self.base.ptr if self.rows > 0 else 0
 
 
 class _Tensor(ctypes.Structure):
@@ -636,17 +634,19 @@ def _need(condition: bool, what: str) -> None:
 def _column_vector(a: Optional[DeviceArray], length: int, what: str):
     if a is None:
         return None
-    _need(_dense(a).length == length, what)
-    return a.ptr
+    if a.length != length or a.stride != 1:
+        _need(_dense(a).length == length, what)
+    return a.bytes.data_ptr()
 
 
 def _statistic(a: Optional[DeviceArray], rows: int, what: str):
     if a is None:
         return None
-    if a.type_code != F32:
+    if a._type_code != F32:
         raise NotSupportedError(ERROR_NOT_SUPPORTED, f"{what} is float32")
-    _need(_dense(a).length >= rows, what)
-    return a.ptr
+    if a.length < rows or a.stride != 1:
+        _need(_dense(a).length >= rows, what)
+    return a.bytes.data_ptr()
 
 
 def embedding(table: DeviceMatrix, tokens: DeviceArray, out: DeviceMatrix, *,

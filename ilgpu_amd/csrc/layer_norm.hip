@@ -252,10 +252,10 @@ __global__ __launch_bounds__(kLongBlock) void layer_norm_long_kernel(
 }
 
 // How a row of `columns` elements of T is shared: V * LANES * W of them at most.  The lanes
-// follow the length, as idle ones take registers and issue like others (2^26 bfloat16
-// elements, gradients, us: 64 columns by a wave 461, by 8 lanes 80; 513 float32 columns
-// in a wave's two vectors 212, by 192 lanes 152).  Calls f(W, LANES, V) with integral
-// constants, or `otherwise` for rows beyond.
+// follow the length, as idle ones take registers and issue like others (gradients of 2^26
+// bfloat16 elements, us: rows of 64 by a wave 461, by 8 lanes 80; rows of 3000 by 512 lanes
+// 103, by 384 95).  Calls f(W, LANES, V) with integral constants, or `otherwise` for rows
+// beyond.
 #define ILGPU_HIP_SHAPE(w, lanes, v)                                                       \
   f(std::integral_constant<int, w>(), std::integral_constant<int, lanes>(), \
     std::integral_constant<int, v>())
