@@ -1,5 +1,6 @@
 """MI355X-native (gfx950) implementation of ILGPU.Algorithms' data-parallel
-primitives: radix sort (keys, pairs), scan, reduce and histogram.
+primitives: radix sort (keys, pairs), scan, reduce and histogram; and, beside them,
+operators of language models (embedding, layer norm, gradient norm and clipping).
 
 The product is the C-ABI shared library built from ``csrc/`` (declared in
 ``include/ilgpu_hip_algorithms.h``) plus the C++ host layer in ``host/`` that
