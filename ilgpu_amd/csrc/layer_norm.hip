@@ -347,7 +347,7 @@ __global__ __launch_bounds__(gradient_block<LANES>()) void layer_norm_gradient_k
   // The next row on its way costs registers that a large block does not have.
   constexpr bool kAhead = LANES * V * W < 1024 * 16;
   __shared__ float lds[2][2][row_waves<LANES>()];
-  __shared__ float joined[kJoins > 1 ? LANES * V * W : 1];
+  __shared__ float joined[kJoins > 1 ? kJoins : 1][kJoins > 1 ? LANES * V * W : 1];
   const Columns<W, LANES, V> own(columns);
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + row_of_block<LANES>();
@@ -411,8 +411,11 @@ __global__ __launch_bounds__(gradient_block<LANES>()) void layer_norm_gradient_k
   if (partials == nullptr) return;
   // The block's sums: over the rows of a wave, then over the waves, in their order; into its
   // row of partials, or, of a single block, to where they belong.
-  const int wave = threadIdx.x / kWaveSize;
   const auto join = [&](float (&sum)[V][W], float* to, TW* result) {
+    const auto put = [&](int64_t c, float total) {
+      if (gridDim.x > 1) to[c] = total;
+      else if (result != nullptr) result[c] = (TW)(accumulate ? (float)result[c] + total : total);
+    };
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
@@ -420,31 +423,32 @@ __global__ __launch_bounds__(gradient_block<LANES>()) void layer_norm_gradient_k
 #pragma unroll
         for (int off = LANES; off < kWaveSize; off <<= 1)
           sum[v][k] += __shfl_xor(sum[v][k], off, kWaveSize);
-    if (kJoins > 1) {
-      for (int i = kJoins - 1; i >= 0; --i) {
-        if (wave == i) {
+    if constexpr (kJoins > 1) {
+      const int wave = threadIdx.x / kWaveSize, lane = threadIdx.x & (kWaveSize - 1);
+      if (lane < LANES) {
 #pragma unroll
-          for (int v = 0; v < V; ++v)
+        for (int v = 0; v < V; ++v)
 #pragma unroll
-            for (int k = 0; k < W; ++k) {
-              float& place = joined[(v * W + k) * LANES + row_lane<LANES>()];
-              if (i < kJoins - 1) sum[v][k] += place;
-              if (i > 0 && (int)(threadIdx.x & (kWaveSize - 1)) < LANES) place = sum[v][k];
-            }
-        }
-        __syncthreads();
+          for (int k = 0; k < W; ++k) joined[wave][(v * W + k) * LANES + lane] = sum[v][k];
       }
+      __syncthreads();
+      for (int i = threadIdx.x; i < LANES * V * W; i += gradient_block<LANES>()) {
+        float total = joined[0][i];
+#pragma unroll
+        for (int j = 1; j < kJoins; ++j) total += joined[j][i];
+        const int k = i / LANES % W;
+        const int64_t first = ((int64_t)(i / (LANES * W)) * LANES + i % LANES) * W;
+        const int64_t at = first + W <= columns ? first : columns - W;
+        if (at + k >= first) put(at + k, total);
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int k = 0; k < W; ++k)
+          if (k >= own.skip[v]) put(own.at[v] + k, sum[v][k]);
     }
-    if (threadIdx.x >= LANES) return;
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-#pragma unroll
-      for (int k = 0; k < W; ++k) {
-        if (k < own.skip[v]) continue;
-        const int64_t c = own.at[v] + k;
-        if (gridDim.x > 1) to[c] = sum[v][k];
-        else if (result != nullptr) result[c] = (TW)(accumulate ? (float)result[c] + sum[v][k] : sum[v][k]);
-      }
   };
   join(sum_w, partials + (int64_t)blockIdx.x * columns, grad_weight);
   join(sum_b, partials + ((int64_t)gridDim.x + blockIdx.x) * columns, grad_bias);
