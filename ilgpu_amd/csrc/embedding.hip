@@ -512,6 +512,78 @@ __global__ __launch_bounds__(kBlock) void embedding_gradient_kernel(
   sum_chunk<TG, TW, W, CHUNK, WHOLE_WAVE>(s, keys, order, group, grad_out, table);
 }
 
+// The lanes of `inside` whose key is `row`, which differs between the groups of a wave.
+__device__ __forceinline__ uint64_t positions_of(uint64_t inside, uint32_t key, uint32_t row) {
+  uint64_t mine = 0;
+  for (; inside != 0; inside &= inside - 1) {
+    const int i = __builtin_ctzll(inside);
+    if ((uint32_t)__builtin_amdgcn_readlane(key, i) == row) mine |= 1ull << i;
+  }
+  return mine;
+}
+
+// Up to 64 tokens, in one launch: every wave holds them all, one a lane, and each row of the
+// table looks for its own among them.  So few tokens are bound by launches and by the clearing
+// of the table (64 tokens, us, this / three launches: into 1000 x 64 5.6 / 12.3, into 30000 x
+// 512 10.9 / 18.7, into 131072 x 1024 89 / 98; the worst, 64 times one token of 4096 columns,
+// 19.7 / 13.8).
+constexpr int64_t kFewTokens = kWaveSize;
+template <typename TG, typename TW, typename TT, int W>
+__global__ __launch_bounds__(kBlock) void embedding_gradient_of_few_kernel(
+    Sums s, const TT* __restrict__ tokens, int64_t padding_token, const TG* __restrict__ grad_out,
+    TW* __restrict__ table) {
+  constexpr int U = 8;  // rows in flight
+  using P = typename Pack<TG, W>::type;
+  const int lane = threadIdx.x & (kWaveSize - 1), log2 = s.clear_lanes_log2;
+  const int64_t token = lane < s.count ? (int64_t)tokens[lane] : -1;
+  const bool counts = (uint64_t)token < (uint64_t)s.vocabulary && token != padding_token;
+  const uint32_t key = counts ? (uint32_t)token : 0xffffffffu;
+  for (int64_t first = (int64_t)blockIdx.x * s.clear_rows; first < s.vocabulary;
+       first += (int64_t)gridDim.x * s.clear_rows) {
+    // The positions whose rows are among the block's.
+    const uint64_t inside = __ballot(counts && key - (uint32_t)first < (uint32_t)s.clear_rows);
+    if (inside == 0 && s.accumulate) continue;
+    for (int64_t r = first + (threadIdx.x >> log2); r < first + s.clear_rows && r < s.vocabulary;
+         r += kBlock >> log2) {
+      const uint64_t mine = inside == 0 ? 0 : positions_of(inside, key, (uint32_t)r);
+      TW* const row = table + r * s.table_stride;
+      for (int64_t c = (int64_t)(threadIdx.x & ((1u << log2) - 1)) * W; c < s.dimension;
+           c += (int64_t)W << log2) {
+        // (The last thread of a row: as in sum_chunk.)
+        const int64_t at = c + W <= s.dimension ? c : s.dimension - W;
+        float sum[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) sum[k] = 0.0f;
+        for (uint64_t left = mine; left != 0;) {
+          typename Pack<TG, W>::vec v[U];
+          bool there[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            there[u] = left != 0;
+            const int i = __builtin_ctzll(there[u] ? left : mine);
+            left &= left - 1;
+            v[u] = *reinterpret_cast<const P*>(grad_out + i * s.grad_stride + at);
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < W; ++k) sum[k] += there[u] ? (float)v[u][k] : 0.0f;
+        }
+        if (mine != 0) {
+          finish_row<TW, W>(row + at, sum, (int)(c - at), s.scale, s.accumulate);
+        } else if (!s.accumulate) {
+          if (at == c) {
+            const typename Pack<TW, W>::vec zeros = {};
+            __builtin_nontemporal_store(zeros, reinterpret_cast<typename Pack<TW, W>::type*>(row + c));
+          } else {
+            for (int64_t k = c; k < s.dimension; ++k) row[k] = (TW)0.0f;
+          }
+        }
+      }
+    }
+  }
+}
+
 // Joins the parts of the long runs: the waves of a block take every fourth part, and
 // their sums are added in the order of the waves.  The blocks behind clear rows.
 constexpr int kJoinBlock = kBlock;
@@ -647,6 +719,55 @@ int32_t launch_embedding(hipStream_t stream, const EmbeddingArgs& a) {
   });
 }
 
+static Sums sums_of(const EmbeddingGradientArgs& a) {
+  Sums s{};
+  s.count = a.count;
+  s.vocabulary = a.vocabulary;
+  s.dimension = a.dimension;
+  s.grad_stride = a.grad_out_stride;
+  s.table_stride = a.table_stride;
+  s.scale = a.scale;
+  s.accumulate = a.accumulate;
+  return s;
+}
+// A block's rows of about kClearBytes, and the lanes that share one.
+template <typename TW> static void set_clear_shape(Sums& s, int width) {
+  s.clear_lanes_log2 = lanes_log2(s.dimension, width);
+  s.clear_rows = kBlock >> s.clear_lanes_log2;
+  while (2 * s.clear_rows * s.dimension * (int64_t)sizeof(TW) <= kClearBytes) s.clear_rows *= 2;
+}
+// Blocks that clear `rows` rows.
+static int64_t clear_blocks(const Sums& s, int64_t rows) {
+  const int64_t blocks = div_up(rows, s.clear_rows);
+  return blocks < kMaxBlocks ? blocks : kMaxBlocks;
+}
+
+static int32_t launch_gradient_of_few(hipStream_t stream, const EmbeddingGradientArgs& a) {
+  return with_type(a.grad_out_type, [&](auto tg) {
+    return with_type(a.table_type, [&](auto tw) {
+      return with_token_type(a.token_type, [&](auto tt) -> int32_t {
+        using TG = decltype(tg);
+        using TW = decltype(tw);
+        using TT = decltype(tt);
+        constexpr int kWide = Width<TG, TW>::value;
+        const int W = a.dimension >= kWide ? kWide : 1;
+        Sums s = sums_of(a);
+        set_clear_shape<TW>(s, W);
+        {
+          ProfileScope scope(stream, "embedding_gradient_of_few");
+          hipLaunchKernelGGL((W == 1 ? embedding_gradient_of_few_kernel<TG, TW, TT, 1>
+                                     : embedding_gradient_of_few_kernel<TG, TW, TT, kWide>),
+                             dim3((unsigned)clear_blocks(s, a.vocabulary)), dim3(kBlock), 0, stream,
+                             s, static_cast<const TT*>(a.tokens), a.padding_token,
+                             static_cast<const TG*>(a.grad_out), static_cast<TW*>(a.grad_table));
+        }
+        ILGPU_HIP_CHECK(hipGetLastError());
+        return ILGPU_HIP_SUCCESS;
+      });
+    });
+  });
+}
+
 int64_t embedding_gradient_temp_bytes(int64_t count, int64_t vocabulary, int64_t dimension) {
   return gradient_temp(count, vocabulary, dimension).bytes;
 }
@@ -657,6 +778,7 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
     const int32_t rc = check_sort_device(stream);  // before anything is launched
     if (rc != ILGPU_HIP_SUCCESS) return rc;
   }
+  if (a.count <= kFewTokens) return launch_gradient_of_few(stream, a);
   const GradientTemp t = gradient_temp(a.count, a.vocabulary, a.dimension);
   char* base = reinterpret_cast<char*>(align_up((int64_t)(uintptr_t)a.temp, 256));
   uint32_t* keys = reinterpret_cast<uint32_t*>(base + t.keys);
@@ -714,31 +836,31 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
       // (That many chunks and slices have parts of 2^42 bytes: no device holds such a temp.)
       if (t.chunks * join_slices > INT32_MAX) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
       const int64_t sum_blocks = div_up(t.chunks * slices, kBlock >> log2);
+      const int64_t items = t.chunks > 2 ? (t.chunks - 2) * join_slices : 0;
+      const int64_t join_blocks = items < kJoinBlocks ? items : kJoinBlocks;
+      Sums s = sums_of(a);
+      s.met = groups ? reinterpret_cast<const uint64_t*>(base + t.met) : nullptr;
+      s.group_log2 = group_log2(a.vocabulary);
+      s.crossings = crossings;
+      s.parts = reinterpret_cast<float*>(base + t.parts);
+      s.chunks = t.chunks;
+      s.part_stride = t.part_stride;
+      s.chunk = t.chunk;
+      s.slices = (uint32_t)slices;
+      s.join_slices = (uint32_t)join_slices;
+      s.sum_blocks = (uint32_t)sum_blocks;
+      s.join_blocks = (uint32_t)join_blocks;
+      s.lanes_log2 = log2;
+      set_clear_shape<TW>(s, 16 / sizeof(TW));
       // Rows cleared beside the join are as many as it has time for while it waits for its
       // own reads; those before them keep the memory busy while the sums wait for theirs
       // (8192 tokens into 50021 x 1024: 43.6 us, 46.9 with all of them beside the sums, 56.9
       // with all beside the join).
       const int64_t late = kLateBytes / ((int64_t)sizeof(TW) * a.dimension);
-      const int64_t row_bytes = (int64_t)sizeof(TW) * a.dimension;
-      const int clear_log2 = lanes_log2(a.dimension, 16 / sizeof(TW));
-      int64_t clear_rows = kBlock >> clear_log2;
-      while (2 * clear_rows * row_bytes <= kClearBytes) clear_rows *= 2;
-      const int64_t early_rows =
-          a.accumulate || a.vocabulary <= late ? 0 : (a.vocabulary - late) / clear_rows * clear_rows;
-      const auto clear_blocks = [&](int64_t rows) {
-        const int64_t blocks = div_up(rows, clear_rows);
-        return blocks < kMaxBlocks ? blocks : kMaxBlocks;
-      };
-      const int64_t early_blocks = clear_blocks(early_rows);
-      const int64_t late_blocks = a.accumulate ? 0 : clear_blocks(a.vocabulary - early_rows);
-      const int64_t items = t.chunks > 2 ? (t.chunks - 2) * join_slices : 0;
-      const int64_t join_blocks = items < kJoinBlocks ? items : kJoinBlocks;
-      const Sums s{groups ? reinterpret_cast<const uint64_t*>(base + t.met) : nullptr,
-                   group_log2(a.vocabulary), crossings, reinterpret_cast<float*>(base + t.parts), a.count,
-                   t.chunks, t.part_stride, t.chunk, a.vocabulary, a.dimension, a.grad_out_stride,
-                   a.table_stride, a.scale, a.accumulate, (uint32_t)slices,
-                   (uint32_t)join_slices, (uint32_t)sum_blocks, (uint32_t)join_blocks,
-                   early_rows, (int32_t)clear_rows, clear_log2, log2};
+      if (!a.accumulate && a.vocabulary > late)
+        s.early_rows = (a.vocabulary - late) / s.clear_rows * s.clear_rows;
+      const int64_t early_blocks = clear_blocks(s, s.early_rows);
+      const int64_t late_blocks = a.accumulate ? 0 : clear_blocks(s, a.vocabulary - s.early_rows);
       if (sum_blocks + early_blocks > 0) {
         ProfileScope scope(stream, "embedding_gradient");
         const auto kernel_of = [&](auto chunk) {

@@ -227,9 +227,10 @@ def test_embedding_gradient_of_skewed_tokens(n, distribution):
 
 
 @pytest.mark.parametrize("table_type", TYPES)
-def test_embedding_gradient_accumulates_and_skips_padding(table_type):
+@pytest.mark.parametrize("n", [40, 3000])
+def test_embedding_gradient_accumulates_and_skips_padding(n, table_type):
     import torch
-    vocabulary, n = 700, 3000
+    vocabulary = 700
     g = _rng(11)
     grad = _normal(g, n, 65, dtype=torch.float16)
     tokens = _tokens(g, n, vocabulary, torch.int32)
@@ -261,10 +262,11 @@ def test_embedding_gradient_of_no_tokens_and_of_broadcast_rows():
     assert out[:, 0].tolist() == [17.0, 16.5, 16.5, 0.0]
 
 
-def test_embedding_gradient_strides():
+@pytest.mark.parametrize("n", [50, 900])
+def test_embedding_gradient_strides(n):
     import torch
-    grad = _normal(_rng(21), 900, 35, dtype=torch.bfloat16)
-    tokens = _tokens(_rng(22), 900, 60, torch.int64)
+    grad = _normal(_rng(21), n, 35, dtype=torch.bfloat16)
+    tokens = _tokens(_rng(22), n, 60, torch.int64)
     g_view, _, _ = _strided(grad, 41, 1)
     o_view, o_memory, guard = _strided(torch.zeros(60, 35, device="cuda"), 37, 1)
     from ilgpu_amd import capi
