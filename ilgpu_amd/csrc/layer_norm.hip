@@ -47,34 +47,44 @@ template <int LANES> __device__ __forceinline__ float lanes_sum(float v) {
   }
 }
 
-// The sum over LANES threads that share a row (lanes of a wave, or a whole block), in all of
-// them. `slot` is LDS of one float per wave that no thread still reads: two slots taken in
-// turn.
-template <int LANES> __device__ __forceinline__ float row_sum(float v, float* slot) {
-  if constexpr (LANES <= kWaveSize) {
-    return lanes_sum<LANES>(v);
-  } else {
-    v = lanes_sum<kWaveSize>(v);
-    if ((threadIdx.x & (kWaveSize - 1)) == 0) slot[threadIdx.x / kWaveSize] = v;
-    __syncthreads();
-    float sum = slot[0];
-#pragma unroll
-    for (int w = 1; w < LANES / kWaveSize; ++w) sum += slot[w];
-    return sum;
-  }
+// LANES is the number of lanes of a wave that share a row (8, 16, 32, 64), or kWholeBlock: all
+// threads of a block do, as many as the row's length asks for.
+constexpr int kWholeBlock = 1024;
+template <int LANES> __device__ __forceinline__ int row_lanes() {
+  return LANES == kWholeBlock ? blockDim.x : LANES;
 }
-
 // A thread's place in its row, and its row among those a block has at a time.
 template <int LANES> __device__ __forceinline__ int row_lane() {
-  return LANES <= kWaveSize ? threadIdx.x & (LANES - 1) : threadIdx.x;
+  return LANES == kWholeBlock ? threadIdx.x : threadIdx.x & (LANES - 1);
 }
 template <int LANES> __device__ __forceinline__ int row_of_block() {
-  if (LANES > kWaveSize) return 0;
+  if (LANES == kWholeBlock) return 0;
   const int row = threadIdx.x / LANES;
   return LANES == kWaveSize ? __builtin_amdgcn_readfirstlane(row) : row;
 }
 
-// The columns of a thread: V times W side by side, LANES * W apart.  Where a row ends
+// The sum over a block's waves of what each has in all of its lanes, in all threads. `slot` is
+// LDS of one float per wave (16 at most) that no thread still reads.
+__device__ __forceinline__ void put_wave(float v, float* slot) {
+  if ((threadIdx.x & (kWaveSize - 1)) == 0) slot[threadIdx.x / kWaveSize] = v;
+}
+__device__ __forceinline__ float sum_waves(const float* slot) {
+  const int i = threadIdx.x & 15;
+  return lanes_sum<16>(i < (int)(blockDim.x / kWaveSize) ? slot[i] : 0.0f);
+}
+
+// The sum over the threads that share a row, in all of them; two slots taken in turn.
+template <int LANES> __device__ __forceinline__ float row_sum(float v, float* slot) {
+  if constexpr (LANES <= kWaveSize) {
+    return lanes_sum<LANES>(v);
+  } else {
+    put_wave(lanes_sum<kWaveSize>(v), slot);
+    __syncthreads();
+    return sum_waves(slot);
+  }
+}
+
+// The columns of a thread: V times W side by side, W times the row's lanes apart.  Where a row ends
 // inside a thread's W columns, the thread reads the last W of the row and leaves those of
 // its neighbour (`skip` of them; W: all) alone, so every load is whole; columns >= W.
 template <int W, int LANES, int V> struct Columns {
@@ -82,11 +92,11 @@ template <int W, int LANES, int V> struct Columns {
   int skip[V];
   bool whole[V];  // every thread has W of its own
   __device__ __forceinline__ explicit Columns(int64_t columns) {
-    const int lane = row_lane<LANES>();
+    const int lane = row_lane<LANES>(), lanes = row_lanes<LANES>();
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      whole[v] = (int64_t)(v + 1) * LANES * W <= columns;
-      const int64_t c = (int64_t)(v * LANES + lane) * W;
+      whole[v] = (int64_t)(v + 1) * lanes * W <= columns;
+      const int64_t c = (int64_t)(v * lanes + lane) * W;
       at[v] = c + W <= columns ? c : columns - W;
       skip[v] = (int)(c - at[v] < W ? c - at[v] : W);
     }
@@ -155,16 +165,22 @@ template <int W, int LANES, int V> struct Columns {
 // with a block for every row, which loads its weights for it alone).
 constexpr int kWavesPerCu = 64;
 
+// The largest block, the threads of one, and the rows it has at a time.
+// Rows of more vectors have two in a thread (32768 x 4096: 512 vectors by 256 threads 98 us, by
+// 512 101.7).
+constexpr int kSingleVectors = 384;
+
 template <int LANES> constexpr int row_block() { return LANES <= kWaveSize ? kBlock : LANES; }
-template <int LANES> constexpr int row_waves() { return LANES <= kWaveSize ? 1 : LANES / kWaveSize; }
+template <int LANES> constexpr int block_rows() { return LANES <= kWaveSize ? kBlock / LANES : 1; }
+constexpr int kMostWaves = kWholeBlock / kWaveSize;
 
 template <typename T, typename TW, int W, int LANES, int V>
 __global__ __launch_bounds__(row_block<LANES>()) void layer_norm_kernel(
     const T* in, int64_t rows, int64_t columns, int64_t in_stride, const TW* __restrict__ weight,
     const TW* __restrict__ bias, float epsilon, T* out, int64_t out_stride,
     float* __restrict__ mean, float* __restrict__ rstd) {
-  constexpr int kRows = row_block<LANES>() / LANES;  // at a time
-  __shared__ float lds[2][row_waves<LANES>()];
+  constexpr int kRows = block_rows<LANES>();
+  __shared__ float lds[2][kMostWaves];
   const Columns<W, LANES, V> own(columns);
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + row_of_block<LANES>();
@@ -203,7 +219,7 @@ __global__ __launch_bounds__(row_block<LANES>()) void layer_norm_kernel(
 
 // Rows too long for the registers: a block reads each of them three times, the second and
 // third time from the caches.
-constexpr int kLongBlock = 1024;
+constexpr int kLongBlock = kWholeBlock;
 template <typename T, typename TW>
 __global__ __launch_bounds__(kLongBlock) void layer_norm_long_kernel(
     const T* in, int64_t rows, int64_t columns, int64_t in_stride, const TW* __restrict__ weight,
@@ -251,64 +267,36 @@ __global__ __launch_bounds__(kLongBlock) void layer_norm_long_kernel(
   }
 }
 
-// How a row of `columns` elements of T is shared: V * LANES * W of them at most.  The lanes
-// follow the length, as idle ones take registers and issue like others (gradients of 2^26
-// bfloat16 elements, us: rows of 64 by a wave 461, by 8 lanes 80; rows of 3000 by 512 lanes
-// 103, by 384 95).  Calls f(W, LANES, V) with integral constants, or `otherwise` for rows
-// beyond.
-#define ILGPU_HIP_SHAPE(w, lanes, v)                                                       \
-  f(std::integral_constant<int, w>(), std::integral_constant<int, lanes>(), \
-    std::integral_constant<int, v>())
+// How a row of `columns` elements of T is shared: by 8 to 64 lanes, or by a block of as many
+// waves as its length asks for, each thread with V vectors.  Idle lanes and waves cost like
+// others (gradients of bfloat16, us: 2^20 rows of 64 by a wave 461, by 8 lanes 80; 21440 rows of
+// 2368 by six waves 78, by five 71).  Calls f(W, LANES, V, threads) with integral constants but for
+// `threads`, which is the block's, or `otherwise` for rows beyond; V is 1 up to `single`
+// vectors.
 template <typename T, typename F, typename G>
-int32_t with_shape(int64_t columns, F f, G otherwise) {
+int32_t with_shape(int64_t columns, int64_t single, F f, G otherwise) {
   constexpr int W = 16 / sizeof(T);
-  if (columns < W) return ILGPU_HIP_SHAPE(1, 8, 1);
+  const auto shape = [&](auto w, auto lanes, auto v, int64_t vectors) {
+    return f(w, lanes, v, (int)align_up(div_up(vectors, decltype(v)::value), kWaveSize));
+  };
+  using std::integral_constant;
+#define ILGPU_HIP_SHAPE(w, lanes, v) \
+  shape(integral_constant<int, w>(), integral_constant<int, lanes>(), integral_constant<int, v>(), vectors)
   const int64_t vectors = div_up(columns, W);
+  if (columns < W) return ILGPU_HIP_SHAPE(1, 8, 1);
   if (vectors <= 8) return ILGPU_HIP_SHAPE(W, 8, 1);
   if (vectors <= 16) return ILGPU_HIP_SHAPE(W, 16, 1);
   if (vectors <= 32) return ILGPU_HIP_SHAPE(W, 32, 1);
   if (vectors <= 64) return ILGPU_HIP_SHAPE(W, 64, 1);
   if (vectors <= 128) return ILGPU_HIP_SHAPE(W, 64, 2);
-  if (vectors <= 192) return ILGPU_HIP_SHAPE(W, 192, 1);
-  if (vectors <= 256) return ILGPU_HIP_SHAPE(W, 256, 1);
-  if (vectors <= 384) return ILGPU_HIP_SHAPE(W, 384, 1);
-  if (vectors <= 512) return ILGPU_HIP_SHAPE(W, 256, 2);
-  if (vectors <= 768) return ILGPU_HIP_SHAPE(W, 384, 2);
-  if (vectors <= 1024) return ILGPU_HIP_SHAPE(W, 512, 2);
-  if (vectors <= 1536) return ILGPU_HIP_SHAPE(W, 768, 2);
-  if (vectors <= 2048) return ILGPU_HIP_SHAPE(W, 1024, 2);
+  if (vectors <= single) return ILGPU_HIP_SHAPE(W, kWholeBlock, 1);
+  if (vectors <= 2048) return ILGPU_HIP_SHAPE(W, kWholeBlock, 2);
   if constexpr (W == 4) {
-    if (vectors <= 3072) return ILGPU_HIP_SHAPE(W, 768, 4);
-    if (vectors <= 4096) return ILGPU_HIP_SHAPE(W, 1024, 4);
+    if (vectors <= 4096) return ILGPU_HIP_SHAPE(W, kWholeBlock, 4);
   }
-  return otherwise();
-}
-// The same for the gradients, which hold more of a row.
-template <typename T, typename F, typename G>
-int32_t with_gradient_shape(int64_t columns, F f, G otherwise) {
-  constexpr int W = 16 / sizeof(T);
-  if (columns < W) return ILGPU_HIP_SHAPE(1, 8, 1);
-  const int64_t vectors = div_up(columns, W);
-  if (vectors <= 8) return ILGPU_HIP_SHAPE(W, 8, 1);
-  if (vectors <= 16) return ILGPU_HIP_SHAPE(W, 16, 1);
-  if (vectors <= 32) return ILGPU_HIP_SHAPE(W, 32, 1);
-  if (vectors <= 64) return ILGPU_HIP_SHAPE(W, 64, 1);
-  if (vectors <= 128) return ILGPU_HIP_SHAPE(W, 64, 2);
-  if (vectors <= 192) return ILGPU_HIP_SHAPE(W, 192, 1);
-  if (vectors <= 256) return ILGPU_HIP_SHAPE(W, 256, 1);
-  if (vectors <= 384) return ILGPU_HIP_SHAPE(W, 384, 1);
-  if (vectors <= 512) return ILGPU_HIP_SHAPE(W, 512, 1);
-  if (vectors <= 768) return ILGPU_HIP_SHAPE(W, 768, 1);
-  if (vectors <= 1024) return ILGPU_HIP_SHAPE(W, 1024, 1);
-  if (vectors <= 1536) return ILGPU_HIP_SHAPE(W, 768, 2);
-  if (vectors <= 2048) return ILGPU_HIP_SHAPE(W, 1024, 2);
-  if constexpr (W == 4) {
-    if (vectors <= 3072) return ILGPU_HIP_SHAPE(W, 768, 4);
-    if (vectors <= 4096) return ILGPU_HIP_SHAPE(W, 1024, 4);
-  }
-  return otherwise();
-}
 #undef ILGPU_HIP_SHAPE
+  return otherwise();
+}
 
 // Weights have the rows' type or float32.
 template <typename F> int32_t with_norm_types(int32_t type, int32_t weight_type, F f) {
@@ -342,11 +330,11 @@ __global__ __launch_bounds__(gradient_block<LANES>()) void layer_norm_gradient_k
     const float* __restrict__ rstd, T* grad_in, int64_t grad_in_stride,
     float* __restrict__ partials, int32_t accumulate, TW* __restrict__ grad_weight,
     TW* __restrict__ grad_bias) {
-  constexpr int kRows = gradient_block<LANES>() / LANES;  // at a time
-  constexpr int kJoins = LANES <= kWaveSize ? gradient_block<LANES>() / kWaveSize : 1;
+  constexpr int kRows = LANES <= kWaveSize ? kGradientBlock / LANES : 1;  // at a time
+  constexpr int kJoins = LANES <= kWaveSize ? kGradientBlock / kWaveSize : 1;
   // The next row on its way costs registers that a large block does not have.
   constexpr bool kAhead = LANES * V * W < 1024 * 16;
-  __shared__ float lds[2][2][row_waves<LANES>()];
+  __shared__ float lds[2][2][kMostWaves];
   __shared__ float joined[kJoins > 1 ? kJoins : 1][kJoins > 1 ? LANES * V * W : 1];
   const Columns<W, LANES, V> own(columns);
   const int64_t step = (int64_t)gridDim.x * kRows;
@@ -386,19 +374,11 @@ __global__ __launch_bounds__(gradient_block<LANES>()) void layer_norm_gradient_k
     float mean_g = lanes_sum<kTogether>(own.sum([&](int v, int k) { return g[v][k]; }));
     float mean_gh = lanes_sum<kTogether>(own.sum([&](int v, int k) { return g[v][k] * h[v][k]; }));
     if (LANES > kWaveSize) {
-      const int wave = threadIdx.x / kWaveSize;
-      if ((threadIdx.x & (kWaveSize - 1)) == 0) {
-        lds[turn][0][wave] = mean_g;
-        lds[turn][1][wave] = mean_gh;
-      }
+      put_wave(mean_g, lds[turn][0]);
+      put_wave(mean_gh, lds[turn][1]);
       __syncthreads();
-      mean_g = lds[turn][0][0];
-      mean_gh = lds[turn][1][0];
-#pragma unroll
-      for (int i = 1; i < LANES / kWaveSize; ++i) {
-        mean_g += lds[turn][0][i];
-        mean_gh += lds[turn][1][i];
-      }
+      mean_g = sum_waves(lds[turn][0]);
+      mean_gh = sum_waves(lds[turn][1]);
     }
     mean_g /= (float)columns;
     mean_gh /= (float)columns;
@@ -568,14 +548,15 @@ int32_t launch_layer_norm(hipStream_t stream, const LayerNormArgs& a) {
       return ILGPU_HIP_SUCCESS;
     };
     return with_shape<T>(
-        a.columns,
-        [&](auto w, auto lanes, auto v) {
-          constexpr int kThreads = row_block<decltype(lanes)::value>();
-          const int64_t blocks = div_up(a.rows, kThreads / decltype(lanes)::value);
-          const int64_t most = (int64_t)device_cu_count() * (kWavesPerCu * kWaveSize / kThreads);
-          return launch(layer_norm_kernel<T, TW, decltype(w)::value, decltype(lanes)::value,
-                                          decltype(v)::value>,
-                        blocks < most ? blocks : most, kThreads);
+        a.columns, kSingleVectors,
+        [&](auto w, auto lanes, auto v, int row_threads) {
+          constexpr int kLanes = decltype(lanes)::value;
+          const int threads = kLanes == kWholeBlock ? row_threads : kBlock;
+          const int64_t blocks = div_up(a.rows, block_rows<kLanes>());
+          const int64_t most = (int64_t)device_cu_count() * (kWavesPerCu * kWaveSize / threads);
+          return launch(
+              layer_norm_kernel<T, TW, decltype(w)::value, kLanes, decltype(v)::value>,
+              blocks < most ? blocks : most, threads);
         },
         [&] {
           return launch(layer_norm_long_kernel<T, TW>, a.rows < kMaxBlocks ? a.rows : kMaxBlocks,
@@ -611,21 +592,23 @@ int32_t launch_layer_norm_gradient(hipStream_t stream, const LayerNormGradientAr
       return ILGPU_HIP_SUCCESS;
     };
     if (a.rows == 0) return fold(0);
-    return with_gradient_shape<T>(
-        a.columns,
-        [&](auto w, auto lanes, auto v) -> int32_t {
+    return with_shape<T>(
+        a.columns, kWholeBlock,
+        [&](auto w, auto lanes, auto v, int row_threads) -> int32_t {
           constexpr int kLanes = decltype(lanes)::value;
-          constexpr int kThreads = gradient_block<kLanes>();
-          const int64_t blocks = div_up(a.rows, kThreads / kLanes);
-          constexpr int kPerCu = kGradientWavesPerCu * kWaveSize / kThreads;
-          static_assert(kPerCu <= kMaxSplitsPerCu, "rows of partials");
-          const int64_t most = (int64_t)device_cu_count() * (kPerCu > 1 ? kPerCu : 1);
-          const int64_t splits = blocks < most ? blocks : most;
+          const int threads = kLanes == kWholeBlock ? row_threads : kGradientBlock;
+          const int64_t blocks =
+              div_up(a.rows, kLanes == kWholeBlock ? 1 : kGradientBlock / kLanes);
+          int64_t per_cu = kGradientWavesPerCu * kWaveSize / threads;
+          per_cu = per_cu < 1 ? 1 : per_cu < kMaxSplitsPerCu ? per_cu : kMaxSplitsPerCu;
+          const int64_t most = device_cu_count() * per_cu;
+          // (Four turns of one block take less than the fold's launch.)
+          const int64_t splits = blocks <= 4 ? 1 : blocks < most ? blocks : most;
           {
             ProfileScope scope(stream, "layer_norm_gradient");
             hipLaunchKernelGGL(
                 (layer_norm_gradient_kernel<T, TW, decltype(w)::value, kLanes, decltype(v)::value>),
-                dim3((unsigned)splits), dim3(kThreads), 0, stream, grad_out, a.grad_out_stride, in,
+                dim3((unsigned)splits), dim3(threads), 0, stream, grad_out, a.grad_out_stride, in,
                 a.in_stride, a.rows, a.columns, weight, a.mean, a.rstd, grad_in, a.grad_in_stride,
                 sums ? partials : nullptr, a.accumulate, static_cast<TW*>(a.grad_weight),
                 static_cast<TW*>(a.grad_bias));
