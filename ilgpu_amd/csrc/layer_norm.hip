@@ -165,10 +165,11 @@ template <int W, int LANES, int V> struct Columns {
 // with a block for every row, which loads its weights for it alone).
 constexpr int kWavesPerCu = 64;
 
-// The largest block, the threads of one, and the rows it has at a time.
 // Rows of more vectors have two in a thread (32768 x 4096: 512 vectors by 256 threads 98 us, by
 // 512 101.7).
 constexpr int kSingleVectors = 384;
+
+// The largest block, and the rows it has at a time.
 
 template <int LANES> constexpr int row_block() { return LANES <= kWaveSize ? kBlock : LANES; }
 template <int LANES> constexpr int block_rows() { return LANES <= kWaveSize ? kBlock / LANES : 1; }
