@@ -121,7 +121,9 @@ constexpr int kGroupWaves = kGroupBlock / kWaveSize;
 constexpr int kGroupMinLog2 = 8;          // blocks: one per compute unit
 constexpr int kGroupMaxLog2 = 10;
 constexpr int kGroupRows = 1024;          // most tokens a block gathers
-constexpr int kGroupList = 1024;          // places a wave remembers; beyond it reads again
+// Places a wave remembers; beyond them it reads its tokens again.  (Two blocks of up to 2^17
+// table rows fit a compute unit with 512.)
+inline int group_list(int64_t count) { return count <= (1 << 16) ? 512 : 1024; }
 constexpr int kGroupCountLog2 = 17;       // most tokens in all: place and row share a word
 static_assert(((uint64_t)kGroupRows << kGroupCountLog2) <= (1ull << 32), "a word");
 
@@ -140,17 +142,52 @@ inline bool takes_groups(int64_t count, int64_t vocabulary) {
          count <= ((int64_t)1 << (kGroupCountLog2 + kGroupMinLog2 - log2));
 }
 
+// The table's last rows from `first` on, which further blocks of the grouping clear, met or
+// not: the sums of those that are met come later.  In units of 16 bits, whatever the type.  As
+// many bytes as are written while the grouping computes, whose blocks leave room for a second
+// one on a compute unit (64 registers; with more of them nothing is gained): 8192 tokens into
+// 50021 x 1024 42.4 to 39.4 us, 65536 into 131072 x 2048 260 to 255.
+constexpr int64_t kGroupClearBytes = 24 << 20, kGroupClearPerToken = 900;
+struct Clearing {
+  uint16_t* table;
+  int64_t first, rows, columns, stride;
+  int lanes_log2;
+};
+
+__device__ __forceinline__ void clear_all(const Clearing& t, uint32_t block, uint32_t blocks) {
+  constexpr int W = 8;
+  const typename Pack<uint16_t, W>::vec zeros = {};
+  const int64_t at_once = kGroupBlock >> t.lanes_log2;
+  for (int64_t r = t.first + block * at_once + (threadIdx.x >> t.lanes_log2); r < t.rows;
+       r += blocks * at_once) {
+    uint16_t* row = t.table + r * t.stride;
+    for (int64_t c = (int64_t)(threadIdx.x & ((1u << t.lanes_log2) - 1)) * W; c < t.columns;
+         c += (int64_t)W << t.lanes_log2) {
+      if (c + W <= t.columns) {
+        __builtin_nontemporal_store(zeros, reinterpret_cast<typename Pack<uint16_t, W>::type*>(row + c));
+      } else {
+        for (int64_t k = c; k < t.columns; ++k) row[k] = 0;
+      }
+    }
+  }
+}
+
 template <typename TT>
-__global__ __launch_bounds__(kGroupBlock) void group_tokens_kernel(
+__global__ __launch_bounds__(kGroupBlock, 8) void group_tokens_kernel(
     const TT* __restrict__ tokens, int64_t count, int64_t padded, int64_t vocabulary,
-    int64_t padding_token, int log2, int rows, uint32_t* __restrict__ keys,
-    uint32_t* __restrict__ order, uint64_t* __restrict__ met, uint32_t* __restrict__ crossings) {
+    int64_t padding_token, int log2, int rows, uint32_t list_length, uint32_t* __restrict__ keys,
+    uint32_t* __restrict__ order, uint64_t* __restrict__ met, uint32_t* __restrict__ crossings,
+    Clearing clearing) {
   extern __shared__ uint32_t group_lds[];
   __shared__ uint32_t wave_rows[kGroupWaves], wave_below[kGroupWaves];
-  const uint32_t group = blockIdx.x, groups = gridDim.x;
+  const uint32_t group = blockIdx.x, groups = 1u << log2;
+  if (group >= groups) {
+    clear_all(clearing, group - groups, gridDim.x - groups);
+    return;
+  }
   const int wave = threadIdx.x / kWaveSize, lane = threadIdx.x & (kWaveSize - 1);
   uint32_t* const counters = group_lds + wave * rows;
-  uint32_t* const list = group_lds + kGroupWaves * rows + wave * kGroupList;
+  uint32_t* const list = group_lds + kGroupWaves * rows + wave * list_length;
   if (group == 0 && threadIdx.x == 0) crossings[0] = 0;
   for (int i = threadIdx.x; i < kGroupWaves * rows; i += kGroupBlock) group_lds[i] = 0;
   __syncthreads();
@@ -216,11 +253,11 @@ __global__ __launch_bounds__(kGroupBlock) void group_tokens_kernel(
     const uint64_t owns = __builtin_amdgcn_ballot_w64(of == group);
     if (owns != 0) {
       const uint32_t place = listed + mbcnt(owns);
-      if (of == group && place < kGroupList) list[place] = (token >> log2) << kGroupCountLog2 | at;
+      if (of == group && place < list_length) list[place] = (token >> log2) << kGroupCountLog2 | at;
       listed += __popcll(owns);
     }
   });
-  if (listed <= kGroupList) {
+  if (listed <= list_length) {
     for (uint32_t j = lane; j < listed; j += kWaveSize) count_row(list[j] >> kGroupCountLog2);
   } else {
     scan([&](uint32_t, uint32_t token, uint32_t of) {
@@ -260,7 +297,7 @@ __global__ __launch_bounds__(kGroupBlock) void group_tokens_kernel(
   }
   __syncthreads();
 
-  if (listed <= kGroupList) {
+  if (listed <= list_length) {
     for (uint32_t j = lane; j < listed; j += kWaveSize) {
       const uint32_t row = list[j] >> kGroupCountLog2;
       const uint32_t to = count_row(row);
@@ -298,7 +335,7 @@ struct Sums {
   uint32_t join_slices;
   uint32_t sum_blocks;   // blocks of the sums and of the join; further ones clear rows,
   uint32_t join_blocks;  // those from early_rows on beside the join
-  int64_t early_rows;
+  int64_t early_rows, late_end;
   int32_t clear_rows;    // rows a block clears, lanes that share one
   int32_t clear_lanes_log2;
   int lanes_log2;        // lanes that share a row
@@ -595,7 +632,7 @@ __global__ __launch_bounds__(kJoinBlock) void join_runs_kernel(
     Sums s, const uint32_t* __restrict__ keys, TW* __restrict__ table) {
   constexpr int W = 4;
   if (blockIdx.x >= s.join_blocks) {
-    clear_rows(s, keys, table, s.early_rows, s.vocabulary, blockIdx.x - s.join_blocks,
+    clear_rows(s, keys, table, s.early_rows, s.late_end, blockIdx.x - s.join_blocks,
                gridDim.x - s.join_blocks);
     return;
   }
@@ -785,18 +822,34 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
   uint32_t* order = reinterpret_cast<uint32_t*>(base + t.order);
   uint32_t* crossings = reinterpret_cast<uint32_t*>(base + t.crossings);
   const bool groups = a.count > 0 && takes_groups(a.count, a.vocabulary);
+  int64_t rows_left = a.vocabulary;  // in front of those that are cleared beside the grouping
+  unsigned clearing_blocks = 0;
+  Clearing clearing{};
+  if (groups && !a.accumulate) {
+    const int64_t units = operator_elem_size(a.table_type) / 2;
+    clearing = {static_cast<uint16_t*>(a.grad_table), 0, a.vocabulary, a.dimension * units,
+                a.table_stride * units, 0};
+    while ((1 << clearing.lanes_log2) < kGroupBlock && (8 << clearing.lanes_log2) < clearing.columns)
+      ++clearing.lanes_log2;
+    const int64_t some = (kGroupClearBytes + a.count * kGroupClearPerToken) / (clearing.columns * 2);
+    rows_left = a.vocabulary > some ? a.vocabulary - some : 0;
+    clearing.first = rows_left;
+    const int64_t blocks =
+        div_up(a.vocabulary - rows_left, kGroupBlock >> clearing.lanes_log2);
+    clearing_blocks = (unsigned)(blocks < kMaxBlocks / 8 ? blocks : kMaxBlocks / 8);
+  }
   if (groups) {
     const int32_t rc = with_token_type(a.token_type, [&](auto tt) -> int32_t {
       using TT = decltype(tt);
       const int log2 = group_log2(a.vocabulary);
-      const int rows = (int)div_up(a.vocabulary, (int64_t)1 << log2);
+      const int rows = (int)div_up(a.vocabulary, (int64_t)1 << log2), list = group_list(a.count);
       {
         ProfileScope scope(stream, "embedding_group_tokens");
-        hipLaunchKernelGGL((group_tokens_kernel<TT>), dim3(1u << log2), dim3(kGroupBlock),
-                           (unsigned)(kGroupWaves * (rows + kGroupList) * 4), stream,
+        hipLaunchKernelGGL((group_tokens_kernel<TT>), dim3((1u << log2) + clearing_blocks),
+                           dim3(kGroupBlock), (unsigned)(kGroupWaves * (rows + list) * 4), stream,
                            static_cast<const TT*>(a.tokens), a.count, t.padded, a.vocabulary,
-                           a.padding_token, log2, rows, keys, order,
-                           reinterpret_cast<uint64_t*>(base + t.met), crossings);
+                           a.padding_token, log2, rows, (uint32_t)list, keys, order,
+                           reinterpret_cast<uint64_t*>(base + t.met), crossings, clearing);
       }
       ILGPU_HIP_CHECK(hipGetLastError());
       return ILGPU_HIP_SUCCESS;
@@ -857,10 +910,11 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
       // (8192 tokens into 50021 x 1024: 43.6 us, 46.9 with all of them beside the sums, 56.9
       // with all beside the join).
       const int64_t late = kLateBytes / ((int64_t)sizeof(TW) * a.dimension);
-      if (!a.accumulate && a.vocabulary > late)
-        s.early_rows = (a.vocabulary - late) / s.clear_rows * s.clear_rows;
+      s.late_end = rows_left;
+      if (!a.accumulate && s.late_end > late)
+        s.early_rows = (s.late_end - late) / s.clear_rows * s.clear_rows;
       const int64_t early_blocks = clear_blocks(s, s.early_rows);
-      const int64_t late_blocks = a.accumulate ? 0 : clear_blocks(s, a.vocabulary - s.early_rows);
+      const int64_t late_blocks = a.accumulate ? 0 : clear_blocks(s, s.late_end - s.early_rows);
       if (sum_blocks + early_blocks > 0) {
         ProfileScope scope(stream, "embedding_gradient");
         const auto kernel_of = [&](auto chunk) {
