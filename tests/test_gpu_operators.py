@@ -321,6 +321,26 @@ def test_offsets_beyond_32_bits():
     _close(out.to(torch.bfloat16), exact, U * grad.double().abs().sum(0))
 
 
+@pytest.mark.parametrize("n", [60, 300, 5000])
+def test_embedding_gradient_keeps_bad_rows_to_their_tokens(n):
+    import torch
+    vocabulary = 97
+    g = _rng(n, 51)
+    grad = _normal(g, n, 300, dtype=torch.bfloat16)
+    tokens = torch.randint(0, vocabulary, (n,), generator=g, device="cuda")
+    good = _embedding_gradient(grad, tokens, vocabulary, torch.float32)
+    bad = [int(tokens[k]) for k in (3, n // 2, n - 1)]
+    grad[3], grad[n // 2, 7], grad[n - 1, 299] = float("nan"), float("inf"), float("nan")
+    out = _embedding_gradient(grad, tokens, vocabulary, torch.float32)
+    kept = torch.ones(vocabulary, dtype=torch.bool, device="cuda")
+    kept[bad] = False
+    assert torch.equal(out[kept], good[kept])
+    assert bool(out[bad[0]].isnan().all()) and not bool(torch.isfinite(out[bad[1], 7]))
+    others = torch.arange(300, device="cuda") != 7
+    if bad[1] not in (bad[0], bad[2]):
+        assert torch.equal(out[bad[1], others], good[bad[1], others])
+
+
 # ---- layer norm -------------------------------------------------------------------
 def _layer_norm(x, weight, bias, epsilon=1e-5, out=None):
     import torch
@@ -426,6 +446,23 @@ def test_layer_norm_keeps_bad_rows_to_themselves():
     bad = torch.zeros(64, dtype=torch.bool, device="cuda")
     bad[[5, 17, 40]] = True
     assert torch.equal(out[~bad], good[~bad]) and bool(out[bad].isnan().all())
+
+
+def test_layer_norm_of_rows_beyond_32_bit_offsets():
+    import torch
+    # three rows 2^30 elements apart: the last one begins at element 2^31
+    rows, columns, stride = 3, 100, 1 << 30
+    memory = torch.zeros(2 * stride + columns, dtype=torch.bfloat16, device="cuda")
+    view = torch.as_strided(memory, (rows, columns), (stride, 1))
+    x = _normal(_rng(95), rows, columns, dtype=torch.bfloat16)
+    view.copy_(x)
+    weight = _normal(_rng(96), columns, dtype=torch.float32)
+    grad = _normal(_rng(97), rows, columns, dtype=torch.bfloat16)
+    mean, rstd = _statistics(x)
+    result = _layer_norm_gradient(grad, view, weight, mean, rstd, torch.float32)
+    _check_layer_norm_gradient(result, grad, x, weight, mean, rstd)
+    out, mean, rstd = _layer_norm(view, weight, None, out=view)
+    _check_layer_norm(out, mean, rstd, x, weight, None)
 
 
 def test_layer_norm_of_no_rows():
@@ -683,6 +720,19 @@ def test_gradient_norm_of_unaligned_tensors():
             assert torch.equal(memory[a:b], kept[a:b])
         wide = kept[30_001:49_999].double() * 0.5
         _close(parts[2], wide, 3 * U * wide.abs())
+
+
+def test_gradient_norm_of_a_tensor_beyond_32_bits():
+    import torch
+    from ilgpu_amd import capi
+    array = capi.DeviceArray.from_tensor
+    n = (1 << 31) + 5
+    t = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    t[0], t[n // 2], t[n - 1] = 3.0, 4.0, 12.0
+    norm = _norm([t])
+    assert float(norm) == 13.0
+    capi.clip_gradients([array(t)], array(norm), 6.5)
+    assert [float(t[k]) for k in (0, 1, n // 2, n - 2, n - 1)] == [1.5, 0.0, 2.0, 0.0, 6.0]
 
 
 # ---- streams and graphs -------------------------------------------------------------
