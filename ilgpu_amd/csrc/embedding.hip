@@ -85,7 +85,8 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(
 // by a wave each, whatever tokens they hold, so a token that fills half of the input
 // takes no longer than the rest: a run of one token goes straight into the table where
 // it ends before the next chunk does, parts of longer ones go into `parts` and are joined
-// by a second kernel.  Rows of no token are cleared by further blocks of both.
+// by a second kernel.  Rows of no token are cleared by further blocks of both and of the
+// grouping.
 constexpr int kChunk = 32, kShortChunk = 8;
 // Few and narrow rows fill the chip only in short chunks.
 inline int chunk_length(int64_t count, int64_t dimension) {
