@@ -10,6 +10,7 @@
 
 #include "elements.hpp"
 #include "kernels.hpp"
+#include "operators.hpp"
 
 namespace ilgpu_hip {
 

@@ -1,7 +1,7 @@
 // Embedding lookup, out[i] = scale * table[tokens[i]], and its gradient,
 // grad_table[v] = scale * sum of grad_out[i] over the positions of token v.
 #include "elements.hpp"
-#include "kernels.hpp"
+#include "operators.hpp"
 
 namespace ilgpu_hip {
 

@@ -10,7 +10,7 @@
 // 6.3 TB/s; both go past the caches.  The conversions and products of float64 stay behind
 // the loads.
 #include "elements.hpp"
-#include "kernels.hpp"
+#include "operators.hpp"
 
 namespace ilgpu_hip {
 

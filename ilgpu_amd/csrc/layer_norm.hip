@@ -10,7 +10,7 @@
 // 4096 bfloat16: 537 MB in 98 us, 5.5 TB/s (three readings from the caches, element by
 // element: 338).
 #include "elements.hpp"
-#include "kernels.hpp"
+#include "operators.hpp"
 
 namespace ilgpu_hip {
 
