@@ -361,7 +361,8 @@ __device__ __forceinline__ void finish_row(TW* to, const float (&sum)[W], int ow
   } else {
 #pragma unroll
     for (int k = 0; k < W; ++k)
-      if (k >= own) to[k] = (TW)(sum[k] * scale + (accumulate ? (float)to[k] : 0.0f));
+      if (k >= own)
+        to[k] = (TW)(accumulate ? sum[k] * scale + (float)to[k] : product_for<TW>(sum[k], scale));
   }
 }
 
@@ -806,18 +807,30 @@ static int32_t launch_gradient_of_few(hipStream_t stream, const EmbeddingGradien
   });
 }
 
+// Whether the sums' launch, with the blocks that clear rows, has fewer threads than a grid can
+// hold (2^32) and its items fit their 32 bits: not so only where the parts alone take 100 GB.
+static bool grid_holds(const GradientTemp& t, const EmbeddingGradientArgs& a) {
+  const int gb = operator_elem_size(a.grad_out_type), wb = operator_elem_size(a.table_type);
+  const int wide = 16 / (gb > wb ? gb : wb), W = a.dimension >= wide ? wide : 1;
+  const int all_log2 = lanes_log2(a.dimension, W), log2 = all_log2 < 6 ? all_log2 : 6;
+  const int64_t blocks = div_up(t.chunks * div_up(a.dimension, (int64_t)W << log2), kBlock >> log2);
+  return blocks + kMaxBlocks < (INT64_C(1) << 32) / kBlock &&
+         t.chunks * div_up(a.dimension, kWaveSize * 4) <= INT32_MAX;
+}
+
 int64_t embedding_gradient_temp_bytes(int64_t count, int64_t vocabulary, int64_t dimension) {
   return gradient_temp(count, vocabulary, dimension).bytes;
 }
 
 int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArgs& a) {
   if (a.vocabulary == 0) return ILGPU_HIP_SUCCESS;
+  const GradientTemp t = gradient_temp(a.count, a.vocabulary, a.dimension);
+  if (!grid_holds(t, a)) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
   if (a.count > 0) {
     const int32_t rc = check_sort_device(stream);  // before anything is launched
     if (rc != ILGPU_HIP_SUCCESS) return rc;
   }
   if (a.count <= kFewTokens) return launch_gradient_of_few(stream, a);
-  const GradientTemp t = gradient_temp(a.count, a.vocabulary, a.dimension);
   char* base = reinterpret_cast<char*>(align_up((int64_t)(uintptr_t)a.temp, 256));
   uint32_t* keys = reinterpret_cast<uint32_t*>(base + t.keys);
   uint32_t* order = reinterpret_cast<uint32_t*>(base + t.order);
@@ -887,8 +900,6 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
       const int log2 = all_log2 < 6 ? all_log2 : 6;
       const int64_t slices = div_up(a.dimension, (int64_t)W << log2);
       const int64_t join_slices = div_up(a.dimension, kWaveSize * 4);
-      // (That many chunks and slices have parts of 2^42 bytes: no device holds such a temp.)
-      if (t.chunks * join_slices > INT32_MAX) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
       const int64_t sum_blocks = div_up(t.chunks * slices, kBlock >> log2);
       const int64_t items = t.chunks > 2 ? (t.chunks - 2) * join_slices : 0;
       const int64_t join_blocks = items < kJoinBlocks ? items : kJoinBlocks;

@@ -170,7 +170,6 @@ constexpr int kWavesPerCu = 64;
 constexpr int kSingleVectors = 384;
 
 // The largest block, and the rows it has at a time.
-
 template <int LANES> constexpr int row_block() { return LANES <= kWaveSize ? kBlock : LANES; }
 template <int LANES> constexpr int block_rows() { return LANES <= kWaveSize ? kBlock / LANES : 1; }
 constexpr int kMostWaves = kWholeBlock / kWaveSize;

@@ -228,6 +228,18 @@ def test_embedding_gradient_of_skewed_tokens(n, distribution):
 
 @pytest.mark.parametrize("table_type", TYPES)
 @pytest.mark.parametrize("n", [40, 3000])
+@pytest.mark.parametrize("dimension", [3, 64, 65, 257])
+def test_embedding_gradient_gives_zeros_one_sign(dimension, n, table_type):
+    # 0 * -1 is -0 in every column, the last ones of a row that is no whole number of vectors too
+    import torch
+    tokens = torch.zeros(n, dtype=torch.int32, device="cuda")
+    out = _embedding_gradient(torch.zeros(n, dimension, device="cuda"), tokens, 2, _t(table_type), -1.0)
+    assert bool((out == 0).all())
+    assert bool(torch.signbit(out[0]).all()) and not bool(torch.signbit(out[1]).any())
+
+
+@pytest.mark.parametrize("table_type", TYPES)
+@pytest.mark.parametrize("n", [40, 3000])
 def test_embedding_gradient_accumulates_and_skips_padding(n, table_type):
     import torch
     vocabulary = 700

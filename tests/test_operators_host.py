@@ -84,6 +84,15 @@ def test_embedding_gradient_is_refused_where_sorts_are():
         capi.sort_set_parameter(capi.SORT_PARAM_ASSUME_LDS_ATOMIC_ORDER, -1)
 
 
+def test_embedding_gradient_of_more_sums_than_a_grid_holds():
+    # Broadcast rows take no memory, but 2^31 - 1 positions of 512 columns want 2^25 blocks of 256.
+    L, n = capi.lib(), (1 << 31) - 1
+    assert capi.embedding_gradient_temp_bytes(n, 10, 512) < BIG
+    assert L.ilgpu_hip_embedding_gradient(
+        None, FAKE, 0, capi.F32, FAKE, n, capi.I32, ONE, -1, 0, FAKE, 10, 512, 512, capi.F32,
+        FAKE, BIG) == capi.ERROR_NOT_SUPPORTED
+
+
 def test_layer_norm_argument_validation():
     def call(x=FAKE, r=4, c=8, xs=8, t=capi.F16, w=FAKE, b=FAKE, wt=capi.F32, eps=number(1e-5),
              out=FAKE, os_=8, mean=FAKE, rstd=FAKE):
