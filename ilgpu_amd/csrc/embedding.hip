@@ -340,6 +340,7 @@ struct Sums {
   int32_t clear_rows;    // rows a block clears, lanes that share one
   int32_t clear_lanes_log2;
   int lanes_log2;        // lanes that share a row
+  int join_lanes_log2;
 };
 
 // A thread's columns of a row, which begin at its `own`-th of W sums (0, or what the last
@@ -636,8 +637,10 @@ __global__ __launch_bounds__(kBlock) void embedding_gradient_of_few_kernel(
   }
 }
 
-// Joins the parts of the long runs: the waves of a block take every fourth part, and
-// their sums are added in the order of the waves.  The blocks behind clear rows.
+// Joins the parts of the long runs: the waves of a block take the parts in turn, of narrow rows
+// several at a time, and their sums are added in the order of the waves.  The blocks behind clear
+// rows.  (10^6 tokens into 1000 x 32 float, where one token has 3000 parts: 14 us; 29 with
+// the run's end looked for 64 chunks at a time, 60 with one part a wave at a time too.)
 constexpr int kJoinBlock = kBlock;
 constexpr int kJoinBlocks = 2048;
 constexpr int kJoinWaves = kJoinBlock / kWaveSize;
@@ -654,42 +657,53 @@ __global__ __launch_bounds__(kJoinBlock) void join_runs_kernel(
   __shared__ float lds[kJoinWaves][kWaveSize * W];
   const uint32_t slices = s.join_slices;
   const int wave = threadIdx.x / kWaveSize, lane = threadIdx.x & (kWaveSize - 1);
+  const int log2 = s.join_lanes_log2, at_once = kJoinBlock >> log2;  // parts
+  const int part = threadIdx.x >> log2, column = lane & ((1 << log2) - 1);
   const uint32_t items = s.crossings[0] * slices;
   for (uint32_t item = blockIdx.x; item < items; item += s.join_blocks) {
     const int64_t chunk = s.crossings[1 + item / slices];
-    const int64_t c = ((int64_t)(item % slices) * kWaveSize + lane) * W;
+    const int64_t c = (((int64_t)(item % slices) << log2) + column) * W;
     const int64_t columns = s.dimension - c;  // a part's row is padded to whole loads
     const uint32_t run = keys[chunk * s.chunk + s.chunk - 1];
-    // Chunks behind it that begin inside the run.
-    int64_t more = 0;
-    for (;;) {
-      const int64_t p = (chunk + 1 + more + lane) * s.chunk;
-      const uint64_t inside = __ballot(p < s.count && keys[p < s.count ? p : 0] == run);
-      if (inside == ~0ull) {
-        more += kWaveSize;
-        continue;
-      }
-      more += __builtin_ctzll(~inside);
-      break;
+    // Chunks behind it that begin inside the run, as all do up to its end: 64 at a time, of long
+    // runs then by 64 places among those that are left, 64 in the stretch between two of them...
+    int64_t more = 0, left = s.chunks - chunk - 1, stretch = 1;
+    while (left > 0) {
+      const int64_t at = (lane + 1) * stretch - 1;
+      const uint64_t inside = __ballot(at < left && keys[(chunk + 1 + more + (at < left ? at : 0)) * s.chunk] == run);
+      const int found = inside == ~0ull ? kWaveSize : __builtin_ctzll(~inside);
+      more += found * stretch;
+      left -= found * stretch;
+      if (found < kWaveSize && left > stretch - 1) left = stretch - 1;
+      stretch = more < 4 * kWaveSize ? 1 : (left + kWaveSize - 1) / kWaveSize;
     }
     float sum[W];
 #pragma unroll
     for (int k = 0; k < W; ++k) sum[k] = 0.0f;
     if (columns > 0) {
       const float* from = s.parts + (chunk + 1) * s.part_stride + c;
-      if (wave == 0) load_floats<float, W>(sum, s.parts + (s.chunks + chunk) * s.part_stride + c, W);
-#pragma unroll 8
-      for (int64_t j = wave; j < more; j += kJoinWaves) {
-        float v[W];
-        load_floats<float, W>(v, from + j * s.part_stride, W);
+      if (part == 0) load_floats<float, W>(sum, s.parts + (s.chunks + chunk) * s.part_stride + c, W);
+      constexpr int U = 8;  // in flight
+      for (int64_t first = part; first < more; first += (int64_t)U * at_once) {
+        float v[U][W];
 #pragma unroll
-        for (int k = 0; k < W; ++k) sum[k] += v[k];
+        for (int u = 0; u < U; ++u) {
+          const int64_t j = first + u * at_once;
+          load_floats<float, W>(v[u], from + (j < more ? j : first) * s.part_stride, W);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int k = 0; k < W; ++k) sum[k] += first + u * at_once < more ? v[u][k] : 0.0f;
       }
     }
+    for (int off = 1 << log2; off < kWaveSize; off <<= 1)
+#pragma unroll
+      for (int k = 0; k < W; ++k) sum[k] += __shfl_xor(sum[k], off, kWaveSize);
 #pragma unroll
     for (int k = 0; k < W; ++k) lds[wave][lane * W + k] = sum[k];
     __syncthreads();
-    if (wave == 0) {
+    if (part == 0) {
       for (int w = 1; w < kJoinWaves; ++w)
 #pragma unroll
         for (int k = 0; k < W; ++k) sum[k] += lds[w][lane * W + k];
@@ -912,6 +926,7 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
       const int all_log2 = lanes_log2(a.dimension, W);
       const int log2 = all_log2 < 6 ? all_log2 : 6;
       const int64_t slices = div_up(a.dimension, (int64_t)W << log2);
+      const int join_log2 = lanes_log2(a.dimension, 4) < 6 ? lanes_log2(a.dimension, 4) : 6;
       const int64_t join_slices = div_up(a.dimension, kWaveSize * 4);
       const int64_t sum_blocks = div_up(t.chunks * slices, kBlock >> log2);
       const int64_t items = t.chunks > 2 ? (t.chunks - 2) * join_slices : 0;
@@ -929,6 +944,7 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
       s.sum_blocks = (uint32_t)sum_blocks;
       s.join_blocks = (uint32_t)join_blocks;
       s.lanes_log2 = log2;
+      s.join_lanes_log2 = join_log2;
       set_clear_shape<TW>(s, 16 / sizeof(TW));
       // Rows cleared beside the join are as many as it has time for while it waits for its
       // own reads; those before them keep the memory busy while the sums wait for theirs

@@ -226,6 +226,22 @@ def test_embedding_gradient_of_skewed_tokens(n, distribution):
     assert torch.equal(out, _embedding_gradient(grad, tokens, vocabulary, torch.float32, 2.0))
 
 
+@pytest.mark.parametrize("dimension", [1, 5, 36, 64, 130, 300])
+@pytest.mark.parametrize("unit", [8, 32])
+def test_embedding_gradient_of_runs_of_many_lengths(unit, dimension):
+    # whole numbers, whose sums are exact in float32 in any order, in runs of up to 5000 chunks
+    import torch
+    lengths = [unit * c + more for c in (1, 2, 63, 64, 65, 128, 255, 256, 257, 320, 321, 700, 5000)
+               for more in (-1, 0, 1)]
+    tokens = torch.repeat_interleave(torch.arange(len(lengths)), torch.tensor(lengths)).cuda()
+    g = _rng(unit, dimension)
+    grad = torch.randint(-3, 4, (len(tokens), dimension), generator=g, device="cuda").float()
+    out = _embedding_gradient(grad, tokens, len(lengths), torch.float32)
+    exact = torch.zeros(len(lengths), dimension, dtype=torch.float64, device="cuda")
+    exact.index_add_(0, tokens, grad.double())
+    assert torch.equal(out.double(), exact)
+
+
 @pytest.mark.parametrize("table_type", TYPES)
 @pytest.mark.parametrize("n", [40, 3000])
 @pytest.mark.parametrize("dimension", [3, 64, 65, 257])
