@@ -313,12 +313,15 @@ template <typename F> int32_t with_norm_types(int32_t type, int32_t weight_type,
 // order of the blocks. A single block writes the results itself.
 //
 // Fewer waves leave fewer partials, and with the next row on its way they keep the memory
-// as busy (32768 x 4096 bfloat16, us: 12 waves a compute unit 141, 16 151, 32 163; 8192 x
-// 1024 15.7, 20.0, 30.8; odd lengths want 12 rather than 8: 3000 columns 83, 95). 32768 x
-// 4096 is 805 MB in 141 us, 5.7 TB/s.
+// as busy (waves wanted a compute unit, 32768 x 4096 bfloat16, us: 12 141, 16 151, 32 163; 8192 x
+// 1024 15.7, 20.0, 30.8; odd lengths want 12 rather than 8: 3000 columns 83, 95; 16384 x
+// 3500 with 14 rather than 7: 74, 105). 32768 x 4096 is 805 MB in 141 us, 5.7 TB/s.
 constexpr int kGradientBlock = 512;       // of rows that a wave or a part of one holds
 constexpr int kGradientWavesPerCu = 12;
 constexpr int kMaxSplitsPerCu = 4;
+// Rows a block at least before a compute unit has two (bfloat16, us, 4 / 1: 1000 rows of 1500 12.0
+// / 19.5, 600 of 2880 12.9 / 16.4, 1000 of 3500 15.9 / 20.3; with 8, 4000 of 2432 25.1 instead of 21.6).
+constexpr int kRowsPerSplit = 4;
 template <int LANES> constexpr int gradient_block() {
   return LANES <= kWaveSize ? kGradientBlock : LANES;
 }
@@ -599,7 +602,10 @@ int32_t launch_layer_norm_gradient(hipStream_t stream, const LayerNormGradientAr
           const int threads = kLanes == kWholeBlock ? row_threads : kGradientBlock;
           const int64_t blocks =
               div_up(a.rows, kLanes == kWholeBlock ? 1 : kGradientBlock / kLanes);
-          int64_t per_cu = kGradientWavesPerCu * kWaveSize / threads;
+          // The blocks that come nearest to the waves wanted, of two numbers the smaller.
+          int64_t per_cu = (kGradientWavesPerCu * kWaveSize + threads / 2 - 1) / threads;
+          // (A block's sums are worth writing after a few rows only.)
+          while (per_cu > 1 && a.rows < device_cu_count() * per_cu * kRowsPerSplit) --per_cu;
           per_cu = per_cu < 1 ? 1 : per_cu < kMaxSplitsPerCu ? per_cu : kMaxSplitsPerCu;
           const int64_t most = device_cu_count() * per_cu;
           // (Four turns of one block take less than the fold's launch.)
