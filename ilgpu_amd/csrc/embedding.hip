@@ -173,6 +173,14 @@ __device__ __forceinline__ void clear_all(const Clearing& t, uint32_t block, uin
   }
 }
 
+// What a wave's lanes have written to LDS, its other lanes read from here on.  (The hardware
+// runs a wave's LDS instructions in order; this keeps the compiler to it.)
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <typename TT>
 __global__ __launch_bounds__(kGroupBlock, 8) void group_tokens_kernel(
     const TT* __restrict__ tokens, int64_t count, int64_t padded, int64_t vocabulary,
@@ -258,6 +266,7 @@ __global__ __launch_bounds__(kGroupBlock, 8) void group_tokens_kernel(
       listed += __popcll(owns);
     }
   });
+  wave_lds_fence();  // the list's entries go to other lanes
   if (listed <= list_length) {
     for (uint32_t j = lane; j < listed; j += kWaveSize) count_row(list[j] >> kGroupCountLog2);
   } else {

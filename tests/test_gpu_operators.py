@@ -369,6 +369,41 @@ def test_embedding_gradient_keeps_bad_rows_to_their_tokens(n):
         assert torch.equal(out[bad[1], others], good[bad[1], others])
 
 
+def _whole_numbers(g, *shape, dtype=None):
+    """Small whole numbers: sums of up to 2^22 of them are exact in float32 in any order."""
+    import torch
+    return torch.randint(-3, 4, shape, generator=g, device="cuda").to(dtype or torch.float32)
+
+
+def _equal_sums(out, grad, tokens, vocabulary):
+    """out is the sum of each token's rows, to the bit."""
+    import torch
+    wide = tokens.long()
+    there = (wide >= 0) & (wide < vocabulary)
+    exact = torch.zeros(vocabulary, grad.shape[1], dtype=torch.float64, device="cuda")
+    exact.index_add_(0, wide[there], grad.double()[there])
+    assert torch.equal(out.double(), exact)
+
+
+@pytest.mark.parametrize("token_type", ["int32", "int64"])
+@pytest.mark.parametrize("n,places", [(65_536, 512), (131_072, 1024)])
+@pytest.mark.parametrize("more", [-1, 0, 1, 64, None])
+def test_embedding_gradient_of_position_lists_about_full(more, n, places, token_type):
+    # Sixteen waves of a block list the positions of its tokens in a sixteenth of the input each;
+    # a list has `places` of them. Tokens 7, 263 and 519 belong to the same block.
+    import torch
+    vocabulary, stretch = 600, n // 16
+    g = _rng(n, places, 0 if more is None else more + 2)
+    listed = stretch if more is None else places + more
+    tokens = torch.randint(0, 7, (16, stretch), generator=g, device="cuda")
+    tokens[:, :listed] = 7 + 256 * torch.randint(0, 3, (16, listed), generator=g, device="cuda")
+    order = torch.rand(16, stretch, generator=g, device="cuda").argsort(1)
+    tokens = tokens.gather(1, order).reshape(-1).to(_t(token_type))
+    grad = _whole_numbers(g, n, 24)
+    out = _embedding_gradient(grad, tokens, vocabulary, torch.float32)
+    _equal_sums(out, grad, tokens, vocabulary)
+
+
 # ---- layer norm -------------------------------------------------------------------
 def _layer_norm(x, weight, bias, epsilon=1e-5, out=None):
     import torch
