@@ -574,7 +574,8 @@ __global__ __launch_bounds__(kBlock) void embedding_gradient_kernel(
   sum_chunk<TG, TW, W, CHUNK, WHOLE_WAVE>(s, keys, order, group, grad_out, table);
 }
 
-// The lanes of `inside` whose key is `row`, which differs between the groups of a wave.
+// The lanes of `inside` whose key is `row`, which differs between the groups of a wave. Any lane's
+// key is read, so all lanes of the wave take part, also those whose row lies beyond the table.
 __device__ __forceinline__ uint64_t positions_of(uint64_t inside, uint32_t key, uint32_t row) {
   uint64_t mine = 0;
   for (; inside != 0; inside &= inside - 1) {
@@ -605,9 +606,10 @@ __global__ __launch_bounds__(kBlock) void embedding_gradient_of_few_kernel(
     // The positions whose rows are among the block's.
     const uint64_t inside = __ballot(counts && key - (uint32_t)first < (uint32_t)s.clear_rows);
     if (inside == 0 && s.accumulate) continue;
-    for (int64_t r = first + (threadIdx.x >> log2); r < first + s.clear_rows && r < s.vocabulary;
-         r += kBlock >> log2) {
+    for (int64_t r0 = first; r0 < first + s.clear_rows && r0 < s.vocabulary; r0 += kBlock >> log2) {
+      const int64_t r = r0 + (threadIdx.x >> log2);
       const uint64_t mine = inside == 0 ? 0 : positions_of(inside, key, (uint32_t)r);
+      if (r >= s.vocabulary) continue;
       TW* const row = table + r * s.table_stride;
       for (int64_t c = (int64_t)(threadIdx.x & ((1u << log2) - 1)) * W; c < s.dimension;
            c += (int64_t)W << log2) {

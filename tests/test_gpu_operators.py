@@ -404,6 +404,22 @@ def test_embedding_gradient_of_position_lists_about_full(more, n, places, token_
     _equal_sums(out, grad, tokens, vocabulary)
 
 
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("dimension", [1, 3, 4, 20, 64, 130, 1030])
+@pytest.mark.parametrize("vocabulary", [1, 2, 17, 63, 65, 257, 1021])
+def test_embedding_gradient_of_few_tokens_and_rows_that_end_inside_a_wave(vocabulary, dimension,
+                                                                         accumulate):
+    # Rows of the table share waves and the table ends inside one; tokens lie in all 64 lanes.
+    import torch
+    g = _rng(vocabulary, dimension, 61)
+    for n in (33, 64):
+        tokens = torch.randint(max(0, vocabulary - 9), vocabulary, (n,), generator=g, device="cuda")
+        grad = _whole_numbers(g, n, dimension)
+        old = _whole_numbers(g, vocabulary, dimension) if accumulate else None
+        out = _embedding_gradient(grad, tokens, vocabulary, torch.float32, into=old)
+        _equal_sums(out if old is None else out - old, grad, tokens, vocabulary)
+
+
 # ---- layer norm -------------------------------------------------------------------
 def _layer_norm(x, weight, bias, epsilon=1e-5, out=None):
     import torch
