@@ -88,9 +88,14 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(
 // by a second kernel.  Rows of no token are cleared by further blocks of both and of the
 // grouping.
 constexpr int kChunk = 32, kShortChunk = 8;
-// Few and narrow rows fill the chip only in short chunks.
+// Few and narrow rows fill the chip only in short chunks: where long ones of 256 columns are
+// fewer than this.
+constexpr int64_t kFewChunks = 1024;
+inline int64_t most_in_short_chunks(int64_t dimension) {
+  return (kFewChunks - 1) / div_up(dimension, 256) * kChunk;
+}
 inline int chunk_length(int64_t count, int64_t dimension) {
-  return div_up(count, kChunk) * div_up(dimension, 256) < 1024 ? kShortChunk : kChunk;
+  return count <= most_in_short_chunks(dimension) ? kShortChunk : kChunk;
 }
 
 // Sort keys of the positions: their tokens, `vocabulary` for those that count nowhere.
@@ -137,10 +142,13 @@ inline int group_log2(int64_t vocabulary) {
 // to 2^17 tokens, with more blocks up to as much fewer.  (Whole gradient into 131072 x 64, us,
 // groups / sort: 8192 tokens 23 / 53, 32768 39 / 88, 131072 65 / 102, of 1000 rows 67 / 70; 2^18
 // tokens, which overflow the waves' lists, 162 / 116.)
-inline bool takes_groups(int64_t count, int64_t vocabulary) {
+inline int64_t most_in_groups(int64_t vocabulary) {  // -1: not even none
   const int log2 = group_log2(vocabulary);
-  return vocabulary <= ((int64_t)kGroupRows << log2) &&
-         count <= ((int64_t)1 << (kGroupCountLog2 + kGroupMinLog2 - log2));
+  if (vocabulary > ((int64_t)kGroupRows << log2)) return -1;
+  return (int64_t)1 << (kGroupCountLog2 + kGroupMinLog2 - log2);
+}
+inline bool takes_groups(int64_t count, int64_t vocabulary) {
+  return count <= most_in_groups(vocabulary);
 }
 
 // The table's last rows from `first` on, which further blocks of the grouping clear, met or
@@ -856,8 +864,17 @@ static bool grid_holds(const GradientTemp& t, const EmbeddingGradientArgs& a) {
          t.chunks * div_up(a.dimension, kWaveSize * 4) <= INT32_MAX;
 }
 
+// What `count` tokens need, or fewer: a program keeps one temp for batches of any length up to a
+// largest.  The layout grows with the tokens but for two steps back: long chunks leave a quarter
+// of the parts, and sorted tokens no bits of met rows.
 int64_t embedding_gradient_temp_bytes(int64_t count, int64_t vocabulary, int64_t dimension) {
-  return gradient_temp(count, vocabulary, dimension).bytes;
+  int64_t bytes = gradient_temp(count, vocabulary, dimension).bytes;
+  for (const int64_t last : {most_in_short_chunks(dimension), most_in_groups(vocabulary)}) {
+    if (last < 0 || last >= count) continue;
+    const int64_t there = gradient_temp(last, vocabulary, dimension).bytes;
+    if (there > bytes) bytes = there;
+  }
+  return bytes;
 }
 
 int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArgs& a) {

@@ -470,7 +470,8 @@ int32_t ilgpu_hip_embedding(ilgpu_hip_stream_t stream, const void *table,
  * are left alone.  Tokens outside [0, vocabulary) and padding_token (pass -1
  * for none) contribute nothing.  grad_table must not overlap grad_out or
  * tokens.  On a device whose LDS fails ilgpu_hip_sort_check_device:
- * ILGPU_HIP_ERROR_NOT_SUPPORTED, like a sort. */
+ * ILGPU_HIP_ERROR_NOT_SUPPORTED, like a sort.  A temp for `count` tokens serves
+ * any smaller number of them (same vocabulary and dimension). */
 int32_t ilgpu_hip_embedding_gradient_temp_bytes(int64_t count,
                                                 int64_t vocabulary,
                                                 int64_t dimension,

@@ -420,6 +420,23 @@ def test_embedding_gradient_of_few_tokens_and_rows_that_end_inside_a_wave(vocabu
         _equal_sums(out if old is None else out - old, grad, tokens, vocabulary)
 
 
+@pytest.mark.parametrize("most,vocabulary,dimension", [(4096, 900, 2048), (40_000, 3000, 256),
+                                                       (131_073, 1000, 64), (140_000, 300_000, 24)])
+def test_embedding_gradient_of_fewer_tokens_in_the_same_temp(most, vocabulary, dimension):
+    import torch
+    from ilgpu_amd import capi
+    g = _rng(most, vocabulary, 71)
+    temp = capi.temp_buffer(capi.embedding_gradient_temp_bytes(most, vocabulary, dimension))
+    for n in (most, most - 1, most - 32, most // 2, most // 5, 100, 3):
+        tokens = _tokens(g, n, vocabulary, torch.int64)
+        grad = _whole_numbers(g, n, dimension)
+        out = torch.full((vocabulary, dimension), float("nan"), device="cuda")
+        capi.embedding_gradient(capi.DeviceMatrix.from_tensor(grad),
+                                capi.DeviceArray.from_tensor(tokens),
+                                capi.DeviceMatrix.from_tensor(out), temp)
+        _equal_sums(out, grad, tokens, vocabulary)
+
+
 # ---- layer norm -------------------------------------------------------------------
 def _layer_norm(x, weight, bias, epsilon=1e-5, out=None):
     import torch

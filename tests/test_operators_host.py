@@ -72,6 +72,19 @@ def test_embedding_gradient_argument_validation():
         capi.embedding_gradient_temp_bytes(1, 1 << 31, 1)
 
 
+@pytest.mark.parametrize("vocabulary", [1, 1000, 50_000, 1 << 18, (1 << 18) + 1, 1 << 19, 1 << 20,
+                                        (1 << 20) + 1, (1 << 31) - 1])
+@pytest.mark.parametrize("dimension", [1, 64, 256, 257, 512, 769, 1024, 2048, 4096, 8192, 300_000])
+def test_a_temp_of_the_embedding_gradient_serves_fewer_tokens(dimension, vocabulary):
+    most = 0
+    steps = [(1 << k) + more for k in range(18, 31) for more in (-1, 0, 1)]
+    near = [(1 << k) + more for k in range(11, 18) for more in (-33, -32, -31, -1, 0, 1, 31, 32)]
+    for n in sorted([*range(2100), *range(2100, 140_000, 31), *near, *steps]):
+        need = capi.embedding_gradient_temp_bytes(n, vocabulary, dimension)
+        assert need >= most, n
+        most = need
+
+
 def test_embedding_gradient_is_refused_where_sorts_are():
     L = capi.lib()
     capi.sort_set_parameter(capi.SORT_PARAM_ASSUME_LDS_ATOMIC_ORDER, 0)
