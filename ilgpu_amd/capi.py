@@ -313,7 +313,7 @@ class DeviceMatrix:
 
     def __init__(self, base: DeviceArray, rows: int, columns: int,
                  row_stride: Optional[int] = None):
-        self.base = base
+        self.base = _dense(base)
         self.rows, self.columns = int(rows), int(columns)
         self.row_stride = self.columns if row_stride is None else int(row_stride)
         self.dtype, self.type_code = base.dtype, base.type_code

@@ -232,6 +232,15 @@ def test_the_bindings_checks_of_views():
         capi.clip_gradients([A(4, f32)], A(1, f32), 1.0, [], stream=0)
 
 
+def test_a_matrix_is_made_of_a_dense_array():
+    # the elements of a strided view do not lie side by side, as those of a row do
+    M, A = capi.DeviceMatrix, host_array
+    for rows, columns, stride in ((2, 4, 4), (1, 8, None), (8, 1, 1), (5, 8, 0)):
+        with pytest.raises(capi.NotSupportedError):
+            M(A(32, np.float32).strided(2), rows, columns, stride)
+    assert M(A(32, np.float32).strided(1), 8, 4).rows == 8
+
+
 def run(*args):
     assert os.path.exists(BINARY), "build it with `python -m ilgpu_amd.build`"
     proc = subprocess.run([BINARY, *args], capture_output=True, text=True, timeout=300)
