@@ -715,6 +715,21 @@ def test_layer_norm_gradient_against_differences():
             assert abs(slope - float(got.view(-1)[i])) <= tolerance * 10, (k, i)
 
 
+def test_layer_norm_gradient_of_rows_longer_than_a_grid_of_threads():
+    # 2^28 columns at 16 threads each are 2^32. With a mean of 0 and a deviation of 1, whole numbers
+    # stay whole.
+    import torch
+    rows, columns = 2, (1 << 28) + 70
+    g = _rng(28, 81)
+    x = _whole_numbers(g, rows, columns, dtype=torch.float16)
+    grad = _whole_numbers(g, rows, columns, dtype=torch.float16)
+    mean, rstd = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+    _, grad_w, grad_b = _layer_norm_gradient(grad, x, None, mean, rstd, torch.float16, want="wb",
+                                             grad_x=x)
+    assert torch.equal(grad_b, grad[0] + grad[1])
+    assert torch.equal(grad_w, grad[0] * x[0] + grad[1] * x[1])
+
+
 # ---- gradient norm and clipping --------------------------------------------------------
 def _lists(g, sizes, spread=1.0):
     import torch
