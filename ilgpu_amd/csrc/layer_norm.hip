@@ -502,37 +502,32 @@ __global__ __launch_bounds__(kBlock) void layer_norm_column_sums_kernel(
   partials[((int64_t)gridDim.y + blockIdx.y) * columns + c] = sum_b;
 }
 
-// Adds up `splits` rows of partials: 64 columns a block at a time, whose waves take every 16th
-// row; blockIdx.y: the weight's, the bias's.  (A grid holds less than 2^32 threads, which 64 columns
-// a block would be at 2^28 columns.)
+// Adds up `splits` rows of partials: 64 columns a block, whose waves take every 16th row;
+// blockIdx.y: the weight's, the bias's.  A launch begins at block `first_block`: a grid holds less
+// than 2^32 threads, which 2^28 columns would be.
 constexpr int kFoldBlock = 1024;
 constexpr int64_t kMaxFoldBlocks = 1 << 20;
 template <typename TW>
 __global__ __launch_bounds__(kFoldBlock) void layer_norm_fold_kernel(
     const float* __restrict__ partials, int64_t splits, int64_t columns, int32_t accumulate,
-    TW* __restrict__ grad_weight, TW* __restrict__ grad_bias) {
+    TW* __restrict__ grad_weight, TW* __restrict__ grad_bias, uint32_t first_block) {
   constexpr int kWaves = kFoldBlock / kWaveSize;
   __shared__ float lds[kWaves][kWaveSize];
   TW* to = blockIdx.y == 0 ? grad_weight : grad_bias;
   if (to == nullptr) return;
   const int wave = threadIdx.x / kWaveSize, lane = threadIdx.x & (kWaveSize - 1);
-  for (int64_t first = (int64_t)blockIdx.x * kWaveSize; first < columns;
-       first += (int64_t)gridDim.x * kWaveSize) {
-    const int64_t c = first + lane;
-    const float* from = partials + blockIdx.y * splits * columns + c;
-    float sum = 0.0f;
-    if (c < columns) {
+  const int64_t c = (int64_t)(first_block + blockIdx.x) * kWaveSize + lane;
+  const float* from = partials + blockIdx.y * splits * columns + c;
+  float sum = 0.0f;
+  if (c < columns) {
 #pragma unroll 8
-      for (int64_t s = wave; s < splits; s += kWaves) sum += from[s * columns];
-    }
-    lds[wave][lane] = sum;
-    __syncthreads();
-    if (wave == 0 && c < columns) {
-      for (int i = 1; i < kWaves; ++i) sum += lds[i][lane];
-      to[c] = (TW)(accumulate ? (float)to[c] + sum : sum);
-    }
-    __syncthreads();
+    for (int64_t s = wave; s < splits; s += kWaves) sum += from[s * columns];
   }
+  lds[wave][lane] = sum;
+  __syncthreads();
+  if (wave != 0 || c >= columns) return;
+  for (int i = 1; i < kWaves; ++i) sum += lds[i][lane];
+  to[c] = (TW)(accumulate ? (float)to[c] + sum : sum);
 }
 
 // Rows of partials at most: one for each block of a launch.
@@ -592,14 +587,17 @@ int32_t launch_layer_norm_gradient(hipStream_t stream, const LayerNormGradientAr
     const auto fold = [&](int64_t splits) -> int32_t {
       if (!sums) return ILGPU_HIP_SUCCESS;
       const int64_t blocks = div_up(a.columns, kWaveSize);
-      {
-        ProfileScope scope(stream, "layer_norm_fold");
-        hipLaunchKernelGGL((layer_norm_fold_kernel<TW>),
-                           dim3((unsigned)(blocks < kMaxFoldBlocks ? blocks : kMaxFoldBlocks), 2),
-                           dim3(kFoldBlock), 0, stream, partials, splits, a.columns, a.accumulate,
-                           static_cast<TW*>(a.grad_weight), static_cast<TW*>(a.grad_bias));
+      for (int64_t first = 0; first < blocks; first += kMaxFoldBlocks) {
+        const int64_t some = blocks - first < kMaxFoldBlocks ? blocks - first : kMaxFoldBlocks;
+        {
+          ProfileScope scope(stream, "layer_norm_fold");
+          hipLaunchKernelGGL((layer_norm_fold_kernel<TW>), dim3((unsigned)some, 2),
+                             dim3(kFoldBlock), 0, stream, partials, splits, a.columns,
+                             a.accumulate, static_cast<TW*>(a.grad_weight),
+                             static_cast<TW*>(a.grad_bias), (uint32_t)first);
+        }
+        ILGPU_HIP_CHECK(hipGetLastError());
       }
-      ILGPU_HIP_CHECK(hipGetLastError());
       return ILGPU_HIP_SUCCESS;
     };
     if (a.rows == 0) return fold(0);
