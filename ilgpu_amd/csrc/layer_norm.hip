@@ -2,7 +2,9 @@
 //
 // Sums are in float32, of a thread's own elements first and then over the lanes and
 // waves in a fixed order; the variance is the mean of the squared deviations from the
-// mean already known, which loses nothing where the mean is large against them.
+// mean already known.  That mean is off by some roundings of the row's size: of a row far from
+// zero (far_from_zero) the deviations themselves, which are small, are added up too, and
+// mean, deviations and variance are put right by their mean.
 //
 // Bound by the memory: a row is read once, stays in the registers of the wave or block
 // that normalises it, and is written once.  Waves and blocks go from row to row and hold
@@ -82,6 +84,17 @@ template <int LANES> __device__ __forceinline__ float row_sum(float v, float* sl
     __syncthreads();
     return sum_waves(slot);
   }
+}
+
+// Whether a row's mean is more than two deviations from zero. Below that its roundings are as
+// small as those of the deviations' own sums; beyond it a third sum finds the `rest` of the mean.  (Added
+// up in every row, us: 8192 x 2000 bfloat16 15.2, 13.6 without, 4099 x 1537 9.5, 8.9.)
+template <int LANES> __device__ __forceinline__ bool far_from_zero(float mean, float variance) {
+  const int far = mean * mean > 4.0f * variance;
+  return __builtin_expect(LANES >= kWaveSize ? __builtin_amdgcn_readfirstlane(far) : far, 0);
+}
+__device__ __forceinline__ float less_rest(float variance, float rest) {
+  return fmaxf(variance - rest * rest, 0.0f);
 }
 
 // The columns of a thread: V times W side by side, W times the row's lanes apart.  Where a row ends
@@ -180,7 +193,7 @@ __global__ __launch_bounds__(row_block<LANES>()) void layer_norm_kernel(
     const TW* __restrict__ bias, float epsilon, T* out, int64_t out_stride,
     float* __restrict__ mean, float* __restrict__ rstd) {
   constexpr int kRows = block_rows<LANES>();
-  __shared__ float lds[2][kMostWaves];
+  __shared__ float lds[3][kMostWaves];
   const Columns<W, LANES, V> own(columns);
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + row_of_block<LANES>();
@@ -197,13 +210,23 @@ __global__ __launch_bounds__(row_block<LANES>()) void layer_norm_kernel(
 #pragma unroll
       for (int k = 0; k < W; ++k) x[v][k] = (float)next[v][k];
     if (row + step < rows) own.load(next, in + (row + step) * in_stride);
-    const float m = row_sum<LANES>(own.sum([&](int v, int k) { return x[v][k]; }), lds[0]) / (float)columns;
+    float m = row_sum<LANES>(own.sum([&](int v, int k) { return x[v][k]; }), lds[0]) / (float)columns;
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
       for (int k = 0; k < W; ++k) x[v][k] -= m;
-    const float variance =
+    float variance =
         row_sum<LANES>(own.sum([&](int v, int k) { return x[v][k] * x[v][k]; }), lds[1]) / (float)columns;
+    if (far_from_zero<LANES>(m, variance)) {  // the same in all threads of a row
+      const float rest =
+          row_sum<LANES>(own.sum([&](int v, int k) { return x[v][k]; }), lds[2]) / (float)columns;
+      m += rest;
+      variance = less_rest(variance, rest);
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int k = 0; k < W; ++k) x[v][k] -= rest;
+    }
     const float r = 1.0f / sqrtf(variance + epsilon);
 #pragma unroll
     for (int v = 0; v < V; ++v)
@@ -218,7 +241,8 @@ __global__ __launch_bounds__(row_block<LANES>()) void layer_norm_kernel(
 }
 
 // Rows too long for the registers: a block reads each of them three times, the second and
-// third time from the caches.
+// third time from the caches.  The rest of the mean is added up beside the squares (64 x 40000
+// bfloat16 11.4 us, 11.2 without; 12.0 by a fourth reading of rows that ask for it).
 constexpr int kLongBlock = kWholeBlock;
 template <typename T, typename TW>
 __global__ __launch_bounds__(kLongBlock) void layer_norm_long_kernel(
@@ -226,7 +250,7 @@ __global__ __launch_bounds__(kLongBlock) void layer_norm_long_kernel(
     const TW* __restrict__ bias, float epsilon, T* out, int64_t out_stride,
     float* __restrict__ mean, float* __restrict__ rstd) {
   constexpr int W = 16 / sizeof(T);
-  __shared__ float lds[2][kLongBlock / kWaveSize];
+  __shared__ float lds[3][kLongBlock / kWaveSize];
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T* x = in + row * in_stride;
     T* y = out + row * out_stride;
@@ -239,15 +263,28 @@ __global__ __launch_bounds__(kLongBlock) void layer_norm_long_kernel(
       sum += part;
     }
     const float m = row_sum<kLongBlock>(sum, lds[0]) / (float)columns;
+    float squares = 0.0f;
     sum = 0.0f;
     for (int64_t c = (int64_t)threadIdx.x * W; c < columns; c += kLongBlock * W) {
-      float v[W], part = 0.0f;
+      float v[W], part = 0.0f, part_squares = 0.0f;
       load_floats<T, W>(v, x + c, columns - c);
 #pragma unroll
-      for (int k = 0; k < W; ++k) part += c + k < columns ? (v[k] - m) * (v[k] - m) : 0.0f;
+      for (int k = 0; k < W; ++k) {
+        const float away = c + k < columns ? v[k] - m : 0.0f;
+        part += away;
+        part_squares += away * away;
+      }
       sum += part;
+      squares += part_squares;
     }
-    const float r = 1.0f / sqrtf(row_sum<kLongBlock>(sum, lds[1]) / (float)columns + epsilon);
+    put_wave(lanes_sum<kWaveSize>(sum), lds[1]);
+    put_wave(lanes_sum<kWaveSize>(squares), lds[2]);
+    __syncthreads();
+    float rest = sum_waves(lds[1]) / (float)columns;
+    float variance = sum_waves(lds[2]) / (float)columns;
+    if (far_from_zero<kLongBlock>(m, variance)) variance = less_rest(variance, rest);
+    else rest = 0.0f;
+    const float r = 1.0f / sqrtf(variance + epsilon), shift = -rest * r;
     for (int64_t c = (int64_t)threadIdx.x * W; c < columns; c += kLongBlock * W) {
       float v[W], w[W], b[W];
       load_floats<T, W>(v, x + c, columns - c);
@@ -255,13 +292,13 @@ __global__ __launch_bounds__(kLongBlock) void layer_norm_long_kernel(
       if (bias != nullptr) load_floats<TW, W>(b, bias + c, columns - c);
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        v[k] = (v[k] - m) * r * (weight != nullptr ? w[k] : 1.0f);
+        v[k] = fmaf(v[k] - m, r, shift) * (weight != nullptr ? w[k] : 1.0f);
         if (bias != nullptr) v[k] += b[k];
       }
       store_floats<T, W>(y + c, v, columns - c);
     }
     if (threadIdx.x == 0) {
-      if (mean != nullptr) mean[row] = m;
+      if (mean != nullptr) mean[row] = m + rest;
       if (rstd != nullptr) rstd[row] = r;
     }
   }

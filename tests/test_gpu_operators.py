@@ -568,6 +568,54 @@ def test_layer_norm_of_no_rows():
     assert out.shape == (0, 9)
 
 
+@pytest.mark.parametrize("kind,middle,spread", [
+    ("float32", 0.0, 1.0), ("float32", 1e4, 1.0), ("float32", -1e6, 1.0), ("float32", 3e7, 40.0),
+    ("float16", 1000.0, 3.0), ("bfloat16", -300.0, 8.0)])
+@pytest.mark.parametrize("columns", [5, 64, 100, 769, 1024, 4096, 4099, 16_384, 16_391, 100_000])
+def test_layer_norm_of_rows_far_from_zero(columns, kind, middle, spread):
+    # A sum passes through at most L additions: a thread adds up to 16 elements of a row in the
+    # registers (V vectors of W) and of a longer one its 1024th part, W at a time; then come at most
+    # six steps over lanes and four over waves.  With A the mean of |x - mean|:
+    #   the first mean is off by D = (L + 1) u mean|x|,
+    #   the mean of the deviations from it by d = (L + 2) u (A + D), and so is the second mean
+    #   (rows whose mean is at most two deviations from zero keep the first: D + d),
+    #   a deviation from that by 2 u (|x - mean| + D) + d,
+    #   the variance v by (L + 6) u (v + D D) + 2 D d + d d.
+    import torch
+    rows = 40
+    g = _rng(columns, int(abs(middle)), 91)
+    x = (middle + spread * torch.randn(rows, columns, generator=g, device="cuda",
+                                       dtype=torch.float64)).to(_t(kind))
+    weight, bias = (_normal(g, columns, dtype=torch.float32) for _ in range(2))
+    out, mean, rstd = _layer_norm(x, weight, bias)
+    L = 30 + columns / 4096
+    wide = x.double()
+    m = wide.mean(1, keepdim=True)
+    away = wide - m
+    v = (away * away).mean(1, keepdim=True)
+    r = 1.0 / (v + float(np.float32(1e-5))).sqrt()
+    D = (L + 1) * U * wide.abs().mean(1, keepdim=True)
+    d = (L + 2) * U * (away.abs().mean(1, keepdim=True) + D) + D * (m * m <= 4.01 * v)
+    r_off = ((L + 6) * U * (v + D * D) + 2 * D * d + d * d) * r * r / 2 + 4 * U     # relative
+    y = away * r * weight.double()
+    slack = (2 * U * (away.abs() + D) + d) * r * weight.abs() + y.abs() * (1.1 * r_off + 4 * U) \
+        + U * (y.abs() + bias.abs())
+    _close(mean, m[:, 0], d[:, 0])
+    _close(rstd, r[:, 0], (1.1 * r * r_off)[:, 0])
+    _close(out, y + bias.double(), slack)
+
+
+@pytest.mark.parametrize("columns", [64, 700, 20_000])
+def test_layer_norm_of_rows_with_infinities_keeps_their_mean(columns):
+    import torch
+    x = _normal(_rng(columns, 92), 6, columns, dtype=torch.float32)
+    x[1, 3], x[2, columns - 1], x[3, 0], x[3, 1] = float("inf"), float("-inf"), float("inf"), float("-inf")
+    out, mean, rstd = _layer_norm(x, None, None)
+    assert float(mean[1]) == float("inf") and float(mean[2]) == float("-inf")
+    assert bool(mean[3].isnan()) and bool(rstd[1:4].isnan().all()) and bool(out[1:4].isnan().all())
+    assert bool(torch.isfinite(out[[0, 4, 5]]).all())
+
+
 # ---- layer norm's gradient ----------------------------------------------------------
 def _layer_norm_gradient(grad, x, weight, mean, rstd, weight_type, want=("x", "w", "b"), into=None,
                          grad_x=None):
