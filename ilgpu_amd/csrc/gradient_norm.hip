@@ -153,7 +153,11 @@ __global__ __launch_bounds__(kBlock) void clip_kernel(TensorTable table,
   const float n = norm[0];
   // (false for NaN; an infinite norm gives no factor either)
   const bool clipped = n > max_norm && n <= 3.402823466e+38f;
-  const float factor = clipped ? max_norm / n : 1.0f;
+  // A factor below the normal numbers has few bits: it is made 2^120 times as large, which gives
+  // products of at most 2^120 max_norm, and taken back behind the product.
+  const bool tiny = clipped && max_norm / n < 0x1p-126f;
+  const float factor = tiny ? max_norm * 0x1p120f / n : clipped ? max_norm / n : 1.0f;
+  const float back = tiny ? 0x1p-120f : 1.0f;
   const uint32_t chunks = table.chunks_end[table.count - 1];
   for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     with_chunk<kClipChunk>(table, chunk, [&](int t, auto type, int64_t from, int64_t count) {
@@ -167,10 +171,10 @@ __global__ __launch_bounds__(kBlock) void clip_kernel(TensorTable table,
           [&](const typename Pack<T, W>::vec& v, int64_t at) {
             typename Pack<T, W>::vec r;
 #pragma unroll
-            for (int k = 0; k < W; ++k) r[k] = (T)product_for<T>((float)v[k], factor);
+            for (int k = 0; k < W; ++k) r[k] = (T)product_for<T>((float)v[k] * factor, back);
             __builtin_nontemporal_store(r, reinterpret_cast<typename Pack<T, W>::type*>(target + at));
           },
-          [&](int64_t at) { target[at] = (T)product_for<T>((float)source[at], factor); });
+          [&](int64_t at) { target[at] = (T)product_for<T>((float)source[at] * factor, back); });
     });
   }
 }

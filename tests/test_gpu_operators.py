@@ -845,6 +845,23 @@ def test_gradient_norm_beyond_float32_squares():
         assert abs(float(_norm([t])) - exact) <= 1.01 * U * exact
 
 
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+@pytest.mark.parametrize("max_norm", [2.0, 1.0, 1e-3, 1e-10, 1e-30, 0.0])
+def test_clipping_by_factors_below_the_normal_numbers(max_norm, kind):
+    # 1 / 3e38 is a subnormal number; norm, factor and product are rounded once each.
+    import torch
+    from ilgpu_amd import capi
+    array = capi.DeviceArray.from_tensor
+    t = torch.randn(10_007, generator=_rng(113), device="cuda", dtype=torch.float64)
+    t = (t * (3e38 / float(t.norm()))).to(_t(kind))
+    norm = _norm([t])
+    assert 2.9e38 < float(norm) < 3.1e38
+    out = torch.empty_like(t)
+    capi.clip_gradients([array(t)], array(norm), max_norm, [array(out)])
+    exact = t.double() * (float(np.float32(max_norm)) / _exact_norm([t]))
+    _close(out, exact, 3 * U * exact.abs())
+
+
 @pytest.mark.parametrize("bad", ["inf", "-inf", "nan"])
 def test_clipping_leaves_gradients_of_no_finite_norm(bad):
     import torch
