@@ -379,10 +379,14 @@ def _equal_sums(out, grad, tokens, vocabulary):
     """out is the sum of each token's rows, to the bit."""
     import torch
     wide = tokens.long()
-    there = (wide >= 0) & (wide < vocabulary)
-    exact = torch.zeros(vocabulary, grad.shape[1], dtype=torch.float64, device="cuda")
-    exact.index_add_(0, wide[there], grad.double()[there])
-    assert torch.equal(out.double(), exact)
+    at = torch.nonzero((wide >= 0) & (wide < vocabulary))[:, 0]
+    at = at[wide[at].argsort()]
+    # sums up to each token's last row less those up to the one before it, all whole numbers
+    sums = torch.zeros(len(at) + 1, grad.shape[1], dtype=torch.float64, device="cuda")
+    sums[1:] = grad.double()[at].cumsum(0)
+    counts = torch.bincount(wide[at], minlength=vocabulary)
+    ends = counts.cumsum(0)
+    assert torch.equal(out.double(), sums[ends] - sums[ends - counts])
 
 
 @pytest.mark.parametrize("token_type", ["int32", "int64"])
@@ -435,6 +439,53 @@ def test_embedding_gradient_of_fewer_tokens_in_the_same_temp(most, vocabulary, d
                                 capi.DeviceArray.from_tensor(tokens),
                                 capi.DeviceMatrix.from_tensor(out), temp)
         _equal_sums(out, grad, tokens, vocabulary)
+
+
+@pytest.mark.parametrize("grad_type", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dimension", [1, 36, 100, 513])
+@pytest.mark.parametrize("distribution", ["one", "two", "alternating", "runs", "ascending",
+                                          "mostly_one"])
+@pytest.mark.parametrize("n", [31, 65, 1000, 1024, 30_000, 120_001, 131_073])
+def test_embedding_gradient_sums_skewed_tokens_to_the_bit(n, distribution, dimension, grad_type):
+    # A sum that misses a row, or has one twice, is another number, however long its run.
+    import torch
+    vocabulary = 513
+    at = torch.arange(n, device="cuda")
+    tokens = {"one": at * 0 + 512, "two": (at * 7 // n) % 2 * 511, "alternating": at % 2,
+              "runs": at // 40 % vocabulary, "ascending": at % vocabulary,
+              "mostly_one": torch.where(at % 11 == 0, at % vocabulary, 7)}[distribution]
+    grad = _whole_numbers(_rng(n, dimension, 93), n, dimension, dtype=_t(grad_type))
+    _equal_sums(_embedding_gradient(grad, tokens, vocabulary, torch.float32), grad, tokens, vocabulary)
+
+
+# Runs of lengths around whole chunks, in the four ways that positions are grouped and cut: chunks of
+# 8 up to 32736 tokens of at most 256 columns, of 32 beyond; grouped in one launch up to 131072
+# tokens of at most 2^20 rows, sorted beyond.
+RUNS = {"grouped_8": (8, (1, 2, 3, 63, 64, 65, 257, 700), 1),
+        "sorted_8": (8, (1, 2, 3, 63, 64, 65, 257, 700), 50_000),
+        "grouped_32": (32, (1, 2, 3, 63, 64, 65, 128, 257, 320), 1),
+        "sorted_32": (32, (1, 2, 3, 63, 64, 65, 257, 1500), 1)}
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("shuffled", [False, True])
+@pytest.mark.parametrize("dimension", [1, 5, 64, 130, 256])
+@pytest.mark.parametrize("way", sorted(RUNS))
+def test_embedding_gradient_of_runs_about_whole_chunks(way, dimension, shuffled, accumulate):
+    import torch
+    unit, chunks, apart = RUNS[way]
+    lengths = [unit * c + more for c in chunks for more in (-1, 0, 1)]
+    n, vocabulary = sum(lengths), (len(lengths) - 1) * apart + 1
+    assert (n <= 32 * 1023) == (unit == 8)
+    assert (n <= 1 << 17 and vocabulary <= 1 << 20) == way.startswith("grouped")
+    g = _rng(n, dimension, vocabulary)
+    tokens = torch.repeat_interleave(torch.arange(len(lengths)) * apart, torch.tensor(lengths)).cuda()
+    if shuffled:
+        tokens = tokens[torch.randperm(n, generator=g, device="cuda")]
+    grad = _whole_numbers(g, n, dimension)
+    old = _whole_numbers(g, vocabulary, dimension) if accumulate else None
+    out = _embedding_gradient(grad, tokens, vocabulary, torch.float32, into=old)
+    _equal_sums(out if old is None else out - old, grad, tokens, vocabulary)
 
 
 # ---- layer norm -------------------------------------------------------------------
