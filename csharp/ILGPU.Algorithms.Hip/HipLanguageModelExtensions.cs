@@ -58,20 +58,26 @@ namespace ILGPU.Algorithms.Hip
         internal unsafe void* Ptr => HipLanguageModelExtensions.PtrOf(View);
     }
 
-    /// <summary>A list of views for the calls over many tensors.</summary>
+    /// <summary>A list of views for the calls over many tensors.  It keeps their
+    /// buffers: memory that nothing else refers to is not collected before the list
+    /// is.</summary>
     public sealed unsafe class HipTensorList
     {
         private readonly List<HipTensor> tensors = new List<HipTensor>();
+        private readonly List<object> views = new List<object>();
 
         public int Count => tensors.Count;
 
-        public void Add<T>(ArrayView<T> view) where T : unmanaged =>
+        public void Add<T>(ArrayView<T> view) where T : unmanaged
+        {
             tensors.Add(new HipTensor
             {
                 Data = HipLanguageModelExtensions.PtrOf(view),
                 Length = view.Length,
                 Type = HipTypeMap.ElementType<T>(),
             });
+            views.Add(view);
+        }
 
         internal HipTensor[] ToArray() => tensors.ToArray();
     }
@@ -264,6 +270,7 @@ namespace ILGPU.Algorithms.Hip
                         HipStream.PtrOf(stream), tensors, gradients.Count, (float*)PtrOf(norm),
                         PtrOf(temp), temp.Length * sizeof(int)),
                     nameof(temp));
+            GC.KeepAlive(gradients);
         }
 
         /// <summary>gradients *= maxNorm / norm[0] where norm[0] is finite and the larger,
@@ -286,6 +293,8 @@ namespace ILGPU.Algorithms.Hip
                         HipStream.PtrOf(stream), sources, places, gradients.Count,
                         (float*)PtrOf(norm), &maxNorm),
                     nameof(gradients));
+            GC.KeepAlive(gradients);
+            GC.KeepAlive(targets);
         }
     }
 }

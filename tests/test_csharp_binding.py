@@ -204,3 +204,16 @@ def test_reference_surface_of_the_neighbouring_primitives_is_there():
                     "Int8Sequencer", "UInt16Sequencer", "HalfSequencer", "FloatSequencer",
                     "DoubleSequencer", "IdentityTransformer"]:
         assert functor in type_map, functor
+
+
+def test_a_tensor_list_keeps_the_buffers_of_its_views():
+    # Its entries are bare pointers; a buffer that nothing refers to is collected, and its
+    # device memory freed, although the list is used again.
+    text = strip_comments(open(os.path.join(CSHARP, "HipLanguageModelExtensions.cs")).read())
+    body = text[text.index("class HipTensorList"):text.index("static unsafe class HipLanguageModelExtensions")]
+    kept = re.search(r"List<object>\s+(\w+)\s*=", body)
+    add = body[body.index("void Add<T>"):]
+    assert kept and re.search(r"\b" + kept.group(1) + r"\.Add\(view\)", add)
+    for call, lists in (("ilgpu_hip_gradient_norm", 1), ("ilgpu_hip_clip_gradients", 2)):
+        behind = text[re.search(r"\b" + call + r"\s*\(", text).end():].split("public static")[0]
+        assert behind.count("GC.KeepAlive(") == lists, call
