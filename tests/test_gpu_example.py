@@ -45,3 +45,14 @@ def test_the_model_learns(activations):
     losses = token_model.main(steps=41, vocabulary=128, dimension=128, positions=2048,
                               activations=getattr(torch, activations))
     assert losses[0] > 4.0 and losses[-1] < 0.7 * losses[0]
+
+
+def test_a_step_over_fewer_positions_than_the_model_was_made_for():
+    # The scratch was taken for 4096 positions; a last batch is a little shorter.
+    import token_model
+    import torch
+    model = token_model.TokenModel(300, 2048, 4096)
+    tokens = torch.arange(4097, device="cuda") * 7 % 300
+    for n in (4096, 4064, 100, 1):
+        loss = model.step(tokens[:n], tokens[1:n + 1], rate=0.01)
+        assert math.isfinite(float(loss)) and math.isfinite(float(model.norm))
