@@ -598,7 +598,13 @@ __device__ __forceinline__ uint64_t positions_of(uint64_t inside, uint32_t key, 
 // of the table (64 tokens, us, this / three launches: into 1000 x 64 5.6 / 12.3, into 30000 x
 // 512 10.9 / 18.7, into 131072 x 1024 89 / 98; the worst, 64 times one token of 4096 columns,
 // 19.7 / 13.8).
+//
+// Accumulated, only the tokens' rows are written, but the launch still has blocks for all rows
+// (64 tokens, us, this / three launches: into 32768 x 1024 8.6 / 13.8, 49152 x 1024 11.3 / 13.7, 65536 x
+// 1024 14.1 / 13.9, 131072 x 4096 52 / 13.7; 2^19 x 128 14.0 / 18.7, 2^19 x 256 26.1 / 18.3, 2^21 x 64 26.3 /
+// 17.3): up to kFewBytes of table, more where the grouping takes more blocks or is a sort.
 constexpr int64_t kFewTokens = kWaveSize;
+constexpr int64_t kFewBytes = 192 << 20, kFewBytesOfManyRows = 320 << 20;
 template <typename TG, typename TW, typename TT, int W>
 __global__ __launch_bounds__(kBlock) void embedding_gradient_of_few_kernel(
     Sums s, const TT* __restrict__ tokens, int64_t padding_token, const TG* __restrict__ grad_out,
@@ -853,6 +859,12 @@ static int32_t launch_gradient_of_few(hipStream_t stream, const EmbeddingGradien
   });
 }
 
+static bool takes_one_launch(const EmbeddingGradientArgs& a) {
+  if (a.count > kFewTokens || !a.accumulate) return a.count <= kFewTokens;
+  const int64_t most = group_log2(a.vocabulary) > kGroupMinLog2 ? kFewBytesOfManyRows : kFewBytes;
+  return a.vocabulary <= most / (a.dimension * operator_elem_size(a.table_type));
+}
+
 // Whether the sums' launch, with the blocks that clear rows, has fewer threads than a grid can
 // hold (2^32) and its items fit their 32 bits: not so only where the parts alone take 100 GB.
 static bool grid_holds(const GradientTemp& t, const EmbeddingGradientArgs& a) {
@@ -885,7 +897,7 @@ int32_t launch_embedding_gradient(hipStream_t stream, const EmbeddingGradientArg
     const int32_t rc = check_sort_device(stream);  // before anything is launched
     if (rc != ILGPU_HIP_SUCCESS) return rc;
   }
-  if (a.count <= kFewTokens) return launch_gradient_of_few(stream, a);
+  if (takes_one_launch(a)) return launch_gradient_of_few(stream, a);
   char* base = reinterpret_cast<char*>(align_up((int64_t)(uintptr_t)a.temp, 256));
   uint32_t* keys = reinterpret_cast<uint32_t*>(base + t.keys);
   uint32_t* order = reinterpret_cast<uint32_t*>(base + t.order);

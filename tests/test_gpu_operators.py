@@ -441,6 +441,31 @@ def test_embedding_gradient_of_fewer_tokens_in_the_same_temp(most, vocabulary, d
         _equal_sums(out, grad, tokens, vocabulary)
 
 
+@pytest.mark.parametrize("n", [1, 33, 64])
+@pytest.mark.parametrize("vocabulary,dimension,in_one", [
+    (49_152, 1024, True), (65_536, 1024, False), (300_000, 200, True), (300_000, 300, False),
+    (1_100_000, 60, True), (1_100_000, 100, False)])
+def test_embedding_gradient_of_few_tokens_accumulated_into_large_tables(vocabulary, dimension,
+                                                                        in_one, n):
+    # One launch has blocks for every row of the table, which is more than the tokens' rows take.
+    import torch
+    from ilgpu_amd import capi
+    g = _rng(vocabulary, dimension, n)
+    tokens = _tokens(g, n, vocabulary, torch.int64)
+    tokens[: n // 2] = tokens[n // 2:n // 2 * 2].clone()
+    grad = _whole_numbers(g, n, dimension)
+    old = _whole_numbers(g, vocabulary, dimension)
+    capi.profile_enable(True)
+    try:
+        out = _embedding_gradient(grad, tokens, vocabulary, torch.float32, into=old)
+        torch.cuda.synchronize()
+        launches = capi.profile_query("embedding_gradient_of_few")[0]
+    finally:
+        capi.profile_enable(False)
+    assert launches == (1 if in_one else 0)
+    _equal_sums(out - old, grad, tokens, vocabulary)
+
+
 @pytest.mark.parametrize("grad_type", ["float32", "bfloat16"])
 @pytest.mark.parametrize("dimension", [1, 36, 100, 513])
 @pytest.mark.parametrize("distribution", ["one", "two", "alternating", "runs", "ascending",
