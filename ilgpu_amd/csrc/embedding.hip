@@ -30,8 +30,9 @@ template <typename TI, typename TO> struct Width {
 // outside the table reads its first row and stores zeros.
 //
 // 65536 x 4096 bfloat16 from 131072 rows, us: 143 (one row at a time 152, plain stores 151).
-// 537 MB are written, and as much is read, a row of the table 3.4 times on average and mostly
-// from the last-level cache: 7.5 TB/s together.
+// 512 MiB are written and as much is asked for, a row of the table 3.4 times on average.  304 MiB
+// of it pass the eight L2s, each of which fetches the frequent rows for itself; 151 are distinct
+// and fit the last-level cache, so how much comes from HBM is not known.
 constexpr int kRowsAtOnce = 4;
 template <typename TI, typename TO, typename TT, int W, int U>
 __global__ __launch_bounds__(kBlock) void embedding_kernel(
@@ -154,8 +155,9 @@ inline bool takes_groups(int64_t count, int64_t vocabulary) {
 // The table's last rows from `first` on, which further blocks of the grouping clear, met or
 // not: the sums of those that are met come later.  In units of 16 bits, whatever the type.  As
 // many bytes as are written while the grouping computes, whose blocks leave room for a second
-// one on a compute unit (64 registers; with more of them nothing is gained): 8192 tokens into
-// 50021 x 1024 42.4 to 39.4 us, 65536 into 131072 x 2048 260 to 255.
+// one on a compute unit (64 registers, of which tokens of 64 bits keep 28 bytes a lane in scratch,
+// outside of loops; with more registers nothing is gained): 8192 tokens into 50021 x 1024 42.4 to
+// 39.4 us, 65536 into 131072 x 2048 260 to 255.
 constexpr int64_t kGroupClearBytes = 24 << 20, kGroupClearPerToken = 900;
 struct Clearing {
   uint16_t* table;
@@ -595,9 +597,9 @@ __device__ __forceinline__ uint64_t positions_of(uint64_t inside, uint32_t key, 
 
 // Up to 64 tokens, in one launch: every wave holds them all, one a lane, and each row of the
 // table looks for its own among them.  So few tokens are bound by launches and by the clearing
-// of the table (64 tokens, us, this / three launches: into 1000 x 64 5.6 / 12.3, into 30000 x
-// 512 10.9 / 18.7, into 131072 x 1024 89 / 98; the worst, 64 times one token of 4096 columns,
-// 19.7 / 13.8).
+// of the table (64 tokens, us, this / three launches: into 1000 x 64 5.9 / 13.0, into 30000 x
+// 512 11.1 / 19.0, into 131072 x 1024 91 / 97; the worst, 64 times one token of 4096 columns,
+// 19.7 / 14.7).
 //
 // Accumulated, only the tokens' rows are written, but the launch still has blocks for all rows
 // (64 tokens, us, this / three launches: into 32768 x 1024 8.6 / 13.8, 49152 x 1024 11.3 / 13.7, 65536 x
@@ -866,7 +868,8 @@ static bool takes_one_launch(const EmbeddingGradientArgs& a) {
 }
 
 // Whether the sums' launch, with the blocks that clear rows, has fewer threads than a grid can
-// hold (2^32) and its items fit their 32 bits: not so only where the parts alone take 100 GB.
+// hold (2^32) and its items fit their 32 bits: not so only where there are more than 12.5 million
+// blocks of sums, whose parts take more than 50 GB.
 static bool grid_holds(const GradientTemp& t, const EmbeddingGradientArgs& a) {
   const int gb = operator_elem_size(a.grad_out_type), wb = operator_elem_size(a.table_type);
   const int wide = 16 / (gb > wb ? gb : wb), W = a.dimension >= wide ? wide : 1;

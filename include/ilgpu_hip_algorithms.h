@@ -439,7 +439,8 @@ int32_t ilgpu_hip_reorder_transform(ilgpu_hip_stream_t stream,
  *    row stride of a matrix that is read may be anything from 0 (one row for
  *    all); that of a matrix that is written is at least its columns
  *    (ILGPU_HIP_ERROR_OUT_OF_RANGE otherwise).  Any element-aligned base and any
- *    stride will do; rows need no alignment of their own.
+ *    stride up to INT32_MAX, as of rows and columns, will do; rows need no
+ *    alignment of their own.
  *  - Types are ILGPU_HIP_F32, F16 and BF16 (others: ILGPU_HIP_ERROR_NOT_SUPPORTED).
  *    All arithmetic is in float32 or wider; each result is rounded to its type
  *    once, to nearest even.
@@ -489,7 +490,10 @@ int32_t ilgpu_hip_embedding_gradient(
  * (`columns` elements of weight_type, which is `type` or F32) may be NULL: 1 and
  * 0.  mean and rstd (float32, one per row) receive m and r and may be NULL.
  * in and out have the same type; out may be in itself (same base and stride).
- * epsilon: finite and not negative. */
+ * epsilon: finite and not negative.  Of a row whose mean is more than two
+ * deviations from zero the mean is found in two steps, so that its size costs
+ * out and rstd no bits.  Squared deviations are float32: a row with deviations
+ * beyond 1e19 overflows (rstd 0), as one with an infinity is NaN. */
 int32_t ilgpu_hip_layer_norm(ilgpu_hip_stream_t stream, const void *in,
                              int64_t rows, int64_t columns, int64_t in_stride,
                              int32_t type, const void *weight,
@@ -502,6 +506,8 @@ int32_t ilgpu_hip_layer_norm(ilgpu_hip_stream_t stream, const void *in,
  *   grad_in     = rstd * (g - mean of g - h * mean of g * h)   (means over the row)
  *   grad_weight = sum over the rows of grad_out * h
  *   grad_bias   = sum over the rows of grad_out
+ * (mean is a float32: where it is large against the row's deviations, its rounding
+ * is in every h.)
  * weight may be NULL (1).  Each of grad_in, grad_weight and grad_bias may be NULL
  * and is not computed then; not all of them.  grad_in may be grad_out itself or in
  * itself (same base and stride).  With accumulate != 0 grad_weight and grad_bias
