@@ -117,5 +117,45 @@ namespace ILGPU.Algorithms.Hip
         [DllImport(LibName)] internal static extern int ilgpu_hip_clip_gradients(
             IntPtr stream, HipTensor* hostSources, HipTensor* hostTargets, long count,
             float* norm, float* hostMaxNorm);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_gated_recurrence_temp_bytes(
+            long rows, long channels, out long tempBytes);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_gated_recurrence(
+            IntPtr stream, void* gate, long gateStride, void* input, long inStride, long rows,
+            long channels, int type, int decay, int complement, void* offsets, int offsetType,
+            long sequences, float* initial, long initialStride, void* output, long outStride,
+            float* finalState, long finalStride, void* temp, long tempBytes);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_gated_recurrence_gradient(
+            IntPtr stream, void* gradOut, long gradOutStride, void* gate, long gateStride,
+            void* input, long inStride, void* output, long outStride, long rows, long channels,
+            int type, int decay, int complement, void* offsets, int offsetType, long sequences,
+            float* initial, long initialStride, float* gradFinal, long gradFinalStride,
+            void* gradGate, long gradGateStride, void* gradIn, long gradInStride,
+            float* gradInitial, long gradInitialStride, void* temp, long tempBytes);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_residual_norm(
+            IntPtr stream, void* input, long inStride, long rows, long columns, int type,
+            int inputNorm, void* inputWeight, void* gate, long gateStride, int gateKind,
+            void* residual, long residualStride, int residualType, float* hostScale,
+            void* weight, int weightType, float* hostEpsilon, void* total, long totalStride,
+            void* output, long outStride, float* inputRstd, float* rstd);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_residual_norm_gradient_temp_bytes(
+            long rows, long columns, out long tempBytes);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_residual_norm_gradient(
+            IntPtr stream, void* gradOut, long gradOutStride, void* gradTotal,
+            long gradTotalStride, void* input, long inStride, long rows, long columns, int type,
+            int inputNorm, void* inputWeight, float* inputRstd, void* gate, long gateStride,
+            int gateKind, void* total, long totalStride, int residualType, float* hostScale,
+            void* weight, int weightType, float* rstd, void* gradIn, long gradInStride,
+            void* gradGate, long gradGateStride, void* gradResidual, long gradResidualStride,
+            void* gradInputWeight, void* gradWeight, int accumulate, void* temp,
+            long tempBytes);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_adamw(
+            IntPtr stream, HipTensor* hostParameters, HipTensor* hostGradients,
+            HipTensor* hostFirst, HipTensor* hostSecond, HipTensor* hostFirstScales,
+            HipTensor* hostSecondScales, HipTensor* hostCopies, long count,
+            HipAdamWNumbers* hostOptions, long* step, float* schedule, float* norm);
+        [DllImport(LibName)] internal static extern int ilgpu_hip_adamw_moments(
+            IntPtr stream, HipTensor* hostFirst, HipTensor* hostFirstScales,
+            HipTensor* hostFirstTargets, HipTensor* hostSecond, HipTensor* hostSecondScales,
+            HipTensor* hostSecondTargets, long count);
     }
 }

@@ -122,6 +122,8 @@ HOST_TEST_SRC = os.path.join(CPP_TESTS, "host_api_tests.cpp")
 HOST_TEST_BIN = os.path.join(CPP_TESTS, "host_api_tests")
 OPERATOR_TEST_SRC = os.path.join(CPP_TESTS, "operator_tests.cpp")
 OPERATOR_TEST_BIN = os.path.join(CPP_TESTS, "operator_tests")
+RECURRENT_TEST_SRC = os.path.join(CPP_TESTS, "recurrent_operator_tests.cpp")
+RECURRENT_TEST_BIN = os.path.join(CPP_TESTS, "recurrent_operator_tests")
 
 
 def build_host_example(source: str = HOST_TEST_SRC, binary: str = HOST_TEST_BIN) -> str:
@@ -151,4 +153,5 @@ if __name__ == "__main__":
         print(build())
         print(build_host_example())
         print(build_host_example(OPERATOR_TEST_SRC, OPERATOR_TEST_BIN))
+        print(build_host_example(RECURRENT_TEST_SRC, RECURRENT_TEST_BIN))
         print(build_bounds())

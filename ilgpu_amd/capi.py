@@ -38,6 +38,9 @@ VALUES_FROM_VIEW, VALUES_FROM_INDEX, VALUES_FROM_INDEX_AS_FLOAT = 0, 1, 2
 LOCATOR_IDENTITY, LOCATOR_MODULO = 0, 1
 (TRANSFORM_CONVERT, TRANSFORM_NEGATE, TRANSFORM_BIT_COMPLEMENT,
  TRANSFORM_MULTIPLY) = 0, 1, 2, 3
+DECAY_SIGMOID, DECAY_EXPONENTIAL = 0, 1
+GATE_SIGMOID, GATE_SILU = 0, 1
+ADAMW_MOMENT_BLOCK = 256
 
 EXPORTS = [
     "ilgpu_hip_version", "ilgpu_hip_status_string",
@@ -57,7 +60,10 @@ EXPORTS = [
     "ilgpu_hip_embedding_gradient", "ilgpu_hip_layer_norm",
     "ilgpu_hip_layer_norm_gradient_temp_bytes", "ilgpu_hip_layer_norm_gradient",
     "ilgpu_hip_gradient_norm_temp_bytes", "ilgpu_hip_gradient_norm",
-    "ilgpu_hip_clip_gradients",
+    "ilgpu_hip_clip_gradients", "ilgpu_hip_gated_recurrence_temp_bytes",
+    "ilgpu_hip_gated_recurrence", "ilgpu_hip_gated_recurrence_gradient",
+    "ilgpu_hip_residual_norm", "ilgpu_hip_residual_norm_gradient_temp_bytes",
+    "ilgpu_hip_residual_norm_gradient", "ilgpu_hip_adamw", "ilgpu_hip_adamw_moments",
 ]
 
 # numpy has no bfloat16: a dtype of its own that holds the 16 bits, so that a
@@ -181,6 +187,23 @@ def lib() -> ctypes.CDLL:
         L.ilgpu_hip_gradient_norm_temp_bytes.argtypes = [i64, p64]
         L.ilgpu_hip_gradient_norm.argtypes = [vp, vp, i64, vp, vp, i64]
         L.ilgpu_hip_clip_gradients.argtypes = [vp, vp, vp, i64, vp, pf]
+        L.ilgpu_hip_gated_recurrence_temp_bytes.argtypes = [i64, i64, p64]
+        L.ilgpu_hip_gated_recurrence.argtypes = [
+            vp, vp, i64, vp, i64, i64, i64, i32, i32, i32, vp, i32, i64, vp, i64, vp, i64, vp, i64,
+            vp, i64]
+        L.ilgpu_hip_gated_recurrence_gradient.argtypes = [
+            vp, vp, i64, vp, i64, vp, i64, vp, i64, i64, i64, i32, i32, i32, vp, i32, i64, vp, i64,
+            vp, i64, vp, i64, vp, i64, vp, i64, vp, i64]
+        L.ilgpu_hip_residual_norm.argtypes = [
+            vp, vp, i64, i64, i64, i32, i32, vp, vp, i64, i32, vp, i64, i32, pf, vp, i32, pf, vp,
+            i64, vp, i64, vp, vp]
+        L.ilgpu_hip_residual_norm_gradient_temp_bytes.argtypes = [i64, i64, p64]
+        L.ilgpu_hip_residual_norm_gradient.argtypes = [
+            vp, vp, i64, vp, i64, vp, i64, i64, i64, i32, i32, vp, vp, vp, i64, i32, vp, i64, i32,
+            pf, vp, i32, vp, vp, i64, vp, i64, vp, i64, vp, vp, i32, vp, i64]
+        L.ilgpu_hip_adamw.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, i64,
+                                      ctypes.POINTER(_AdamwOptions), vp, vp, vp]
+        L.ilgpu_hip_adamw_moments.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64]
         for name in EXPORTS:
             if name.endswith(("_bytes", "_keys", "_pairs", "_scan", "_reduce",
                               "_histogram")):
@@ -345,6 +368,12 @@ class DeviceMatrix:
 class _Tensor(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("length", ctypes.c_int64),
                 ("type", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class _AdamwOptions(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_double) for name in (
+        "rate", "beta1", "beta2", "epsilon", "weight_decay", "max_norm")] + [
+        ("seed", ctypes.c_int64)]
 
 
 class TensorList:
@@ -763,3 +792,229 @@ def clip_gradients(gradients, norm: DeviceArray, max_norm: float, targets=None, 
     check((_lib or lib()).ilgpu_hip_clip_gradients(
         _stream_ptr(stream), gradients.table, None if targets is None else targets.table,
         len(gradients), _statistic(norm, 1, "norm"), _float(max_norm)))
+
+
+def _same_type(first: DeviceMatrix, *others) -> None:
+    for m in others:
+        if m is not None and m.type_code != first.type_code:
+            raise NotSupportedError(ERROR_NOT_SUPPORTED, "types differ")
+
+
+def _same_shape(first: DeviceMatrix, **others) -> None:
+    for what, m in others.items():
+        if m is not None and (m.rows != first.rows or m.columns != first.columns):
+            raise ArgumentOutOfRangeError(ERROR_OUT_OF_RANGE, what)
+
+
+def _matrix(m: Optional[DeviceMatrix]):
+    return (None, 0) if m is None else (m.ptr, m.row_stride)
+
+
+def _states(m: Optional[DeviceMatrix], sequences: int, channels: int, what: str):
+    """A float32 matrix of one row for each sequence."""
+    if m is None:
+        return None, 0
+    if m.type_code != F32:
+        raise NotSupportedError(ERROR_NOT_SUPPORTED, f"{what} is float32")
+    _need(m.rows == sequences and m.columns == channels, what)
+    return m.ptr, m.row_stride
+
+
+def _offsets(offsets: Optional[DeviceArray], sequences: int):
+    if offsets is None:
+        return None, I32
+    _need(_dense(offsets).length == sequences + 1, "offsets")
+    return offsets.ptr, offsets.type_code
+
+
+def gated_recurrence_temp_bytes(rows: int, channels: int) -> int:
+    """0 where a call over so many rows needs no temp."""
+    return _query(lib().ilgpu_hip_gated_recurrence_temp_bytes, rows, channels)
+
+
+def _recurrence_temp(temp, rows: int, channels: int, step: bool, stream):
+    if temp is None and not step:
+        nbytes = gated_recurrence_temp_bytes(rows, channels)
+        temp = _scratch(nbytes, stream) if nbytes > 0 else None
+    return (None, 0) if temp is None else (temp.ptr, temp.nbytes)
+
+
+def gated_recurrence(gate: DeviceMatrix, inp: DeviceMatrix, out: DeviceMatrix,
+                     temp: Optional[DeviceArray] = None, *, sequences: int = 1,
+                     offsets: Optional[DeviceArray] = None,
+                     initial: Optional[DeviceMatrix] = None,
+                     final: Optional[DeviceMatrix] = None, decay: int = DECAY_SIGMOID,
+                     complement: bool = False, stream=None) -> None:
+    """out[t] = h[t] = a * h[t-1] + b in every channel (column) of every sequence of rows, with
+    a = sigmoid(gate) or exp(gate) and b = inp or (1 - a) * inp.  The rows are `sequences`
+    equal parts, or cut at offsets (sequences + 1 of them, int32 or int64).  initial and
+    final (float32, one row a sequence) are the states in front and behind; one row a
+    sequence is the step from token to token."""
+    _same_shape(inp, gate=gate, out=out)
+    _same_type(inp, gate, out)
+    rows, channels = inp.rows, inp.columns
+    temp_ptr, temp_bytes = _recurrence_temp(temp, rows, channels,
+                                            offsets is None and sequences == rows, stream)
+    check((_lib or lib()).ilgpu_hip_gated_recurrence(
+        _stream_ptr(stream), gate.ptr, gate.row_stride, inp.ptr, inp.row_stride, rows, channels,
+        inp.type_code, decay, 1 if complement else 0, *_offsets(offsets, sequences), sequences,
+        *_states(initial, sequences, channels, "initial"), out.ptr, out.row_stride,
+        *_states(final, sequences, channels, "final"), temp_ptr, temp_bytes))
+
+
+def gated_recurrence_gradient(grad_out: DeviceMatrix, gate: DeviceMatrix, inp: DeviceMatrix,
+                              out: DeviceMatrix, grad_gate: Optional[DeviceMatrix] = None,
+                              grad_in: Optional[DeviceMatrix] = None,
+                              temp: Optional[DeviceArray] = None, *, sequences: int = 1,
+                              offsets: Optional[DeviceArray] = None,
+                              initial: Optional[DeviceMatrix] = None,
+                              grad_final: Optional[DeviceMatrix] = None,
+                              grad_initial: Optional[DeviceMatrix] = None,
+                              decay: int = DECAY_SIGMOID, complement: bool = False,
+                              stream=None) -> None:
+    """The gradients of gated_recurrence from those of out and of final (none: zeros), and
+    from out as it left it; those passed as None are not computed."""
+    _same_shape(inp, grad_out=grad_out, gate=gate, out=out, grad_gate=grad_gate, grad_in=grad_in)
+    _same_type(inp, grad_out, gate, out, grad_gate, grad_in)
+    rows, channels = inp.rows, inp.columns
+    temp_ptr, temp_bytes = _recurrence_temp(temp, rows, channels, False, stream)
+    check((_lib or lib()).ilgpu_hip_gated_recurrence_gradient(
+        _stream_ptr(stream), grad_out.ptr, grad_out.row_stride, gate.ptr, gate.row_stride,
+        inp.ptr, inp.row_stride, out.ptr, out.row_stride, rows, channels, inp.type_code, decay,
+        1 if complement else 0, *_offsets(offsets, sequences), sequences,
+        *_states(initial, sequences, channels, "initial"),
+        *_states(grad_final, sequences, channels, "grad_final"), *_matrix(grad_gate),
+        *_matrix(grad_in), *_states(grad_initial, sequences, channels, "grad_initial"),
+        temp_ptr, temp_bytes))
+
+
+def _weights(columns: int, otherwise: int, **vectors):
+    """The type of the vectors that are there, and a pointer for each."""
+    there = [a for a in vectors.values() if a is not None]
+    kind = there[0].type_code if there else otherwise
+    if any(a.type_code != kind for a in there):
+        raise NotSupportedError(ERROR_NOT_SUPPORTED, "types differ")
+    return (kind, *(_column_vector(a, columns, what) for what, a in vectors.items()))
+
+
+def residual_norm(inp: DeviceMatrix, residual: Optional[DeviceMatrix],
+                  total: Optional[DeviceMatrix], out: Optional[DeviceMatrix],
+                  weight: Optional[DeviceArray] = None, *, scale: float = 1.0,
+                  gate: Optional[DeviceMatrix] = None, gate_kind: int = GATE_SILU,
+                  input_norm: Optional[bool] = None, input_weight: Optional[DeviceArray] = None,
+                  epsilon: float = 1e-5, input_rstd: Optional[DeviceArray] = None,
+                  rstd: Optional[DeviceArray] = None, stream=None) -> None:
+    """total = residual + scale * y and out = total * rstd * weight, with y = inp
+    [* input_rstd * input_weight] [* act(gate)] and rstd = 1 / sqrt(mean of the row's
+    squares + epsilon), input_rstd the same of inp.  inp is normalised with input_norm, which
+    an input_weight or input_rstd stands for.  input_rstd and rstd (float32) receive what the
+    gradients need."""
+    if input_norm is None:
+        input_norm = input_weight is not None or input_rstd is not None
+    _same_shape(inp, residual=residual, total=total, out=out, gate=gate)
+    _same_type(inp, gate, out)
+    stream_type = next((m.type_code for m in (residual, total) if m is not None), inp.type_code)
+    if total is not None and total.type_code != stream_type:
+        raise NotSupportedError(ERROR_NOT_SUPPORTED, "types differ")
+    kind, weight_ptr, input_ptr = _weights(inp.columns, inp.type_code, weight=weight,
+                                           input_weight=input_weight)
+    check((_lib or lib()).ilgpu_hip_residual_norm(
+        _stream_ptr(stream), inp.ptr, inp.row_stride, inp.rows, inp.columns, inp.type_code,
+        1 if input_norm else 0, input_ptr, *_matrix(gate), gate_kind, *_matrix(residual),
+        stream_type, _float(scale), weight_ptr, kind, _float(epsilon), *_matrix(total),
+        *_matrix(out), _statistic(input_rstd, inp.rows, "input_rstd"),
+        _statistic(rstd, inp.rows, "rstd")))
+
+
+def residual_norm_gradient_temp_bytes(rows: int, columns: int) -> int:
+    return _query(lib().ilgpu_hip_residual_norm_gradient_temp_bytes, rows, columns)
+
+
+def residual_norm_gradient(grad_out: Optional[DeviceMatrix], grad_total: Optional[DeviceMatrix],
+                           inp: DeviceMatrix, total: Optional[DeviceMatrix],
+                           weight: Optional[DeviceArray], rstd: Optional[DeviceArray],
+                           grad_in: Optional[DeviceMatrix] = None,
+                           grad_residual: Optional[DeviceMatrix] = None,
+                           grad_weight: Optional[DeviceArray] = None,
+                           temp: Optional[DeviceArray] = None, *, scale: float = 1.0,
+                           gate: Optional[DeviceMatrix] = None, gate_kind: int = GATE_SILU,
+                           grad_gate: Optional[DeviceMatrix] = None,
+                           input_norm: Optional[bool] = None,
+                           input_weight: Optional[DeviceArray] = None,
+                           input_rstd: Optional[DeviceArray] = None,
+                           grad_input_weight: Optional[DeviceArray] = None,
+                           accumulate: bool = False, stream=None) -> None:
+    """The gradients of residual_norm from those of out (None: not used) and of total (None:
+    not used), and from total, rstd and input_rstd as it left them; those passed as None are
+    not computed.  With accumulate grad_weight and grad_input_weight are added to."""
+    if input_norm is None:
+        input_norm = input_rstd is not None
+    _same_shape(inp, grad_out=grad_out, grad_total=grad_total, total=total, grad_in=grad_in,
+                grad_residual=grad_residual, gate=gate, grad_gate=grad_gate)
+    _same_type(inp, grad_out, gate, grad_in, grad_gate)
+    of_stream = [m for m in (total, grad_total, grad_residual) if m is not None]
+    stream_type = of_stream[0].type_code if of_stream else inp.type_code
+    if any(m.type_code != stream_type for m in of_stream):
+        raise NotSupportedError(ERROR_NOT_SUPPORTED, "types differ")
+    kind, weight_ptr, input_ptr, grad_weight_ptr, grad_input_ptr = _weights(
+        inp.columns, inp.type_code, weight=weight, input_weight=input_weight,
+        grad_weight=grad_weight, grad_input_weight=grad_input_weight)
+    if temp is None:
+        temp = _scratch(residual_norm_gradient_temp_bytes(inp.rows, inp.columns), stream)
+    check((_lib or lib()).ilgpu_hip_residual_norm_gradient(
+        _stream_ptr(stream), *_matrix(grad_out), *_matrix(grad_total), inp.ptr, inp.row_stride,
+        inp.rows, inp.columns, inp.type_code, 1 if input_norm else 0, input_ptr,
+        _statistic(input_rstd, inp.rows, "input_rstd"), *_matrix(gate), gate_kind,
+        *_matrix(total), stream_type, _float(scale), weight_ptr, kind,
+        _statistic(rstd, inp.rows, "rstd"), *_matrix(grad_in), *_matrix(grad_gate),
+        *_matrix(grad_residual), grad_input_ptr, grad_weight_ptr, 1 if accumulate else 0,
+        temp.ptr, temp.nbytes))
+
+
+def _table(tensors, count: int, what: str):
+    if tensors is None:
+        return None, None
+    tensors = _tensor_list(tensors)
+    _need(len(tensors) == count, what)
+    return tensors, tensors.table
+
+
+def adamw(parameters, gradients, first, second, step: DeviceArray, *, rate: float,
+          betas=(0.9, 0.999), epsilon: float = 1e-8, weight_decay: float = 0.0,
+          first_scales=None, second_scales=None, copies=None,
+          schedule: Optional[DeviceArray] = None, norm: Optional[DeviceArray] = None,
+          max_norm: float = float("inf"), seed: int = 0, stream=None) -> None:
+    """One AdamW step, in place, over TensorLists (or lists of DeviceArrays).  step[0]
+    (int64, on the device) is its number, 1 for the first; the rate is multiplied by
+    schedule[0] (float32, on the device) where there is one.  Gradients are scaled to at most
+    max_norm by norm[0] (on the device, gradient_norm's); one that is not finite leaves
+    everything as it is.  Moments are float32, or, with scales (float32, one for each
+    ADAMW_MOMENT_BLOCK elements begun), uint8; zeros before the first step.  copies receive the
+    parameters in their own types."""
+    parameters = _tensor_list(parameters)
+    count = len(parameters)
+    kept = [_table(t, count, what) for t, what in (
+        (gradients, "gradients"), (first, "first"), (second, "second"),
+        (first_scales, "first_scales"), (second_scales, "second_scales"), (copies, "copies"))]
+    if step.type_code != I64:
+        raise NotSupportedError(ERROR_NOT_SUPPORTED, "step is int64")
+    _need(_dense(step).length >= 1, "step")
+    options = _AdamwOptions(rate, betas[0], betas[1], epsilon, weight_decay, max_norm, seed)
+    check((_lib or lib()).ilgpu_hip_adamw(
+        _stream_ptr(stream), parameters.table, *(table for _, table in kept), count,
+        ctypes.byref(options), step.ptr, _statistic(schedule, 1, "schedule"),
+        _statistic(norm, 1, "norm")))
+
+
+def adamw_moments(first=None, first_scales=None, first_targets=None, second=None,
+                  second_scales=None, second_targets=None, *, stream=None) -> None:
+    """Moments in 8 bits as the numbers they stand for, into tensors of any of the three
+    types; of the first moment, of the second, or of both."""
+    some = first if first is not None else second
+    count = 0 if some is None else len(some)
+    kept = [_table(t, count, what) for t, what in (
+        (first, "first"), (first_scales, "first_scales"), (first_targets, "first_targets"),
+        (second, "second"), (second_scales, "second_scales"),
+        (second_targets, "second_targets"))]
+    check((_lib or lib()).ilgpu_hip_adamw_moments(
+        _stream_ptr(stream), *(table for _, table in kept), count))

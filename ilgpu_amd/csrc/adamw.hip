@@ -1,0 +1,524 @@
+// One step of AdamW over a list of tensors, with moments in 32 bits or in 8.
+//
+// The lists go to the kernel by value, as many tensors a launch as fit into 4 KB of arguments, cut
+// into chunks of equal length, so tensors of any lengths fill the chip together.  The clip's
+// factor and the corrections of the moments come from device memory and are made in every block while its
+// loads are on their way.
+//
+// Moments in 8 bits share a scale, the largest of 256, which a wave holds four in each lane: it decodes
+// them, steps, finds the new largest over its lanes and encodes again.  The first stands for the square of its code,
+// the second for its fourth power (its root, which the step divides by, for the square), so small
+// values keep four and a half digits below the largest.
+//
+// Bound by the memory: everything is read once and written once.
+#include "elements.hpp"
+#include "operators.hpp"
+
+namespace ilgpu_hip {
+
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kW = 4;                         // elements of a thread side by side
+static_assert(kW * kWaveSize == kMomentBlock, "a wave has the moments of one scale");
+constexpr int kTurn = kBlock * kW;            // elements of a block at a time
+constexpr int kTurns = 4;
+constexpr int kChunk = kTurns * kTurn;
+constexpr int kTensors = 46;                  // per launch
+constexpr int64_t kMaxBlocks = 1 << 22;
+
+struct StepTable {
+  void* parameter[kTensors];
+  const void* gradient[kTensors];
+  void* first[kTensors];
+  void* second[kTensors];
+  float* first_scale[kTensors];
+  float* second_scale[kTensors];
+  void* copy[kTensors];
+  int64_t length[kTensors];
+  uint32_t chunks_end[kTensors];              // chunks of this and all tensors before it
+  uint32_t number[kTensors];                  // in the list
+  int32_t types[kTensors];                    // of parameter, gradient and copy, 8 bits each
+  int32_t count;
+};
+struct StepNumbers {
+  double log_beta1, log_beta2;
+  const int64_t* step;
+  const float* schedule;
+  const float* norm;
+  float rate, keep1, keep2, new1, new2, epsilon, weight_decay, max_norm;
+  uint32_t seed_low, seed_high;
+};
+static_assert(sizeof(StepTable) + sizeof(StepNumbers) <= 4000, "kernel arguments");
+
+template <typename Table> __device__ __forceinline__ int tensor_of(const Table& table, uint32_t chunk) {
+  int low = 0, high = table.count - 1;
+  while (low < high) {
+    const int middle = (low + high) >> 1;
+    if (table.chunks_end[middle] <= chunk) low = middle + 1;
+    else high = middle;
+  }
+  return low;
+}
+
+// Four elements of any of the three types as they lie in memory: the loads of several can be on
+// their way, whatever their types, before the first is made a float.
+struct Raw {
+  uint32_t w[4];
+};
+typedef uint32_t Words2 __attribute__((ext_vector_type(2)));
+typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
+typedef Words2 Words2At2 __attribute__((aligned(2)));
+typedef Words4 Words4At4 __attribute__((aligned(4)));
+
+__device__ __forceinline__ Raw load_raw(const void* p, int32_t type, int64_t at) {
+  Raw r{};
+  if (type == ILGPU_HIP_F32) {
+    const Words4 v = __builtin_nontemporal_load(
+        reinterpret_cast<const Words4At4*>(static_cast<const float*>(p) + at));
+    r.w[0] = v[0];
+    r.w[1] = v[1];
+    r.w[2] = v[2];
+    r.w[3] = v[3];
+  } else {
+    const Words2 v = __builtin_nontemporal_load(
+        reinterpret_cast<const Words2At2*>(static_cast<const uint16_t*>(p) + at));
+    r.w[0] = v[0];
+    r.w[1] = v[1];
+  }
+  return r;
+}
+// Elements [0, count) of them.
+__device__ __forceinline__ Raw load_some(const void* p, int32_t type, int64_t at, int count) {
+  Raw r{};
+#pragma unroll
+  for (int k = 0; k < kW; ++k) {
+    if (k >= count) break;
+    if (type == ILGPU_HIP_F32) r.w[k] = static_cast<const uint32_t*>(p)[at + k];
+    else r.w[k / 2] |= (uint32_t) static_cast<const uint16_t*>(p)[at + k] << (k % 2 * 16);
+  }
+  return r;
+}
+__device__ __forceinline__ void to_floats(float (&v)[kW], const Raw& r, int32_t type) {
+  if (type == ILGPU_HIP_F32) {
+#pragma unroll
+    for (int k = 0; k < kW; ++k) v[k] = __builtin_bit_cast(float, r.w[k]);
+  } else if (type == ILGPU_HIP_F16) {
+#pragma unroll
+    for (int k = 0; k < kW; ++k)
+      v[k] = (float)__builtin_bit_cast(half_t, (uint16_t)(r.w[k / 2] >> (k % 2 * 16)));
+  } else {
+#pragma unroll
+    for (int k = 0; k < kW; ++k)
+      v[k] = __builtin_bit_cast(float, k % 2 != 0 ? r.w[k / 2] & 0xffff0000u : r.w[k / 2] << 16);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_as(void* p, int64_t at, const float (&v)[kW], int count) {
+  using P = typename Pack<T, kW>::type;
+  T* to = static_cast<T*>(p) + at;
+  if (count >= kW) {
+    typename Pack<T, kW>::vec r;
+#pragma unroll
+    for (int k = 0; k < kW; ++k) r[k] = (T)v[k];
+    __builtin_nontemporal_store(r, reinterpret_cast<P*>(to));
+  } else {
+#pragma unroll
+    for (int k = 0; k < kW; ++k)
+      if (k < count) to[k] = (T)v[k];
+  }
+}
+__device__ __forceinline__ void store_any(void* p, int32_t type, int64_t at, const float (&v)[kW],
+                                          int count) {
+  if (type == ILGPU_HIP_F32) store_as<float>(p, at, v, count);
+  else if (type == ILGPU_HIP_F16) store_as<half_t>(p, at, v, count);
+  else store_as<bfloat_t>(p, at, v, count);
+}
+
+// What is the same for all elements of a step.
+struct Step {
+  float factor, back;                      // of the gradients, one after the other
+  float rate, inverse1, inverse2;          // r; 1 / (1 - beta^t)
+  bool finite;
+};
+__device__ __forceinline__ Step step_of(const StepNumbers& n) {
+  Step s;
+  s.factor = s.back = 1.0f;
+  s.finite = true;
+  if (n.norm != nullptr) {
+    const float norm = n.norm[0];
+    s.finite = fabsf(norm) <= 3.402823466e+38f;
+    if (norm > n.max_norm) {
+      // A factor below the normal numbers has few bits: it is made 2^120 times as large and taken
+      // back behind the product.
+      const bool tiny = n.max_norm / norm < 0x1p-126f;
+      s.factor = tiny ? n.max_norm * 0x1p120f / norm : n.max_norm / norm;
+      s.back = tiny ? 0x1p-120f : 1.0f;
+    }
+  }
+  s.rate = n.schedule != nullptr ? n.rate * n.schedule[0] : n.rate;
+  const double t = (double)n.step[0];
+  s.inverse1 = 1.0f / -expm1f((float)(t * n.log_beta1));
+  s.inverse2 = 1.0f / -expm1f((float)(t * n.log_beta2));
+  return s;
+}
+
+// One element's step from its moments, which become the new ones; returns the new parameter.
+__device__ __forceinline__ float stepped(const StepNumbers& n, const Step& s, float p, float gradient,
+                                         float& m, float& v) {
+  {
+    // (Each rounded by itself: see first_value.)
+#pragma clang fp contract(off)
+    const float g = gradient * s.factor * s.back;
+    m = n.keep1 * m + n.new1 * g;
+    v = n.keep2 * v + n.new2 * (g * g);
+  }
+  const float root = __builtin_amdgcn_sqrtf(v * s.inverse2) + n.epsilon;
+  const float along = m * s.inverse1 * __builtin_amdgcn_rcpf(root);
+  return p - s.rate * fmaf(n.weight_decay, p, along);
+}
+
+// A hash of a 32-bit number: xor-shifts and products with odd numbers (the first bits of the fractions of
+// the roots of 2 and 3), each of which can be undone, so no two numbers share a hash.
+__host__ __device__ __forceinline__ uint32_t mixed(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0x6a09e667u;
+  x ^= x >> 15;
+  x *= 0xbb67ae85u;
+  return x ^ (x >> 16);
+}
+
+// The largest of a wave's lanes, of numbers whose order is that of their bits (none negative; a
+// NaN is larger than all).
+template <int CONTROL, int ROWS = 0xf> __device__ __forceinline__ uint32_t moved_bits(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, ROWS, 0xf, true);
+}
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ float wave_largest(float x) {
+  uint32_t v = __builtin_bit_cast(uint32_t, x);
+  v = larger(v, moved_bits<0x111>(v));       // row_shr:1, 2, 4, 8
+  v = larger(v, moved_bits<0x112>(v));
+  v = larger(v, moved_bits<0x114>(v));
+  v = larger(v, moved_bits<0x118>(v));
+  v = larger(v, moved_bits<0x142, 0xa>(v));  // row_bcast:15 into rows 1 and 3
+  v = larger(v, moved_bits<0x143, 0xc>(v));  // row_bcast:31 into rows 2 and 3
+  return __builtin_bit_cast(float, (uint32_t)__builtin_amdgcn_readlane((int)v, 63));
+}
+__device__ __forceinline__ float larger_bits(float a, float b) {
+  return __builtin_bit_cast(float, larger(__builtin_bit_cast(uint32_t, a),
+                                          __builtin_bit_cast(uint32_t, b)));
+}
+
+// What codes stand for.  Which of two codes a value near a border gets is decided by its last bit, and
+// the next steps go on from there, so the order of roundings is a part of the format: the code's
+// power, the scale's part and their product, each rounded to float32 by itself, the power by the
+// library's function, as a program that computes in whole arrays does it.
+constexpr float kFirstUnit = 1.0f / (127.0f * 127.0f);
+constexpr float kSecondUnit = 1.0f / (255.0f * 255.0f * 255.0f * 255.0f);
+__device__ __forceinline__ float first_value(uint32_t code, float unit) {  // unit: scale * kFirstUnit
+  const float q = (float)(int)code - 128.0f;
+  return q * fabsf(q) * unit;
+}
+// The fourth powers of all codes, in LDS.
+using Powers = float[256];
+__device__ __forceinline__ void fill_powers(Powers& powers) {
+  static_assert(kBlock == 256, "a thread a code");
+  powers[threadIdx.x] = powf((float)threadIdx.x, 4.0f);
+  __syncthreads();
+}
+
+// The code of a value that is not negative: the last whose value is not above it, or the next one
+// if `chance` / 2^16 of the way to it is less than the rest.  The share of the scale is a quotient rounded to
+// float32, everything behind it float64, in which its products with the powers are as good as
+// exact.  (The quotient by the reciprocal and one correction, which is right where the
+// reciprocal is the nearest.)
+constexpr float kSmallest = 0x1p-126f;
+__device__ __forceinline__ float share_of(float value, float scale, float inverse) {
+  const float q = value * inverse;
+  return fmaf(fmaf(-q, scale, value), inverse, q);
+}
+template <int POWER> __device__ __forceinline__ double power_of(float code) {
+  const double square = (double)(code * code);  // (exact in float32)
+  return POWER == 2 ? square : square * square;
+}
+template <int POWER> __device__ __forceinline__ uint32_t code_of(float share, uint32_t chance) {
+  constexpr float kLevels = POWER == 2 ? 127.0f : 255.0f;
+  const double z = (double)share * (POWER == 2 ? 127.0 * 127.0 : 255.0 * 255.0 * 255.0 * 255.0);
+  const double u = (double)chance * 0x1p-16;
+  float low = floorf(POWER == 2 ? __builtin_amdgcn_sqrtf((float)z)
+                                : __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)z)));
+  double below = power_of<POWER>(low), way = z - below;
+  double span = power_of<POWER>(low + 1.0f) - below;
+  if (way < 0.0 || way >= span) {  // (the root's roundings: rare)
+    low += way < 0.0 ? -1.0f : 1.0f;
+    below = power_of<POWER>(low);
+    way = z - below;
+    span = power_of<POWER>(low + 1.0f) - below;
+  }
+  return (uint32_t)fminf(low + (way > u * span ? 1.0f : 0.0f), kLevels);
+}
+
+typedef uint32_t WordAt1 __attribute__((aligned(1)));
+__device__ __forceinline__ uint32_t load_codes(const void* p, int64_t at, int count) {
+  const uint8_t* from = static_cast<const uint8_t*>(p) + at;
+  if (count >= kW) return *reinterpret_cast<const WordAt1*>(from);
+  uint32_t w = 0;
+#pragma unroll
+  for (int k = 0; k < kW; ++k)
+    if (k < count) w |= (uint32_t)from[k] << (8 * k);
+  return w;
+}
+__device__ __forceinline__ void store_codes(void* p, int64_t at, uint32_t w, int count) {
+  uint8_t* to = static_cast<uint8_t*>(p) + at;
+  if (count >= kW) {
+    *reinterpret_cast<WordAt1*>(to) = w;
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < kW; ++k)
+    if (k < count) to[k] = (uint8_t)(w >> (8 * k));
+}
+
+template <bool EIGHT>
+__global__ __launch_bounds__(kBlock) void adamw_kernel(StepTable table, StepNumbers numbers) {
+  __shared__ Powers powers;
+  if (EIGHT) fill_powers(powers);
+  const uint32_t chunks = table.chunks_end[table.count - 1];
+  for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    const int t = tensor_of(table, chunk);
+    const int64_t first = (int64_t)(chunk - (t > 0 ? table.chunks_end[t - 1] : 0)) * kChunk;
+    const int64_t length = table.length[t];
+    const int32_t types = table.types[t];
+    const int32_t type_p = types & 255, type_g = types >> 8 & 255, type_c = types >> 16;
+    Raw p[kTurns], g[kTurns], m[kTurns], v[kTurns];
+    float unit1[kTurns], unit2[kTurns];
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u) {
+      const int64_t at = first + u * kTurn + threadIdx.x * kW, left = length - at;
+      if (left >= kW) {
+        p[u] = load_raw(table.parameter[t], type_p, at);
+        g[u] = load_raw(table.gradient[t], type_g, at);
+        if (!EIGHT) {
+          m[u] = load_raw(table.first[t], ILGPU_HIP_F32, at);
+          v[u] = load_raw(table.second[t], ILGPU_HIP_F32, at);
+        }
+      } else {
+        p[u] = load_some(table.parameter[t], type_p, at, (int)left);
+        g[u] = load_some(table.gradient[t], type_g, at, (int)left);
+        if (!EIGHT) {
+          m[u] = load_some(table.first[t], ILGPU_HIP_F32, at, (int)left);
+          v[u] = load_some(table.second[t], ILGPU_HIP_F32, at, (int)left);
+        }
+      }
+      if (EIGHT) {
+        const int count = left < kW ? (int)left : kW;
+        m[u].w[0] = load_codes(table.first[t], at, count);
+        v[u].w[0] = load_codes(table.second[t], at, count);
+        const int64_t block = (first + u * kTurn) / kMomentBlock + threadIdx.x / kWaveSize;
+        const bool there = block * kMomentBlock < length;
+        unit1[u] = there ? table.first_scale[t][block] * kFirstUnit : 0.0f;
+        unit2[u] = there ? table.second_scale[t][block] * kSecondUnit : 0.0f;
+      }
+    }
+    const Step s = step_of(numbers);
+    if (!s.finite) return;
+    uint32_t key = 0;
+    if (EIGHT) {
+      key = mixed(numbers.seed_low + (uint32_t)numbers.step[0] * 0x3c6ef373u);
+      key = mixed(key + numbers.seed_high + table.number[t] * 0x9e3779b9u);
+    }
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u) {
+      const int64_t at = first + u * kTurn + threadIdx.x * kW;
+      const int count = length - at < kW ? (int)(length - at) : kW;
+      if (!EIGHT && count <= 0) break;
+      float parameter[kW], gradient[kW], moment1[kW], moment2[kW];
+      to_floats(parameter, p[u], type_p);
+      to_floats(gradient, g[u], type_g);
+#pragma unroll
+      for (int k = 0; k < kW; ++k) {
+        if (EIGHT) {
+          moment1[k] = first_value(m[u].w[0] >> (8 * k) & 255u, unit1[u]);
+          moment2[k] = powers[v[u].w[0] >> (8 * k) & 255u] * unit2[u];
+        } else {
+          moment1[k] = __builtin_bit_cast(float, m[u].w[k]);
+          moment2[k] = __builtin_bit_cast(float, v[u].w[k]);
+        }
+        parameter[k] = stepped(numbers, s, parameter[k], gradient[k], moment1[k], moment2[k]);
+      }
+      if (count > 0) {
+        store_any(table.parameter[t], type_p, at, parameter, count);
+        if (table.copy[t] != nullptr) store_any(table.copy[t], type_c, at, parameter, count);
+      }
+      if (!EIGHT) {
+        store_as<float>(table.first[t], at, moment1, count);
+        store_as<float>(table.second[t], at, moment2, count);
+        continue;
+      }
+      float largest1 = 0.0f, largest2 = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kW; ++k) {
+        if (k < count) {
+          largest1 = larger_bits(largest1, fabsf(moment1[k]));
+          largest2 = larger_bits(largest2, fabsf(moment2[k]));
+        }
+      }
+      const float scale1 = wave_largest(largest1), scale2 = wave_largest(largest2);
+      const float inverse1 = 1.0f / scale1, inverse2 = 1.0f / scale2;
+      uint32_t codes1 = 0, codes2 = 0;
+#pragma unroll
+      for (int k = 0; k < kW; ++k) {
+        const uint32_t chance = mixed((uint32_t)(at + k) * 0x9e3779b9u + key);
+        const float share1 = share_of(fabsf(moment1[k]), scale1, inverse1);
+        const float share2 = share_of(moment2[k], scale2, inverse2);
+        const uint32_t q = scale1 < kSmallest ? 0u : code_of<2>(share1, chance & 0xffffu);
+        codes1 |= (moment1[k] < 0.0f ? 128u - q : 128u + q) << (8 * k);
+        codes2 |= (scale2 < kSmallest ? 0u : code_of<4>(share2, chance >> 16)) << (8 * k);
+      }
+      if (count > 0) {
+        store_codes(table.first[t], at, codes1, count);
+        store_codes(table.second[t], at, codes2, count);
+      }
+      const int64_t block = (first + u * kTurn) / kMomentBlock + threadIdx.x / kWaveSize;
+      if ((threadIdx.x & (kWaveSize - 1)) == 0 && block * kMomentBlock < length) {
+        table.first_scale[t][block] = scale1 < kSmallest ? 0.0f : scale1;
+        table.second_scale[t][block] = scale2 < kSmallest ? 0.0f : scale2;
+      }
+    }
+  }
+}
+
+constexpr int kReadTensors = 90;
+struct ReadTable {
+  const void* codes[kReadTensors];
+  const float* scales[kReadTensors];
+  void* target[kReadTensors];
+  int64_t length[kReadTensors];
+  uint32_t chunks_end[kReadTensors];
+  int32_t type[kReadTensors];
+  int32_t count;
+};
+static_assert(sizeof(ReadTable) <= 4000, "kernel arguments");
+
+template <bool SECOND>
+__global__ __launch_bounds__(kBlock) void adamw_moments_kernel(ReadTable table) {
+  __shared__ Powers powers;
+  if (SECOND) fill_powers(powers);
+  const uint32_t chunks = table.chunks_end[table.count - 1];
+  for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+    const int t = tensor_of(table, chunk);
+    const int64_t first = (int64_t)(chunk - (t > 0 ? table.chunks_end[t - 1] : 0)) * kChunk;
+    uint32_t codes[kTurns];
+    float unit[kTurns];
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u) {
+      const int64_t at = first + u * kTurn + threadIdx.x * kW, left = table.length[t] - at;
+      codes[u] = load_codes(table.codes[t], at, left < kW ? (int)left : kW);
+      unit[u] = left > 0 ? table.scales[t][at / kMomentBlock] * (SECOND ? kSecondUnit : kFirstUnit)
+                         : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u) {
+      const int64_t at = first + u * kTurn + threadIdx.x * kW, left = table.length[t] - at;
+      if (left <= 0) break;
+      float v[kW];
+#pragma unroll
+      for (int k = 0; k < kW; ++k) {
+        const uint32_t code = codes[u] >> (8 * k) & 255u;
+        v[k] = SECOND ? powers[code] * unit[u] : first_value(code, unit[u]);
+      }
+      store_any(table.target[t], table.type[t], at, v, left < kW ? (int)left : kW);
+    }
+  }
+}
+
+}  // namespace
+
+int32_t launch_adamw(hipStream_t stream, const AdamwArgs& a) {
+  const ilgpu_hip_adamw_options& o = a.options;
+  StepNumbers numbers;
+  numbers.log_beta1 = log(o.beta1);
+  numbers.log_beta2 = log(o.beta2);
+  numbers.step = a.step;
+  numbers.schedule = a.schedule;
+  numbers.norm = a.norm;
+  numbers.rate = (float)o.rate;
+  numbers.keep1 = (float)o.beta1;
+  numbers.keep2 = (float)o.beta2;
+  numbers.new1 = (float)(1.0 - o.beta1);
+  numbers.new2 = (float)(1.0 - o.beta2);
+  numbers.epsilon = (float)o.epsilon;
+  numbers.weight_decay = (float)o.weight_decay;
+  numbers.max_norm = (float)o.max_norm;
+  numbers.seed_low = (uint32_t)(uint64_t)o.seed;
+  numbers.seed_high = (uint32_t)((uint64_t)o.seed >> 32);
+  const bool eight = a.first_scales != nullptr;
+  StepTable table;
+  for (int64_t next = 0; next < a.count;) {
+    int used = 0;
+    int64_t chunks = 0;
+    for (; next < a.count && used < kTensors; ++next) {
+      const int64_t length = a.parameters[next].length;
+      if (length == 0) continue;
+      chunks += div_up(length, kChunk);  // (at most 2^28 and one per tensor)
+      table.parameter[used] = a.parameters[next].data;
+      table.gradient[used] = a.gradients[next].data;
+      table.first[used] = a.first[next].data;
+      table.second[used] = a.second[next].data;
+      table.first_scale[used] = eight ? static_cast<float*>(a.first_scales[next].data) : nullptr;
+      table.second_scale[used] = eight ? static_cast<float*>(a.second_scales[next].data) : nullptr;
+      table.copy[used] = a.copies != nullptr ? a.copies[next].data : nullptr;
+      table.length[used] = length;
+      table.chunks_end[used] = (uint32_t)chunks;
+      table.number[used] = (uint32_t)next;
+      table.types[used] = a.parameters[next].type | a.gradients[next].type << 8 |
+                          (a.copies != nullptr ? a.copies[next].type << 16 : 0);
+      ++used;
+    }
+    if (used == 0) break;
+    table.count = used;
+    {
+      ProfileScope scope(stream, eight ? "adamw_8bit" : "adamw");
+      const dim3 grid((unsigned)(chunks < kMaxBlocks ? chunks : kMaxBlocks));
+      if (eight) hipLaunchKernelGGL((adamw_kernel<true>), grid, dim3(kBlock), 0, stream, table, numbers);
+      else hipLaunchKernelGGL((adamw_kernel<false>), grid, dim3(kBlock), 0, stream, table, numbers);
+    }
+    ILGPU_HIP_CHECK(hipGetLastError());
+  }
+  return ILGPU_HIP_SUCCESS;
+}
+
+int32_t launch_adamw_moments(hipStream_t stream, const ilgpu_hip_tensor* codes,
+                             const ilgpu_hip_tensor* scales, const ilgpu_hip_tensor* targets,
+                             int64_t count, bool second) {
+  ReadTable table;
+  for (int64_t next = 0; next < count;) {
+    int used = 0;
+    int64_t chunks = 0;
+    for (; next < count && used < kReadTensors; ++next) {
+      if (codes[next].length == 0) continue;
+      chunks += div_up(codes[next].length, kChunk);
+      table.codes[used] = codes[next].data;
+      table.scales[used] = static_cast<const float*>(scales[next].data);
+      table.target[used] = targets[next].data;
+      table.length[used] = codes[next].length;
+      table.chunks_end[used] = (uint32_t)chunks;
+      table.type[used] = targets[next].type;
+      ++used;
+    }
+    if (used == 0) break;
+    table.count = used;
+    {
+      ProfileScope scope(stream, "adamw_moments");
+      const dim3 grid((unsigned)(chunks < kMaxBlocks ? chunks : kMaxBlocks));
+      if (second)
+        hipLaunchKernelGGL((adamw_moments_kernel<true>), grid, dim3(kBlock), 0, stream, table);
+      else
+        hipLaunchKernelGGL((adamw_moments_kernel<false>), grid, dim3(kBlock), 0, stream, table);
+    }
+    ILGPU_HIP_CHECK(hipGetLastError());
+  }
+  return ILGPU_HIP_SUCCESS;
+}
+
+}  // namespace ilgpu_hip

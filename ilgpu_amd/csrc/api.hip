@@ -787,4 +787,334 @@ int32_t ilgpu_hip_clip_gradients(ilgpu_hip_stream_t stream,
                                *max_norm);
 }
 
+/* ---- gated recurrence ------------------------------------------------------------ */
+
+static int32_t check_sequences(const void* offsets, int32_t offset_type, int64_t sequences,
+                               int64_t rows) {
+  if (sequences < 0) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  if (sequences >= INT32_MAX) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  if (offsets == nullptr)
+    return (sequences > 0 ? rows % sequences : rows) == 0 ? ILGPU_HIP_SUCCESS
+                                                          : ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  return check_tokens(offsets, sequences + 1, offset_type);
+}
+
+// A temp that may be missing where none is needed.
+static int32_t check_optional_temp(const void* temp, int64_t temp_bytes, int64_t required) {
+  return required == 0 ? ILGPU_HIP_SUCCESS : check_temp(temp, temp_bytes, required);
+}
+
+int32_t ilgpu_hip_gated_recurrence_temp_bytes(int64_t rows, int64_t channels,
+                                              int64_t* temp_bytes) {
+  if (temp_bytes == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (rows < 0 || channels < 1) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  if (rows > INT32_MAX || channels > INT32_MAX) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  *temp_bytes = gated_recurrence_temp_bytes(rows, channels);
+  return ILGPU_HIP_SUCCESS;
+}
+
+static int32_t check_recurrence(GatedRecurrenceArgs& a, int64_t temp_bytes) {
+  const int eb = operator_elem_size(a.type);
+  if (eb < 0) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  if (a.decay != ILGPU_HIP_DECAY_SIGMOID && a.decay != ILGPU_HIP_DECAY_EXPONENTIAL)
+    return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  int32_t rc = check_matrix(a.gate, a.rows, a.channels, a.gate_stride, eb, false);
+  if (rc == ILGPU_HIP_SUCCESS) rc = check_matrix(a.in, a.rows, a.channels, a.in_stride, eb, false);
+  if (rc == ILGPU_HIP_SUCCESS)
+    rc = check_matrix(a.out, a.rows, a.channels, a.out_stride, eb, !a.backwards);
+  if (rc == ILGPU_HIP_SUCCESS)
+    rc = check_sequences(a.offsets, a.offset_type, a.sequences, a.rows);
+  if (rc == ILGPU_HIP_SUCCESS && a.initial != nullptr)
+    rc = check_matrix(a.initial, a.sequences, a.channels, a.initial_stride, 4, false);
+  if (rc == ILGPU_HIP_SUCCESS && a.final_state != nullptr)
+    rc = check_matrix(a.final_state, a.sequences, a.channels, a.final_stride, 4, true);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  const bool step = !a.backwards && a.offsets == nullptr && a.sequences == a.rows;
+  return check_optional_temp(a.temp, temp_bytes,
+                             step ? 0 : gated_recurrence_temp_bytes(a.rows, a.channels));
+}
+
+int32_t ilgpu_hip_gated_recurrence(
+    ilgpu_hip_stream_t stream, const void* gate, int64_t gate_stride, const void* in,
+    int64_t in_stride, int64_t rows, int64_t channels, int32_t type, int32_t decay,
+    int32_t complement, const void* offsets, int32_t offset_type, int64_t sequences,
+    const float* initial, int64_t initial_stride, void* out, int64_t out_stride,
+    float* final_state, int64_t final_stride, void* temp, int64_t temp_bytes) {
+  GatedRecurrenceArgs a{};
+  a.gate = gate;
+  a.gate_stride = gate_stride;
+  a.in = in;
+  a.in_stride = in_stride;
+  a.rows = rows;
+  a.channels = channels;
+  a.type = type;
+  a.decay = decay;
+  a.complement = complement != 0 ? 1 : 0;
+  a.offsets = offsets;
+  a.offset_type = offset_type;
+  a.sequences = sequences;
+  a.initial = initial;
+  a.initial_stride = initial_stride;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.final_state = final_state;
+  a.final_stride = final_stride;
+  a.temp = temp;
+  const int32_t rc = check_recurrence(a, temp_bytes);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  return launch_gated_recurrence(static_cast<hipStream_t>(stream), a);
+}
+
+int32_t ilgpu_hip_gated_recurrence_gradient(
+    ilgpu_hip_stream_t stream, const void* grad_out, int64_t grad_out_stride, const void* gate,
+    int64_t gate_stride, const void* in, int64_t in_stride, const void* out, int64_t out_stride,
+    int64_t rows, int64_t channels, int32_t type, int32_t decay, int32_t complement,
+    const void* offsets, int32_t offset_type, int64_t sequences, const float* initial,
+    int64_t initial_stride, const float* grad_final, int64_t grad_final_stride, void* grad_gate,
+    int64_t grad_gate_stride, void* grad_in, int64_t grad_in_stride, float* grad_initial,
+    int64_t grad_initial_stride, void* temp, int64_t temp_bytes) {
+  GatedRecurrenceArgs a{};
+  a.gate = gate;
+  a.gate_stride = gate_stride;
+  a.in = in;
+  a.in_stride = in_stride;
+  a.rows = rows;
+  a.channels = channels;
+  a.type = type;
+  a.decay = decay;
+  a.complement = complement != 0 ? 1 : 0;
+  a.offsets = offsets;
+  a.offset_type = offset_type;
+  a.sequences = sequences;
+  a.initial = initial;
+  a.initial_stride = initial_stride;
+  a.out = const_cast<void*>(out);  // read only
+  a.out_stride = out_stride;
+  a.backwards = true;
+  a.grad_out = grad_out;
+  a.grad_out_stride = grad_out_stride;
+  a.grad_final = grad_final;
+  a.grad_final_stride = grad_final_stride;
+  a.grad_gate = grad_gate;
+  a.grad_gate_stride = grad_gate_stride;
+  a.grad_in = grad_in;
+  a.grad_in_stride = grad_in_stride;
+  a.grad_initial = grad_initial;
+  a.grad_initial_stride = grad_initial_stride;
+  a.temp = temp;
+  int32_t rc = check_recurrence(a, temp_bytes);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  const int eb = operator_elem_size(type);
+  rc = check_matrix(grad_out, rows, channels, grad_out_stride, eb, false);
+  if (rc == ILGPU_HIP_SUCCESS && grad_final != nullptr)
+    rc = check_matrix(grad_final, sequences, channels, grad_final_stride, 4, false);
+  if (rc == ILGPU_HIP_SUCCESS && grad_gate != nullptr)
+    rc = check_matrix(grad_gate, rows, channels, grad_gate_stride, eb, true);
+  if (rc == ILGPU_HIP_SUCCESS && grad_in != nullptr)
+    rc = check_matrix(grad_in, rows, channels, grad_in_stride, eb, true);
+  if (rc == ILGPU_HIP_SUCCESS && grad_initial != nullptr)
+    rc = check_matrix(grad_initial, sequences, channels, grad_initial_stride, 4, true);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  if (rows > 0 && grad_gate == nullptr && grad_in == nullptr && grad_initial == nullptr)
+    return ILGPU_HIP_ERROR_NULL_VIEW;
+  return launch_gated_recurrence(static_cast<hipStream_t>(stream), a);
+}
+
+/* ---- residual norm ----------------------------------------------------------------- */
+
+// The types of the matrices, of the residual stream and of the weights.
+static int32_t check_residual_types(int32_t type, int32_t residual_type, int32_t weight_type) {
+  const int32_t rc = check_norm_types(type, residual_type);
+  return rc != ILGPU_HIP_SUCCESS ? rc : check_norm_types(type, weight_type);
+}
+static int32_t check_gate(const void* gate, int64_t rows, int64_t columns, int64_t stride,
+                          int elem_bytes, int32_t kind) {
+  if (gate == nullptr) return ILGPU_HIP_SUCCESS;
+  if (kind != ILGPU_HIP_GATE_SIGMOID && kind != ILGPU_HIP_GATE_SILU)
+    return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  return check_matrix(gate, rows, columns, stride, elem_bytes, false);
+}
+
+int32_t ilgpu_hip_residual_norm(
+    ilgpu_hip_stream_t stream, const void* in, int64_t in_stride, int64_t rows, int64_t columns,
+    int32_t type, int32_t input_norm, const void* input_weight, const void* gate,
+    int64_t gate_stride, int32_t gate_kind, const void* residual, int64_t residual_stride,
+    int32_t residual_type, const float* scale, const void* weight, int32_t weight_type,
+    const float* epsilon, void* total, int64_t total_stride, void* out, int64_t out_stride,
+    float* input_rstd, float* rstd) {
+  int32_t rc = check_residual_types(type, residual_type, weight_type);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  const int eb = operator_elem_size(type), rb = operator_elem_size(residual_type),
+            wb = operator_elem_size(weight_type);
+  if (epsilon == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  rc = check_matrix(in, rows, columns, in_stride, eb, false);
+  if (rc == ILGPU_HIP_SUCCESS) rc = check_gate(gate, rows, columns, gate_stride, eb, gate_kind);
+  if (rc == ILGPU_HIP_SUCCESS && residual != nullptr)
+    rc = check_matrix(residual, rows, columns, residual_stride, rb, false);
+  if (rc == ILGPU_HIP_SUCCESS && total != nullptr)
+    rc = check_matrix(total, rows, columns, total_stride, rb, true);
+  if (rc == ILGPU_HIP_SUCCESS && out != nullptr)
+    rc = check_matrix(out, rows, columns, out_stride, eb, true);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  if (rows > 0 && total == nullptr && out == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (!(*epsilon >= 0.0f && *epsilon <= 3.402823466e+38f)) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  if (!aligned_to(weight, wb) || !aligned_to(input_weight, wb) || !aligned_to(input_rstd, 4) ||
+      !aligned_to(rstd, 4))
+    return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  const ResidualNormArgs a{in, in_stride, rows, columns, type, input_norm != 0 ? 1 : 0,
+                           input_norm != 0 ? input_weight : nullptr, gate, gate_stride, gate_kind,
+                           residual, residual_stride, residual_type,
+                           scale != nullptr ? *scale : 1.0f, weight, weight_type, *epsilon, total,
+                           total_stride, out, out_stride, input_rstd, rstd};
+  return launch_residual_norm(static_cast<hipStream_t>(stream), a);
+}
+
+int32_t ilgpu_hip_residual_norm_gradient_temp_bytes(int64_t rows, int64_t columns,
+                                                    int64_t* temp_bytes) {
+  if (temp_bytes == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (rows < 0 || columns < 1) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  if (rows > INT32_MAX || columns > INT32_MAX) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  *temp_bytes = residual_norm_gradient_temp_bytes(rows, columns);
+  return ILGPU_HIP_SUCCESS;
+}
+
+int32_t ilgpu_hip_residual_norm_gradient(
+    ilgpu_hip_stream_t stream, const void* grad_out, int64_t grad_out_stride,
+    const void* grad_total, int64_t grad_total_stride, const void* in, int64_t in_stride,
+    int64_t rows, int64_t columns, int32_t type, int32_t input_norm, const void* input_weight,
+    const float* input_rstd, const void* gate, int64_t gate_stride, int32_t gate_kind,
+    const void* total, int64_t total_stride, int32_t residual_type, const float* scale,
+    const void* weight, int32_t weight_type, const float* rstd, void* grad_in,
+    int64_t grad_in_stride, void* grad_gate, int64_t grad_gate_stride, void* grad_residual,
+    int64_t grad_residual_stride, void* grad_input_weight, void* grad_weight, int32_t accumulate,
+    void* temp, int64_t temp_bytes) {
+  int32_t rc = check_residual_types(type, residual_type, weight_type);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  const int eb = operator_elem_size(type), rb = operator_elem_size(residual_type),
+            wb = operator_elem_size(weight_type);
+  rc = check_matrix(in, rows, columns, in_stride, eb, false);
+  if (rc == ILGPU_HIP_SUCCESS) rc = check_gate(gate, rows, columns, gate_stride, eb, gate_kind);
+  if (rc == ILGPU_HIP_SUCCESS && grad_out != nullptr) {
+    rc = check_matrix(grad_out, rows, columns, grad_out_stride, eb, false);
+    if (rc == ILGPU_HIP_SUCCESS) rc = check_matrix(total, rows, columns, total_stride, rb, false);
+    if (rc == ILGPU_HIP_SUCCESS && rows > 0 && rstd == nullptr) rc = ILGPU_HIP_ERROR_NULL_VIEW;
+  }
+  if (rc == ILGPU_HIP_SUCCESS && grad_total != nullptr)
+    rc = check_matrix(grad_total, rows, columns, grad_total_stride, rb, false);
+  if (rc == ILGPU_HIP_SUCCESS && grad_in != nullptr)
+    rc = check_matrix(grad_in, rows, columns, grad_in_stride, eb, true);
+  if (rc == ILGPU_HIP_SUCCESS && grad_gate != nullptr)
+    rc = check_matrix(grad_gate, rows, columns, grad_gate_stride, eb, true);
+  if (rc == ILGPU_HIP_SUCCESS && grad_residual != nullptr)
+    rc = check_matrix(grad_residual, rows, columns, grad_residual_stride, rb, true);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  if (rows > 0) {
+    if (grad_out == nullptr && grad_total == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+    if (input_norm != 0 && input_rstd == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+    // What was not a part of the forward call has no gradient.
+    if (grad_gate != nullptr && gate == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+    if (grad_weight != nullptr && grad_out == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+    if (grad_in == nullptr && grad_gate == nullptr && grad_residual == nullptr &&
+        grad_input_weight == nullptr && grad_weight == nullptr)
+      return ILGPU_HIP_ERROR_NULL_VIEW;
+  }
+  if (grad_input_weight != nullptr && input_norm == 0) return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (!aligned_to(weight, wb) || !aligned_to(input_weight, wb) || !aligned_to(grad_weight, wb) ||
+      !aligned_to(grad_input_weight, wb) || !aligned_to(input_rstd, 4) || !aligned_to(rstd, 4))
+    return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  rc = check_temp(temp, temp_bytes, residual_norm_gradient_temp_bytes(rows, columns));
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  const ResidualNormGradientArgs a{grad_out, grad_out_stride, grad_total, grad_total_stride, in,
+                                   in_stride, rows, columns, type, input_norm != 0 ? 1 : 0,
+                                   input_norm != 0 ? input_weight : nullptr, input_rstd, gate,
+                                   gate_stride, gate_kind, total, total_stride, residual_type,
+                                   scale != nullptr ? *scale : 1.0f, weight, weight_type, rstd,
+                                   grad_in, grad_in_stride, grad_gate, grad_gate_stride,
+                                   grad_residual, grad_residual_stride, grad_input_weight,
+                                   grad_weight, accumulate != 0 ? 1 : 0};
+  return launch_residual_norm_gradient(static_cast<hipStream_t>(stream), a, temp);
+}
+
+/* ---- AdamW ---------------------------------------------------------------------------- */
+
+// A list whose tensors are as long as those of `like`, or have an element for each `per` of
+// theirs, and of one of the operators' types, or of `type`.
+static int32_t check_tensors_like(const ilgpu_hip_tensor* tensors, const ilgpu_hip_tensor* like,
+                                  int64_t count, int32_t type, int64_t per) {
+  if (count > 0 && tensors == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  for (int64_t k = 0; k < count; ++k) {
+    const int eb = type < 0 ? operator_elem_size(tensors[k].type)
+                            : tensors[k].type == type ? elem_size(type) : -1;
+    if (eb < 0) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+    if (tensors[k].length != div_up(like[k].length, per)) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+    if (tensors[k].length == 0) continue;
+    if (tensors[k].data == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+    if (!aligned_to(tensors[k].data, eb)) return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  }
+  return ILGPU_HIP_SUCCESS;
+}
+// Three lists of a moment in 8 bits, or none.
+static int32_t check_moments(const ilgpu_hip_tensor* codes, const ilgpu_hip_tensor* scales,
+                             const ilgpu_hip_tensor* targets, int64_t count) {
+  if (codes == nullptr && scales == nullptr && targets == nullptr) return ILGPU_HIP_SUCCESS;
+  int32_t rc = check_tensors(targets, count);
+  if (rc == ILGPU_HIP_SUCCESS) rc = check_tensors_like(codes, targets, count, ILGPU_HIP_U8, 1);
+  if (rc == ILGPU_HIP_SUCCESS)
+    rc = check_tensors_like(scales, targets, count, ILGPU_HIP_F32, kMomentBlock);
+  return rc;
+}
+
+int32_t ilgpu_hip_adamw(ilgpu_hip_stream_t stream, const ilgpu_hip_tensor* parameters,
+                        const ilgpu_hip_tensor* gradients, const ilgpu_hip_tensor* first,
+                        const ilgpu_hip_tensor* second, const ilgpu_hip_tensor* first_scales,
+                        const ilgpu_hip_tensor* second_scales, const ilgpu_hip_tensor* copies,
+                        int64_t count, const ilgpu_hip_adamw_options* options,
+                        const int64_t* step, const float* schedule, const float* norm) {
+  int32_t rc = check_tensors(parameters, count);
+  if (rc == ILGPU_HIP_SUCCESS) rc = check_tensors_like(gradients, parameters, count, -1, 1);
+  if (rc == ILGPU_HIP_SUCCESS && copies != nullptr)
+    rc = check_tensors_like(copies, parameters, count, -1, 1);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  if ((first_scales == nullptr) != (second_scales == nullptr)) return ILGPU_HIP_ERROR_NULL_VIEW;
+  const int32_t moments = first_scales != nullptr ? ILGPU_HIP_U8 : ILGPU_HIP_F32;
+  rc = check_tensors_like(first, parameters, count, moments, 1);
+  if (rc == ILGPU_HIP_SUCCESS) rc = check_tensors_like(second, parameters, count, moments, 1);
+  if (rc == ILGPU_HIP_SUCCESS && first_scales != nullptr)
+    rc = check_tensors_like(first_scales, parameters, count, ILGPU_HIP_F32, kMomentBlock);
+  if (rc == ILGPU_HIP_SUCCESS && second_scales != nullptr)
+    rc = check_tensors_like(second_scales, parameters, count, ILGPU_HIP_F32, kMomentBlock);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  if (options == nullptr || step == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  if (!aligned_to(step, 8) || !aligned_to(schedule, 4) || !aligned_to(norm, 4))
+    return ILGPU_HIP_ERROR_NOT_SUPPORTED;
+  const ilgpu_hip_adamw_options& o = *options;
+  constexpr double kLargest = 3.402823466e+38;
+  const auto beta = [](double b) { return b >= 0.0 && b < 1.0 && (float)b < 1.0f; };
+  if (!(o.rate >= 0.0 && o.rate <= kLargest) || !beta(o.beta1) || !beta(o.beta2) ||
+      !((float)o.epsilon >= 0x1p-126f && o.epsilon <= kLargest) ||
+      !(o.weight_decay >= 0.0 && o.weight_decay <= kLargest) || !(o.max_norm >= 0.0))
+    return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  const AdamwArgs a{parameters, gradients, first, second, first_scales, second_scales, copies,
+                    count, o, step, schedule, norm};
+  return launch_adamw(static_cast<hipStream_t>(stream), a);
+}
+
+int32_t ilgpu_hip_adamw_moments(ilgpu_hip_stream_t stream, const ilgpu_hip_tensor* first,
+                                const ilgpu_hip_tensor* first_scales,
+                                const ilgpu_hip_tensor* first_targets,
+                                const ilgpu_hip_tensor* second,
+                                const ilgpu_hip_tensor* second_scales,
+                                const ilgpu_hip_tensor* second_targets, int64_t count) {
+  if (count < 0) return ILGPU_HIP_ERROR_OUT_OF_RANGE;
+  int32_t rc = check_moments(first, first_scales, first_targets, count);
+  if (rc == ILGPU_HIP_SUCCESS) rc = check_moments(second, second_scales, second_targets, count);
+  if (rc != ILGPU_HIP_SUCCESS) return rc;
+  if (count > 0 && first == nullptr && second == nullptr) return ILGPU_HIP_ERROR_NULL_VIEW;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (first != nullptr) rc = launch_adamw_moments(s, first, first_scales, first_targets, count, false);
+  if (rc == ILGPU_HIP_SUCCESS && second != nullptr)
+    rc = launch_adamw_moments(s, second, second_scales, second_targets, count, true);
+  return rc;
+}
+
 }  // extern "C"

@@ -1,0 +1,564 @@
+// Gated linear recurrence over packed sequences, and its gradients.
+//
+// h = a h + b is a scan of affine maps, one scan a channel.  A tile is 64 channels of some
+// hundred rows: a thread folds its rows' maps into one, (A, B) with h -> A h + B, the maps of
+// the row groups are scanned through LDS, and the state in front of the tile comes by a look-back over the
+// tiles before it.  Rows are read once, stay in registers, and are written once.
+//
+// The look-back applies maps to a state, one after the other, and never joins two of them: whether
+// it begins at the state that the tile before it has published or at one some tiles further back, it goes
+// through the same operations on the same numbers, so every run gives the same bits.
+//
+// A sequence's first row is a reset: its map forgets what comes in, whatever that is (a NaN
+// times 0 would still be one).  A reset is marked by A = -0, which no product of
+// decays gives.  Backwards, with P[t] = a[t] G[t] for the state, G[t] = grad_out[t] + P[t+1] is the same scan
+// from the last row to the first; what is said of first rows holds of last ones.
+#include "gates.hpp"
+#include "operators.hpp"
+
+namespace ilgpu_hip {
+
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kWaves = kBlock / kWaveSize;
+constexpr int kTileChannels = kWaveSize;  // a wave's lanes walk back, a channel each
+constexpr int kWindow = 8;                // tiles that a look-back asks at a time
+constexpr uint32_t kMostPolls = 1 << 24;  // of a look-back: many seconds
+constexpr int64_t kMostBlocks = 1 << 22;  // of a launch
+
+// Rows of a thread; row groups of a tile; rows of a tile.
+template <int W> constexpr int groups_of() { return kBlock * W / kTileChannels; }
+#ifndef ILGPU_HIP_RECURRENCE_ROWS
+#define ILGPU_HIP_RECURRENCE_ROWS 8
+#endif
+#ifndef ILGPU_HIP_RECURRENCE_BACK_ROWS
+#define ILGPU_HIP_RECURRENCE_BACK_ROWS 4
+#endif
+constexpr int kRows = ILGPU_HIP_RECURRENCE_ROWS, kBackRows = ILGPU_HIP_RECURRENCE_BACK_ROWS;
+constexpr int kFewestRows = kRows < kBackRows ? kRows : kBackRows;
+
+constexpr int64_t kTicketBytes = 128;  // of a column of tiles: a line of its own
+constexpr int64_t kStateBytes = kTileChannels * 16;
+
+struct Map {
+  float a, b;
+};
+__device__ __forceinline__ bool is_reset(float a) {
+  return __builtin_bit_cast(uint32_t, a) == 0x80000000u;
+}
+// The map that does `first`, then `then`.
+__device__ __forceinline__ Map behind(Map then, Map first) {
+  Map m;
+  m.a = is_reset(then.a) || is_reset(first.a) ? -0.0f : then.a * first.a;
+  m.b = is_reset(then.a) ? then.b : fmaf(then.a, first.b, then.b);
+  return m;
+}
+__device__ __forceinline__ float apply(Map m, float h) {
+  return is_reset(m.a) ? m.b : fmaf(m.a, h, m.b);
+}
+
+// a and 1 - a of a gate, each to some units in its last place.
+template <bool SIGMOID> __device__ __forceinline__ void decay_of(float gate, float& a, float& left) {
+  if constexpr (SIGMOID) {
+    logistic(gate, a, left);
+  } else {
+    a = exp_of(gate);
+    // Near 0, where the difference has lost its bits, 1 - exp by its series (off by 2e-8 at most).
+    const float series =
+        -gate * fmaf(gate * (1.0f / 2), fmaf(gate * (1.0f / 3), fmaf(gate * (1.0f / 4), fmaf(gate * (1.0f / 5), fmaf(
+        gate * (1.0f / 6), fmaf(gate, 1.0f / 7, 1.0f), 1.0f), 1.0f), 1.0f), 1.0f), 1.0f);
+    left = fabsf(gate) < 0.35f ? series : 1.0f - a;
+  }
+}
+
+struct Sequences {
+  const void* offsets;   // nullptr: `count` of `length` rows each
+  int32_t wide;          // offsets are int64
+  int64_t count;
+  uint32_t length;
+  __device__ __forceinline__ int64_t offset(int64_t i) const {
+    return wide ? static_cast<const int64_t*>(offsets)[i]
+                : (int64_t) static_cast<const int32_t*>(offsets)[i];
+  }
+};
+
+// The sequence that begins, and that ends, in each row of a tile, or -1; called by the whole
+// block, ends with a barrier.  Rows [*from, *to) belong to sequences.
+template <int ROWS>
+__device__ __forceinline__ void mark_rows(const Sequences& s, int64_t first, int64_t rows,
+                                          int32_t* begins, int32_t* ends, int64_t* from,
+                                          int64_t* to) {
+  if (s.offsets == nullptr) {
+    for (int i = threadIdx.x; i < ROWS; i += kBlock) {
+      const uint32_t row = (uint32_t)first + i;
+      const bool in = row < (uint64_t)rows;
+      begins[i] = in && row % s.length == 0 ? (int32_t)(row / s.length) : -1;
+      ends[i] = in && (row + 1) % s.length == 0 ? (int32_t)(row / s.length) : -1;
+    }
+    *from = 0;
+    *to = rows;
+    __syncthreads();
+    return;
+  }
+  for (int i = threadIdx.x; i < ROWS; i += kBlock) begins[i] = ends[i] = -1;
+  // The first offset that is not below `first` lies in [at, at + left].
+  int64_t at = 0, left = s.count + 1;
+  while (left > kBlock) {
+    const int64_t step = (left + kBlock - 1) / kBlock, i = at + threadIdx.x * step;
+    const int below = __syncthreads_count(i < at + left && s.offset(i) < first);
+    const int64_t end = at + left;
+    if (below > 0) at += (below - 1) * step;
+    left = step < end - at ? step : end - at;
+  }
+  __syncthreads();
+  for (int64_t j = at + threadIdx.x; j <= s.count; j += kBlock) {
+    const int64_t o = s.offset(j), row = o - first;
+    if (row > ROWS) break;
+    if (row >= 0 && row < ROWS && j < s.count && s.offset(j + 1) > o) begins[row] = (int32_t)j;
+    if (row > 0 && j > 0 && s.offset(j - 1) < o) ends[row - 1] = (int32_t)(j - 1);
+  }
+  const int64_t low = s.offset(0), high = s.offset(s.count);
+  *from = low > 0 ? low : 0;
+  *to = high < rows ? high : rows;
+  __syncthreads();
+}
+
+struct Scan {
+  const void *gate, *in, *grad_out, *states;  // grad_out and states: backwards
+  int64_t gate_stride, in_stride, grad_out_stride, states_stride;
+  int64_t rows, channels;
+  int32_t complement;
+  Sequences sequences;
+  const float* initial;     // nullptr: zeros
+  const float* grad_final;  // backwards
+  int64_t initial_stride, grad_final_stride;
+  void *out, *grad_in;      // backwards: out is the gate's gradient; each may be nullptr
+  int64_t out_stride, grad_in_stride;
+  float* last;              // the state that a sequence leaves; may be nullptr
+  int64_t last_stride;
+  uint32_t* tickets;        // nullptr: one tile of rows
+  uint64_t* words;
+  int64_t tiles;            // of rows
+  uint32_t columns_of_tiles;
+  int64_t first_block;      // of this launch
+};
+
+// What a tile leaves for those behind it, two words a channel: {B, 1} and {A, 1} of its map, then
+// {state behind it, 2} in the first.
+__device__ __forceinline__ uint64_t* words_of(const Scan& s, int64_t tile, uint32_t column) {
+  return s.words + (tile * s.columns_of_tiles + column) * (kStateBytes / 8) +
+         2 * (threadIdx.x & (kWaveSize - 1));
+}
+__device__ __forceinline__ void put_word(uint64_t* w, uint32_t flag, float v) {
+  __hip_atomic_store(w, (uint64_t)flag << 32 | __builtin_bit_cast(uint32_t, v), __ATOMIC_RELAXED,
+                     __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t get_word(const uint64_t* w) {
+  return __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float value_of(uint64_t w) {
+  return __builtin_bit_cast(float, (uint32_t)w);
+}
+
+// The state in front of a tile, a channel a lane, by one wave.  The tiles in front have drawn
+// their tickets before this one, so they run and publish, and no wait is long.  (It ends all the same, with a
+// NaN, if the words are another call's, to which the temp was given at the same time.)
+__device__ __forceinline__ float look_back(const Scan& s, int64_t tile, uint32_t column, Map own) {
+  uint64_t* mine = words_of(s, tile, column);
+  float h = 0.0f;
+  if (tile > 0) {
+    if (is_reset(own.a)) {
+      put_word(mine, 2, own.b);
+    } else {
+      put_word(mine + 1, 1, own.a);
+      put_word(mine, 1, own.b);
+    }
+    h = __builtin_nanf("");
+    for (uint32_t polls = 0; polls < kMostPolls; ++polls) {
+      uint64_t low[kWindow], high[kWindow];
+#pragma unroll
+      for (int d = 0; d < kWindow; ++d) {
+        const int64_t front = tile - 1 - d;
+        const uint64_t* w = words_of(s, front > 0 ? front : 0, column);
+        low[d] = get_word(w);
+        high[d] = get_word(w + 1);
+      }
+      int found = -1;  // the nearest tile whose state is known, all maps behind it being there
+      bool whole = true;
+#pragma unroll
+      for (int d = 0; d < kWindow; ++d) {
+        if (whole && found < 0 && low[d] >> 32 == 2) found = d;
+        whole = whole && low[d] >> 32 == 1 && high[d] >> 32 == 1;
+      }
+      if (__all(found >= 0)) {
+#pragma unroll
+        for (int d = kWindow - 1; d >= 0; --d) {
+          if (d == found) h = value_of(low[d]);
+          else if (d < found) h = apply(Map{value_of(high[d]), value_of(low[d])}, h);
+        }
+        break;
+      }
+      __builtin_amdgcn_s_sleep(1);
+    }
+  }
+  put_word(mine, 2, apply(own, h));
+  return h;
+}
+
+template <typename T, int W, int R, bool BACK, bool SIGMOID>
+__global__ __launch_bounds__(kBlock) void recurrence_kernel(Scan s) {
+  constexpr int kGroups = groups_of<W>(), kTileRows = kGroups * R, kLanes = kTileChannels / W;
+  constexpr int kWaveGroups = kGroups / kWaves;
+  using V = typename Pack<T, W>::vec;
+  using P = typename Pack<T, W>::type;
+  __shared__ Map maps[kGroups][kTileChannels];
+  __shared__ Map wave_maps[kWaves][kTileChannels];
+  __shared__ float wave_states[kWaves][kTileChannels];
+  __shared__ int32_t begins[kTileRows], ends[kTileRows];
+  __shared__ uint32_t ticket;
+
+  const uint32_t column = (uint32_t)((s.first_block + blockIdx.x) % s.columns_of_tiles);
+  int64_t tile = 0;
+  if (s.tickets != nullptr) {
+    if (threadIdx.x == 0)
+      ticket = __hip_atomic_fetch_add(s.tickets + column * (kTicketBytes / 4), 1u,
+                                      __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    tile = ticket;
+    if (tile >= s.tiles) return;
+  }
+  const int64_t first = (BACK ? s.tiles - 1 - tile : tile) * kTileRows;
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  // This thread's channels: the last W of the row where it ends inside them, `skip` of which
+  // are another thread's.
+  const int64_t c = (int64_t)column * kTileChannels + lane * W;
+  const int64_t at = c + W <= s.channels ? c : s.channels - W;
+  const int skip = (int)(c - at < W ? c - at : W);
+  // Its rows, in the order of the scan.
+  const auto row_in_tile = [&](int r) {
+    return BACK ? kTileRows - 1 - (group * R + r) : group * R + r;
+  };
+  const auto row_to_read = [&](int r) {
+    const int64_t row = first + row_in_tile(r);
+    return row < s.rows ? row : s.rows - 1;
+  };
+  V gate[R], in[R], grad[BACK ? R : 1], before[BACK ? R : 1];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t row = row_to_read(r);
+    gate[r] = *reinterpret_cast<const P*>(static_cast<const T*>(s.gate) + row * s.gate_stride + at);
+    in[r] = *reinterpret_cast<const P*>(static_cast<const T*>(s.in) + row * s.in_stride + at);
+    if constexpr (BACK) {
+      grad[r] = *reinterpret_cast<const P*>(static_cast<const T*>(s.grad_out) +
+                                            row * s.grad_out_stride + at);
+      before[r] = *reinterpret_cast<const P*>(static_cast<const T*>(s.states) +
+                                              (row > 0 ? row - 1 : 0) * s.states_stride + at);
+    }
+  }
+  int64_t from, to;
+  mark_rows<kTileRows>(s.sequences, first, s.rows, begins, ends, &from, &to);
+  // Rows that forget what comes in, and rows of a sequence, a bit each.
+  uint32_t resets = 0, there = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = row_in_tile(r);
+    if (first + i >= from && first + i < to) there |= 1u << r;
+    if ((BACK ? ends : begins)[i] >= 0) resets |= 1u << r;
+  }
+  resets &= there;
+
+  float a[R][W], left[BACK ? R : 1][W], b[R][W];
+  Map own[W];
+#pragma unroll
+  for (int k = 0; k < W; ++k) own[k] = Map{1.0f, 0.0f};
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      float l;
+      decay_of<SIGMOID>((float)gate[r][k], a[r][k], l);
+      if constexpr (BACK) {
+        left[r][k] = l;
+        b[r][k] = (float)grad[r][k];
+      } else {
+        b[r][k] = s.complement ? l * (float)in[r][k] : (float)in[r][k];
+      }
+    }
+    if (resets >> r & 1u) {  // what the sequence begins with is a part of b
+      const float* state = BACK ? s.grad_final : s.initial;
+      if (state != nullptr) {
+        state += (BACK ? ends : begins)[row_in_tile(r)] *
+                     (BACK ? s.grad_final_stride : s.initial_stride) + at;
+#pragma unroll
+        for (int k = 0; k < W; ++k) b[r][k] = BACK ? b[r][k] + state[k] : fmaf(a[r][k], state[k], b[r][k]);
+      }
+    }
+    if (!(there >> r & 1u)) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        a[r][k] = 1.0f;
+        b[r][k] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      const float h = resets >> r & 1u ? 0.0f : own[k].b;
+      own[k].b = BACK ? a[r][k] * (b[r][k] + h) : fmaf(a[r][k], h, b[r][k]);
+      own[k].a *= a[r][k];
+    }
+  }
+  if (resets != 0) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) own[k].a = -0.0f;
+  }
+#pragma unroll
+  for (int k = 0; k < W; ++k) maps[group][lane * W + k] = own[k];
+  __syncthreads();
+  // The maps in front of each group of a wave, then those in front of each wave.
+  const int wave = threadIdx.x / kWaveSize, channel = threadIdx.x % kWaveSize;
+  Map front{1.0f, 0.0f};
+#pragma unroll
+  for (int g = 0; g < kWaveGroups; ++g) {
+    const Map here = maps[wave * kWaveGroups + g][channel];
+    maps[wave * kWaveGroups + g][channel] = front;
+    front = behind(here, front);
+  }
+  wave_maps[wave][channel] = front;
+  __syncthreads();
+  if (wave == 0) {
+    Map all = wave_maps[0][channel];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) all = behind(wave_maps[w][channel], all);
+    float h = s.tickets != nullptr ? look_back(s, tile, column, all) : 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      wave_states[w][channel] = h;
+      h = apply(wave_maps[w][channel], h);
+    }
+  }
+  __syncthreads();
+  float h[W];
+#pragma unroll
+  for (int k = 0; k < W; ++k)
+    h[k] = apply(maps[group][lane * W + k], wave_states[wave][lane * W + k]);
+
+  const auto store = [&](void* to_, int64_t stride, int64_t row, const float (&v)[W]) {
+    T* p = static_cast<T*>(to_) + row * stride + at;
+    if (skip == 0) {
+      V packed;
+#pragma unroll
+      for (int k = 0; k < W; ++k) packed[k] = (T)v[k];
+      *reinterpret_cast<P*>(p) = packed;
+    } else {
+#pragma unroll
+      for (int k = 0; k < W; ++k)
+        if (k >= skip) p[k] = (T)v[k];
+    }
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int i = row_in_tile(r);
+    const int64_t row = first + i;
+    if (!(there >> r & 1u)) continue;
+    if constexpr (!BACK) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) h[k] = fmaf(a[r][k], resets >> r & 1u ? 0.0f : h[k], b[r][k]);
+      store(s.out, s.out_stride, row, h);
+    } else {
+      float reaches[W], of_gate[W], of_in[W], state[W];
+#pragma unroll
+      for (int k = 0; k < W; ++k) state[k] = (float)before[r][k];
+      if (begins[i] >= 0) {
+#pragma unroll
+        for (int k = 0; k < W; ++k)
+          state[k] = s.initial != nullptr ? s.initial[begins[i] * s.initial_stride + at + k] : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        reaches[k] = b[r][k] + (resets >> r & 1u ? 0.0f : h[k]);
+        h[k] = a[r][k] * reaches[k];
+        const float slope = SIGMOID ? a[r][k] * left[r][k] : a[r][k];
+        of_gate[k] = reaches[k] * (s.complement ? state[k] - (float)in[r][k] : state[k]) * slope;
+        of_in[k] = s.complement ? reaches[k] * left[r][k] : reaches[k];
+      }
+      if (s.out != nullptr) store(s.out, s.out_stride, row, of_gate);
+      if (s.grad_in != nullptr) store(s.grad_in, s.grad_in_stride, row, of_in);
+    }
+    const int32_t last = (BACK ? begins : ends)[i];
+    if (s.last != nullptr && last >= 0) {
+      float* p = s.last + last * s.last_stride + at;
+#pragma unroll
+      for (int k = 0; k < W; ++k)
+        if (k >= skip) p[k] = h[k];
+    }
+  }
+  // Sequences without rows leave what they begin with.
+  if (s.last == nullptr || s.sequences.offsets == nullptr) return;
+  const float* begin = BACK ? s.grad_final : s.initial;
+  const int64_t begin_stride = BACK ? s.grad_final_stride : s.initial_stride;
+  for (int64_t i = tile * kBlock + threadIdx.x; i < s.sequences.count; i += s.tiles * kBlock) {
+    if (s.sequences.offset(i + 1) > s.sequences.offset(i)) continue;
+    for (int64_t k = (int64_t)column * kTileChannels;
+         k < s.channels && k < (int64_t)(column + 1) * kTileChannels; ++k)
+      s.last[i * s.last_stride + k] = begin != nullptr ? begin[i * begin_stride + k] : 0.0f;
+  }
+}
+
+// One row for each sequence.
+template <typename T, int W, bool SIGMOID>
+__global__ __launch_bounds__(kBlock) void recurrence_step_kernel(Scan s) {
+  const int64_t vectors = (s.channels + W - 1) / W, step = (int64_t)gridDim.x * kBlock;
+  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < s.rows * vectors; i += step) {
+    const int64_t row = i / vectors, c = i % vectors * W, count = s.channels - c;
+    float gate[W], in[W], h[W];
+    load_floats<T, W>(gate, static_cast<const T*>(s.gate) + row * s.gate_stride + c, count);
+    load_floats<T, W>(in, static_cast<const T*>(s.in) + row * s.in_stride + c, count);
+    if (s.initial != nullptr) {
+      load_floats<float, W>(h, s.initial + row * s.initial_stride + c, count);
+    } else {
+#pragma unroll
+      for (int k = 0; k < W; ++k) h[k] = 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      float a, left;
+      decay_of<SIGMOID>(gate[k], a, left);
+      h[k] = fmaf(a, h[k], s.complement ? left * in[k] : in[k]);
+    }
+    store_floats<T, W>(static_cast<T*>(s.out) + row * s.out_stride + c, h, count);
+    if (s.last != nullptr) store_floats<float, W>(s.last + row * s.last_stride + c, h, count);
+  }
+}
+
+// No rows at all: every sequence leaves what it begins with.
+__global__ __launch_bounds__(kBlock) void recurrence_states_kernel(
+    const float* from, int64_t from_stride, float* to, int64_t to_stride, int64_t sequences,
+    int64_t channels) {
+  const int64_t step = (int64_t)gridDim.x * kBlock;
+  for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < sequences * channels; i += step) {
+    const int64_t row = i / channels, c = i % channels;
+    to[row * to_stride + c] = from != nullptr ? from[row * from_stride + c] : 0.0f;
+  }
+}
+
+inline unsigned blocks_for_elements(int64_t threads) {
+  const int64_t blocks = div_up(threads, kBlock);
+  return (unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks);
+}
+
+inline int64_t columns_of_tiles(int64_t channels) { return div_up(channels, kTileChannels); }
+
+template <typename T, int W, int R, bool BACK, bool SIGMOID>
+int32_t launch_scan_tiles(hipStream_t stream, Scan s, void* temp) {
+  s.tiles = div_up(s.rows, (int64_t)groups_of<W>() * R);
+  s.columns_of_tiles = (uint32_t)columns_of_tiles(s.channels);
+  if (s.tiles > 1) {
+    char* base = reinterpret_cast<char*>(align_up((int64_t)(uintptr_t)temp, 128));
+    const int64_t tickets = s.columns_of_tiles * kTicketBytes;
+    s.tickets = reinterpret_cast<uint32_t*>(base);
+    s.words = reinterpret_cast<uint64_t*>(base + tickets);
+    const int32_t rc = launch_zero_words(
+        stream, s.tickets, (tickets + s.tiles * s.columns_of_tiles * kStateBytes) / 4);
+    if (rc != ILGPU_HIP_SUCCESS) return rc;
+  }
+  const int64_t blocks = s.tiles * s.columns_of_tiles;
+  for (s.first_block = 0; s.first_block < blocks; s.first_block += kMostBlocks) {
+    const int64_t left = blocks - s.first_block;
+    {
+      ProfileScope scope(stream, BACK ? "recurrence_gradient" : "recurrence");
+      hipLaunchKernelGGL((recurrence_kernel<T, W, R, BACK, SIGMOID>),
+                         dim3((unsigned)(left < kMostBlocks ? left : kMostBlocks)), dim3(kBlock), 0,
+                         stream, s);
+    }
+    ILGPU_HIP_CHECK(hipGetLastError());
+  }
+  return ILGPU_HIP_SUCCESS;
+}
+
+template <bool BACK, bool SIGMOID>
+int32_t launch_scan_of(hipStream_t stream, int32_t type, const Scan& s, void* temp) {
+  return with_type(type, [&](auto t) -> int32_t {
+    using T = decltype(t);
+    constexpr int W = 16 / sizeof(T), R = BACK ? kBackRows : kRows;
+    if (!BACK && s.sequences.offsets == nullptr && s.sequences.length == 1) {
+      {
+        ProfileScope scope(stream, "recurrence_step");
+        hipLaunchKernelGGL((recurrence_step_kernel<T, W, SIGMOID>),
+                           dim3(blocks_for_elements(s.rows * div_up(s.channels, W))), dim3(kBlock),
+                           0, stream, s);
+      }
+      ILGPU_HIP_CHECK(hipGetLastError());
+      return ILGPU_HIP_SUCCESS;
+    }
+    // (A row shorter than a vector: an element a thread.)
+    if (s.channels < W) return launch_scan_tiles<T, 1, R, BACK, SIGMOID>(stream, s, temp);
+    return launch_scan_tiles<T, W, R, BACK, SIGMOID>(stream, s, temp);
+  });
+}
+
+template <bool BACK>
+int32_t launch_scan(hipStream_t stream, int32_t type, int32_t decay, const Scan& s, void* temp) {
+  if (s.rows == 0) {
+    if (s.last == nullptr || s.sequences.count == 0) return ILGPU_HIP_SUCCESS;
+    {
+      ProfileScope scope(stream, "recurrence_states");
+      hipLaunchKernelGGL(recurrence_states_kernel,
+                         dim3(blocks_for_elements(s.sequences.count * s.channels)), dim3(kBlock), 0,
+                         stream, BACK ? s.grad_final : s.initial,
+                         BACK ? s.grad_final_stride : s.initial_stride, s.last, s.last_stride,
+                         s.sequences.count, s.channels);
+    }
+    ILGPU_HIP_CHECK(hipGetLastError());
+    return ILGPU_HIP_SUCCESS;
+  }
+  return decay == ILGPU_HIP_DECAY_SIGMOID ? launch_scan_of<BACK, true>(stream, type, s, temp)
+                                          : launch_scan_of<BACK, false>(stream, type, s, temp);
+}
+
+}  // namespace
+
+// Tickets and words of the shortest tiles that such a call may take.
+int64_t gated_recurrence_temp_bytes(int64_t rows, int64_t channels) {
+  const int64_t tile_rows = (channels < 8 ? groups_of<1>() : groups_of<4>()) * kFewestRows;
+  const int64_t tiles = div_up(rows, tile_rows);
+  if (tiles <= 1) return 0;
+  return 128 + columns_of_tiles(channels) * (kTicketBytes + tiles * kStateBytes);
+}
+
+int32_t launch_gated_recurrence(hipStream_t stream, const GatedRecurrenceArgs& a) {
+  Scan s{};
+  s.gate = a.gate;
+  s.gate_stride = a.gate_stride;
+  s.in = a.in;
+  s.in_stride = a.in_stride;
+  s.rows = a.rows;
+  s.channels = a.channels;
+  s.complement = a.complement;
+  s.sequences = Sequences{a.offsets, a.offset_type == ILGPU_HIP_I64, a.sequences,
+                          (uint32_t)(a.sequences > 0 ? a.rows / a.sequences : 0)};
+  s.initial = a.initial;
+  s.initial_stride = a.initial_stride;
+  if (!a.backwards) {
+    s.out = a.out;
+    s.out_stride = a.out_stride;
+    s.last = a.final_state;
+    s.last_stride = a.final_stride;
+    return launch_scan<false>(stream, a.type, a.decay, s, a.temp);
+  }
+  s.states = a.out;
+  s.states_stride = a.out_stride;
+  s.grad_out = a.grad_out;
+  s.grad_out_stride = a.grad_out_stride;
+  s.grad_final = a.grad_final;
+  s.grad_final_stride = a.grad_final_stride;
+  s.out = a.grad_gate;
+  s.out_stride = a.grad_gate_stride;
+  s.grad_in = a.grad_in;
+  s.grad_in_stride = a.grad_in_stride;
+  s.last = a.grad_initial;
+  s.last_stride = a.grad_initial_stride;
+  return launch_scan<true>(stream, a.type, a.decay, s, a.temp);
+}
+
+}  // namespace ilgpu_hip

@@ -245,49 +245,11 @@ __global__ __launch_bounds__(gradient_block<LANES>()) void layer_norm_gradient_k
     own.store(grad_in + row * grad_in_stride, h);
   }
   if (partials == nullptr) return;
-  // The block's sums: over the rows of a wave, then over the waves, in their order; into its
-  // row of partials, or, of a single block, to where they belong.
-  const auto join = [&](float (&sum)[V][W], float* to, TW* result) {
-    const auto put = [&](int64_t c, float total) {
-      if (gridDim.x > 1) to[c] = total;
-      else if (result != nullptr) result[c] = (TW)(accumulate ? (float)result[c] + total : total);
-    };
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-#pragma unroll
-      for (int k = 0; k < W; ++k)
-#pragma unroll
-        for (int off = LANES; off < kWaveSize; off <<= 1)
-          sum[v][k] += __shfl_xor(sum[v][k], off, kWaveSize);
-    if constexpr (kJoins > 1) {
-      const int wave = threadIdx.x / kWaveSize, lane = threadIdx.x & (kWaveSize - 1);
-      if (lane < LANES) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-          for (int k = 0; k < W; ++k) joined[wave][(v * W + k) * LANES + lane] = sum[v][k];
-      }
-      __syncthreads();
-      for (int i = threadIdx.x; i < LANES * V * W; i += gradient_block<LANES>()) {
-        float total = joined[0][i];
-#pragma unroll
-        for (int j = 1; j < kJoins; ++j) total += joined[j][i];
-        const int k = i / LANES % W;
-        const int64_t first = ((int64_t)(i / (LANES * W)) * LANES + i % LANES) * W;
-        const int64_t at = first + W <= columns ? first : columns - W;
-        if (at + k >= first) put(at + k, total);
-      }
-      __syncthreads();
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-#pragma unroll
-        for (int k = 0; k < W; ++k)
-          if (k >= own.skip[v]) put(own.at[v] + k, sum[v][k]);
-    }
-  };
-  join(sum_w, partials + (int64_t)blockIdx.x * columns, grad_weight);
-  join(sum_b, partials + ((int64_t)gridDim.x + blockIdx.x) * columns, grad_bias);
+  join_columns<TW, W, LANES, V, kJoins>(own, sum_w, columns, partials + (int64_t)blockIdx.x * columns,
+                                        grad_weight, accumulate, joined);
+  join_columns<TW, W, LANES, V, kJoins>(own, sum_b, columns,
+                                        partials + ((int64_t)gridDim.x + blockIdx.x) * columns,
+                                        grad_bias, accumulate, joined);
 }
 
 // Rows too long for the registers: a block a row for grad_in, and the columns' sums apart.

@@ -194,6 +194,52 @@ template <typename F> int32_t with_norm_types(int32_t type, int32_t weight_type,
   });
 }
 
+// The column sums of a block: over the rows of a wave, then over the waves, in their order; into
+// the block's row of partials, or, of a single block, to where they belong (result, which may be
+// nullptr).  `joined` is LDS of one row of floats for each wave, where more waves than one share the columns.
+template <typename TW, int W, int LANES, int V, int WAVES, typename Joined>
+__device__ __forceinline__ void join_columns(const Columns<W, LANES, V>& own, float (&sum)[V][W],
+                                             int64_t columns, float* to, TW* result,
+                                             int32_t accumulate, Joined& joined) {
+  const auto put = [&](int64_t c, float total) {
+    if (gridDim.x > 1) to[c] = total;
+    else if (result != nullptr) result[c] = (TW)(accumulate ? (float)result[c] + total : total);
+  };
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+#pragma unroll
+    for (int k = 0; k < W; ++k)
+#pragma unroll
+      for (int off = LANES; off < kWaveSize; off <<= 1)
+        sum[v][k] += __shfl_xor(sum[v][k], off, kWaveSize);
+  if constexpr (WAVES > 1) {
+    const int wave = threadIdx.x / kWaveSize, lane = threadIdx.x & (kWaveSize - 1);
+    if (lane < LANES) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int k = 0; k < W; ++k) joined[wave][(v * W + k) * LANES + lane] = sum[v][k];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < LANES * V * W; i += WAVES * kWaveSize) {
+      float total = joined[0][i];
+#pragma unroll
+      for (int j = 1; j < WAVES; ++j) total += joined[j][i];
+      const int k = i / LANES % W;
+      const int64_t first = ((int64_t)(i / (LANES * W)) * LANES + i % LANES) * W;
+      const int64_t at = first + W <= columns ? first : columns - W;
+      if (at + k >= first) put(at + k, total);
+    }
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int k = 0; k < W; ++k)
+        if (k >= own.skip[v]) put(own.at[v] + k, sum[v][k]);
+  }
+}
+
 // Adds up `splits` rows of partials: 64 columns a block, whose waves take every 16th row;
 // blockIdx.y: the weight's, the bias's.  A launch begins at block `first_block`: a grid holds less
 // than 2^32 threads, which 2^28 columns would be.

@@ -1220,5 +1220,248 @@ inline void ClipGradients(Accelerator& accelerator, AcceleratorStream& stream,
   ClipGradients(accelerator, stream, gradients, gradients, norm, maxNorm);
 }
 
+// What the gated recurrence makes of its gates and inputs.
+enum class DecayKind : int32_t {
+  Sigmoid = ILGPU_HIP_DECAY_SIGMOID,
+  Exponential = ILGPU_HIP_DECAY_EXPONENTIAL
+};
+
+template <typename T> bool SameShape(const MatrixView<T>& view, int64_t rows, int64_t columns) {
+  return view.LoadEffectiveAddressAsPtr() == nullptr ||
+         (view.Rows() == rows && view.Columns() == columns);
+}
+
+// In 32-bit ints; 0 where a call over so many rows needs no temp.
+inline int64_t ComputeGatedRecurrenceTempStorageSize(Accelerator&, int64_t rows,
+                                                     int64_t channels) {
+  int64_t bytes = 0;
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_gated_recurrence_temp_bytes(rows, channels, &bytes), "rows");
+  return (bytes + 3) / 4;
+}
+// The sequences of a packed batch: `Count` equal parts of the rows, or cut at offsets (one more
+// than sequences).
+template <typename TOffset> struct PackedSequences {
+  int64_t Count = 1;
+  ArrayView<TOffset> Offsets = {};
+  void Check() const {
+    CheckLength(!Offsets.IsValid() || Offsets.Length() == Count + 1, "sequences");
+  }
+};
+// output[t] = h[t] = a * h[t-1] + b in every channel of every sequence, with a = sigmoid(gate) or
+// exp(gate), b = input or (1 - a) * input.  initial and final may be views without a buffer.
+template <typename T, typename TOffset>
+void GatedRecurrence(Accelerator&, AcceleratorStream& stream, MatrixView<T> gate,
+                     MatrixView<T> input, MatrixView<T> output,
+                     PackedSequences<TOffset> sequences, DecayKind decay, bool complement,
+                     MatrixView<float> initial, MatrixView<float> final,
+                     ArrayView<int32_t> temp) {
+  CheckLength(gate.Rows() == input.Rows() && gate.Columns() == input.Columns(), "gate");
+  CheckLength(output.Rows() == input.Rows() && output.Columns() == input.Columns(), "output");
+  CheckLength(SameShape(initial, sequences.Count, input.Columns()), "initial");
+  CheckLength(SameShape(final, sequences.Count, input.Columns()), "final");
+  sequences.Check();
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_gated_recurrence(
+          stream.StreamPtr(), gate.LoadEffectiveAddressAsPtr(), gate.RowStride(),
+          input.LoadEffectiveAddressAsPtr(), input.RowStride(), input.Rows(), input.Columns(),
+          TypeCode<T>::value, (int32_t)decay, complement ? 1 : 0,
+          sequences.Offsets.LoadEffectiveAddressAsPtr(), TypeCode<TOffset>::value,
+          sequences.Count, initial.LoadEffectiveAddressAsPtr(), initial.RowStride(),
+          output.LoadEffectiveAddressAsPtr(), output.RowStride(),
+          final.LoadEffectiveAddressAsPtr(), final.RowStride(),
+          temp.LoadEffectiveAddressAsPtr(), temp.Length() * 4),
+      "temp");
+}
+// Its gradients; gradGate, gradInput and gradInitial may be views without a buffer: not wanted.
+template <typename T, typename TOffset>
+void GatedRecurrenceGradient(Accelerator&, AcceleratorStream& stream, MatrixView<T> gradOutput,
+                             MatrixView<T> gate, MatrixView<T> input, MatrixView<T> output,
+                             PackedSequences<TOffset> sequences, DecayKind decay, bool complement,
+                             MatrixView<float> initial, MatrixView<float> gradFinal,
+                             MatrixView<T> gradGate, MatrixView<T> gradInput,
+                             MatrixView<float> gradInitial, ArrayView<int32_t> temp) {
+  const int64_t rows = input.Rows(), channels = input.Columns();
+  CheckLength(gradOutput.Rows() == rows && gradOutput.Columns() == channels, "gradOutput");
+  CheckLength(gate.Rows() == rows && gate.Columns() == channels, "gate");
+  CheckLength(output.Rows() == rows && output.Columns() == channels, "output");
+  CheckLength(SameShape(gradGate, rows, channels), "gradGate");
+  CheckLength(SameShape(gradInput, rows, channels), "gradInput");
+  CheckLength(SameShape(initial, sequences.Count, channels), "initial");
+  CheckLength(SameShape(gradFinal, sequences.Count, channels), "gradFinal");
+  CheckLength(SameShape(gradInitial, sequences.Count, channels), "gradInitial");
+  sequences.Check();
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_gated_recurrence_gradient(
+          stream.StreamPtr(), gradOutput.LoadEffectiveAddressAsPtr(), gradOutput.RowStride(),
+          gate.LoadEffectiveAddressAsPtr(), gate.RowStride(), input.LoadEffectiveAddressAsPtr(),
+          input.RowStride(), output.LoadEffectiveAddressAsPtr(), output.RowStride(), rows,
+          channels, TypeCode<T>::value, (int32_t)decay, complement ? 1 : 0,
+          sequences.Offsets.LoadEffectiveAddressAsPtr(), TypeCode<TOffset>::value,
+          sequences.Count, initial.LoadEffectiveAddressAsPtr(), initial.RowStride(),
+          gradFinal.LoadEffectiveAddressAsPtr(), gradFinal.RowStride(),
+          gradGate.LoadEffectiveAddressAsPtr(), gradGate.RowStride(),
+          gradInput.LoadEffectiveAddressAsPtr(), gradInput.RowStride(),
+          gradInitial.LoadEffectiveAddressAsPtr(), gradInitial.RowStride(),
+          temp.LoadEffectiveAddressAsPtr(), temp.Length() * 4),
+      "temp");
+}
+
+enum class GateKind : int32_t { Sigmoid = ILGPU_HIP_GATE_SIGMOID, Silu = ILGPU_HIP_GATE_SILU };
+
+// What a block's output passes through on its way into the residual stream: a norm, a gate and
+// a scale.  Views without a buffer: a weight of 1, no gate.
+template <typename T, typename TWeight> struct BlockOutput {
+  bool Normalized = false;
+  ArrayView<TWeight> Weight = {};
+  MatrixView<T> Gate = {};
+  GateKind Kind = GateKind::Silu;
+  float Scale = 1.0f;
+  void Check(const MatrixView<T>& input) const {
+    CheckLength(!Weight.IsValid() || Weight.Length() == input.Columns(), "Weight");
+    CheckLength(SameShape(Gate, input.Rows(), input.Columns()), "Gate");
+  }
+};
+// total = residual + scale * y, output = total * rstd * weight, with y the input behind its
+// BlockOutput.  residual, total, output, weight and both rstd may be views without a buffer.
+template <typename T, typename TResidual, typename TWeight>
+void ResidualNorm(Accelerator&, AcceleratorStream& stream, MatrixView<T> input,
+                  BlockOutput<T, TWeight> block, MatrixView<TResidual> residual,
+                  MatrixView<TResidual> total, MatrixView<T> output, ArrayView<TWeight> weight,
+                  float epsilon, ArrayView<float> inputRstd = {}, ArrayView<float> rstd = {}) {
+  const int64_t rows = input.Rows(), columns = input.Columns();
+  block.Check(input);
+  CheckLength(SameShape(residual, rows, columns), "residual");
+  CheckLength(SameShape(total, rows, columns), "total");
+  CheckLength(SameShape(output, rows, columns), "output");
+  CheckLength(!weight.IsValid() || weight.Length() == columns, "weight");
+  CheckLength(!inputRstd.IsValid() || inputRstd.Length() >= rows, "inputRstd");
+  CheckLength(!rstd.IsValid() || rstd.Length() >= rows, "rstd");
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_residual_norm(
+          stream.StreamPtr(), input.LoadEffectiveAddressAsPtr(), input.RowStride(), rows, columns,
+          TypeCode<T>::value, block.Normalized ? 1 : 0, block.Weight.LoadEffectiveAddressAsPtr(),
+          block.Gate.LoadEffectiveAddressAsPtr(), block.Gate.RowStride(), (int32_t)block.Kind,
+          residual.LoadEffectiveAddressAsPtr(), residual.RowStride(), TypeCode<TResidual>::value,
+          &block.Scale, weight.LoadEffectiveAddressAsPtr(), TypeCode<TWeight>::value, &epsilon,
+          total.LoadEffectiveAddressAsPtr(), total.RowStride(),
+          output.LoadEffectiveAddressAsPtr(), output.RowStride(),
+          inputRstd.LoadEffectiveAddressAsPtr(), rstd.LoadEffectiveAddressAsPtr()),
+      "input");
+}
+
+inline int64_t ComputeResidualNormGradientTempStorageSize(Accelerator&, int64_t rows,
+                                                          int64_t columns) {
+  int64_t bytes = 0;
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_residual_norm_gradient_temp_bytes(rows, columns, &bytes), "rows");
+  return (bytes + 3) / 4;
+}
+// Where its gradients go; views without a buffer are not wanted.
+template <typename T, typename TResidual, typename TWeight> struct ResidualNormGradients {
+  MatrixView<T> Input = {};
+  MatrixView<T> Gate = {};
+  MatrixView<TResidual> Residual = {};
+  ArrayView<TWeight> InputWeight = {};
+  ArrayView<TWeight> Weight = {};
+  bool Accumulate = false;
+};
+// gradOutput or gradTotal may be a view without a buffer: not used.
+template <typename T, typename TResidual, typename TWeight>
+void ResidualNormGradient(Accelerator&, AcceleratorStream& stream, MatrixView<T> gradOutput,
+                          MatrixView<TResidual> gradTotal, MatrixView<T> input,
+                          BlockOutput<T, TWeight> block, ArrayView<float> inputRstd,
+                          MatrixView<TResidual> total, ArrayView<TWeight> weight,
+                          ArrayView<float> rstd,
+                          ResidualNormGradients<T, TResidual, TWeight> gradients,
+                          ArrayView<int32_t> temp) {
+  const int64_t rows = input.Rows(), columns = input.Columns();
+  block.Check(input);
+  CheckLength(SameShape(gradOutput, rows, columns), "gradOutput");
+  CheckLength(SameShape(gradTotal, rows, columns), "gradTotal");
+  CheckLength(SameShape(total, rows, columns), "total");
+  CheckLength(!weight.IsValid() || weight.Length() == columns, "weight");
+  CheckLength(!inputRstd.IsValid() || inputRstd.Length() >= rows, "inputRstd");
+  CheckLength(!rstd.IsValid() || rstd.Length() >= rows, "rstd");
+  CheckLength(SameShape(gradients.Input, rows, columns), "gradients.Input");
+  CheckLength(SameShape(gradients.Gate, rows, columns), "gradients.Gate");
+  CheckLength(SameShape(gradients.Residual, rows, columns), "gradients.Residual");
+  CheckLength(!gradients.InputWeight.IsValid() || gradients.InputWeight.Length() == columns,
+              "gradients.InputWeight");
+  CheckLength(!gradients.Weight.IsValid() || gradients.Weight.Length() == columns,
+              "gradients.Weight");
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_residual_norm_gradient(
+          stream.StreamPtr(), gradOutput.LoadEffectiveAddressAsPtr(), gradOutput.RowStride(),
+          gradTotal.LoadEffectiveAddressAsPtr(), gradTotal.RowStride(),
+          input.LoadEffectiveAddressAsPtr(), input.RowStride(), rows, columns, TypeCode<T>::value,
+          block.Normalized ? 1 : 0, block.Weight.LoadEffectiveAddressAsPtr(),
+          inputRstd.LoadEffectiveAddressAsPtr(), block.Gate.LoadEffectiveAddressAsPtr(),
+          block.Gate.RowStride(), (int32_t)block.Kind, total.LoadEffectiveAddressAsPtr(),
+          total.RowStride(), TypeCode<TResidual>::value, &block.Scale,
+          weight.LoadEffectiveAddressAsPtr(), TypeCode<TWeight>::value,
+          rstd.LoadEffectiveAddressAsPtr(), gradients.Input.LoadEffectiveAddressAsPtr(),
+          gradients.Input.RowStride(), gradients.Gate.LoadEffectiveAddressAsPtr(),
+          gradients.Gate.RowStride(), gradients.Residual.LoadEffectiveAddressAsPtr(),
+          gradients.Residual.RowStride(), gradients.InputWeight.LoadEffectiveAddressAsPtr(),
+          gradients.Weight.LoadEffectiveAddressAsPtr(), gradients.Accumulate ? 1 : 0,
+          temp.LoadEffectiveAddressAsPtr(), temp.Length() * 4),
+      "temp");
+}
+
+// The numbers of an AdamW step.
+struct AdamWOptions {
+  double Rate, Beta1 = 0.9, Beta2 = 0.999, Epsilon = 1e-8, WeightDecay = 0.0;
+  double MaxNorm = std::numeric_limits<double>::infinity();
+  int64_t Seed = 0;
+};
+// A moment: float32 tensors, or bytes with a scale for each 256 of their elements.
+struct Moments {
+  TensorList Values;
+  TensorList Scales;  // empty: float32
+};
+// One step, in place; copies may be empty, schedule and norm views without a buffer.
+inline void AdamW(Accelerator&, AcceleratorStream& stream, const TensorList& parameters,
+                  const TensorList& gradients, const Moments& first, const Moments& second,
+                  const AdamWOptions& options, ArrayView<int64_t> step,
+                  const TensorList& copies = {}, ArrayView<float> schedule = {},
+                  ArrayView<float> norm = {}) {
+  const int64_t count = parameters.Count();
+  CheckLength(gradients.Count() == count, "gradients");
+  CheckLength(first.Values.Count() == count, "first");
+  CheckLength(second.Values.Count() == count, "second");
+  const bool bytes = first.Scales.Count() > 0 || second.Scales.Count() > 0;
+  CheckLength(!bytes || first.Scales.Count() == count, "first");
+  CheckLength(!bytes || second.Scales.Count() == count, "second");
+  CheckLength(copies.Count() == 0 || copies.Count() == count, "copies");
+  if (!step.IsValid()) throw ArgumentNullException("step");
+  const ilgpu_hip_adamw_options o{options.Rate,        options.Beta1,   options.Beta2,
+                                  options.Epsilon,     options.WeightDecay,
+                                  options.MaxNorm,     options.Seed};
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_adamw(stream.StreamPtr(), parameters.Data(), gradients.Data(),
+                      first.Values.Data(), second.Values.Data(),
+                      bytes ? first.Scales.Data() : nullptr,
+                      bytes ? second.Scales.Data() : nullptr,
+                      copies.Count() > 0 ? copies.Data() : nullptr, count, &o,
+                      step.LoadEffectiveAddressAsPtr(), schedule.LoadEffectiveAddressAsPtr(),
+                      norm.LoadEffectiveAddressAsPtr()),
+      "parameters");
+}
+// 8-bit moments as the numbers they stand for.
+inline void AdamWMoments(Accelerator&, AcceleratorStream& stream, const Moments& first,
+                         const TensorList& firstTargets, const Moments& second,
+                         const TensorList& secondTargets) {
+  const int64_t count = firstTargets.Count();
+  CheckLength(first.Values.Count() == count && first.Scales.Count() == count, "first");
+  CheckLength(second.Values.Count() == count && second.Scales.Count() == count, "second");
+  CheckLength(secondTargets.Count() == count, "secondTargets");
+  HipAlgorithmsException::ThrowIfFailed(
+      ilgpu_hip_adamw_moments(stream.StreamPtr(), first.Values.Data(), first.Scales.Data(),
+                              firstTargets.Data(), second.Values.Data(), second.Scales.Data(),
+                              secondTargets.Data(), count),
+      "first");
+}
+
 }  // namespace Algorithms
 }  // namespace ilgpu

@@ -553,6 +553,184 @@ int32_t ilgpu_hip_clip_gradients(ilgpu_hip_stream_t stream,
                                  int64_t count, const float *norm,
                                  const float *max_norm);
 
+/* Gated linear recurrence, one of its own in every channel (column):
+ *   h[t] = a[t] * h[t-1] + b[t]
+ * with a = 1 / (1 + exp(-gate)) or exp(gate) (decay) and b = in, or (1 - a) * in
+ * with complement != 0; 1 - a keeps its precision where a is near 1.  out[t] is
+ * h[t], rounded to `type`; the states themselves are float32 throughout.
+ * Sequences lie behind one another in the rows: sequence i is rows
+ * [offsets[i], offsets[i+1]) with offsets (sequences + 1 numbers, int32 or int64)
+ * in DEVICE memory, or, with offsets NULL, the i-th of `sequences` equal parts
+ * (rows must be a multiple: ILGPU_HIP_ERROR_OUT_OF_RANGE).  In front of its first
+ * row a sequence has the state initial[i] (sequences x channels, float32; NULL:
+ * zeros), behind its last it leaves final_state[i] (NULL: not wanted), and a
+ * sequence without rows leaves what it began with.  Nothing passes from one
+ * sequence to another, NaN and infinities neither.  Rows in front of the first
+ * sequence and behind the last are not written.  offsets ascend from 0 or more to
+ * at most rows; others give unspecified results, but no access outside the
+ * matrices.
+ * One row for each sequence (offsets NULL, sequences == rows) is the step from
+ * token to token; it needs no temp.
+ * out may be gate or in itself, final_state may be initial itself (same base and
+ * stride); otherwise what is written overlaps nothing.  A temp for so many rows
+ * serves any fewer (same channels), and both directions; it may be NULL where the
+ * size asked for is 0. */
+enum ilgpu_hip_decay {
+  ILGPU_HIP_DECAY_SIGMOID = 0,    /* a = 1 / (1 + exp(-gate)) */
+  ILGPU_HIP_DECAY_EXPONENTIAL = 1 /* a = exp(gate) */
+};
+int32_t ilgpu_hip_gated_recurrence_temp_bytes(int64_t rows, int64_t channels,
+                                              int64_t *temp_bytes);
+int32_t ilgpu_hip_gated_recurrence(
+    ilgpu_hip_stream_t stream, const void *gate, int64_t gate_stride,
+    const void *in, int64_t in_stride, int64_t rows, int64_t channels,
+    int32_t type, int32_t decay, int32_t complement, const void *offsets,
+    int32_t offset_type, int64_t sequences, const float *initial,
+    int64_t initial_stride, void *out, int64_t out_stride, float *final_state,
+    int64_t final_stride, void *temp, int64_t temp_bytes);
+
+/* Its gradients from those of out and of the final states (grad_final NULL:
+ * zeros).  With G[t] = grad_out[t] + a[t+1] * G[t+1], the last G of a sequence
+ * being its grad_out + grad_final:
+ *   grad_in      = G, or (1 - a) * G with complement
+ *   grad_gate    = G * (h[t-1], less in[t] with complement) * da
+ *                  with da = a * (1 - a) or a
+ *   grad_initial = a * G of the first row, or grad_final where there is none
+ * h[t-1] is out as the forward call left it, or initial.  Each of grad_gate,
+ * grad_in and grad_initial may be NULL and is not computed then; not all of them.
+ * grad_gate and grad_in may be grad_out, gate or in itself, not both the same;
+ * grad_initial may be grad_final itself. */
+int32_t ilgpu_hip_gated_recurrence_gradient(
+    ilgpu_hip_stream_t stream, const void *grad_out, int64_t grad_out_stride,
+    const void *gate, int64_t gate_stride, const void *in, int64_t in_stride,
+    const void *out, int64_t out_stride, int64_t rows, int64_t channels,
+    int32_t type, int32_t decay, int32_t complement, const void *offsets,
+    int32_t offset_type, int64_t sequences, const float *initial,
+    int64_t initial_stride, const float *grad_final, int64_t grad_final_stride,
+    void *grad_gate, int64_t grad_gate_stride, void *grad_in,
+    int64_t grad_in_stride, float *grad_initial, int64_t grad_initial_stride,
+    void *temp, int64_t temp_bytes);
+
+/* What stands between two blocks of a model: the norm behind the one and its gate,
+ * the residual stream with its scale, and the norm in front of the next.  For every
+ * row, with rms(v) = 1 / sqrt(mean of v^2 + epsilon):
+ *   y     = in [* input_rstd * input_weight] [* act(gate)]    input_rstd = rms(in)
+ *   total = residual + scale * y
+ *   out   = total * rstd * weight                             rstd = rms(total)
+ * The input is normalised with input_norm != 0, and input_weight NULL is 1 then;
+ * act(gate) is gate_kind's function of the matrix gate, or 1 where gate is NULL.
+ * residual NULL: 0.  weight NULL: 1.  scale NULL: 1.  total and out may each be NULL
+ * and are not written then; not both.  Weights have `columns` elements of
+ * weight_type, which is `type` or F32; residual and total are of residual_type,
+ * which is `type` or F32 too.  input_rstd and rstd (float32, one per row) receive
+ * what the gradients need and may be NULL.  out is made from total before it is
+ * rounded to its type.  total may be residual itself; out (and total, of the same
+ * type) may be in or gate itself (same base and stride).  Squares are float32: rows beyond
+ * 1e19 overflow. */
+enum ilgpu_hip_gate {
+  ILGPU_HIP_GATE_SIGMOID = 0, /* 1 / (1 + exp(-gate)) */
+  ILGPU_HIP_GATE_SILU = 1     /* gate / (1 + exp(-gate)) */
+};
+int32_t ilgpu_hip_residual_norm(
+    ilgpu_hip_stream_t stream, const void *in, int64_t in_stride, int64_t rows,
+    int64_t columns, int32_t type, int32_t input_norm,
+    const void *input_weight, const void *gate, int64_t gate_stride,
+    int32_t gate_kind, const void *residual, int64_t residual_stride,
+    int32_t residual_type, const float *scale, const void *weight,
+    int32_t weight_type, const float *epsilon, void *total,
+    int64_t total_stride, void *out, int64_t out_stride, float *input_rstd,
+    float *rstd);
+
+/* Its gradients from those of out (NULL: out was not used; then total, weight and
+ * rstd are not either) and of total (NULL: only out was used); not both NULL.  total
+ * and both rstd are the forward call's.  With h = total * rstd, g = grad_out * weight,
+ * k = in * input_rstd:
+ *   grad_residual     = grad_total + rstd * (g - h * mean of g * h)     =: d
+ *   grad_weight       = sum over the rows of grad_out * h
+ *   grad_gate         = scale * d * (k * input_weight) * act'(gate)
+ *   grad_input_weight = sum over the rows of e * k       e = scale * d * act(gate)
+ *   grad_in           = input_rstd * (f - k * mean of f * k)  f = e * input_weight
+ * and without input_norm k * input_weight is in, and grad_in is e.  Each of the
+ * five may be NULL and is not computed then; not all of them.
+ * grad_in, grad_gate and grad_residual may be any of the matrices that are read
+ * (of the same type; same base and stride), not the same one.  With accumulate != 0 grad_weight and
+ * grad_input_weight are added to what is there.  No rows leave sums of zero.  A temp
+ * for so many rows serves any fewer (same columns). */
+int32_t ilgpu_hip_residual_norm_gradient_temp_bytes(int64_t rows,
+                                                    int64_t columns,
+                                                    int64_t *temp_bytes);
+int32_t ilgpu_hip_residual_norm_gradient(
+    ilgpu_hip_stream_t stream, const void *grad_out, int64_t grad_out_stride,
+    const void *grad_total, int64_t grad_total_stride, const void *in,
+    int64_t in_stride, int64_t rows, int64_t columns, int32_t type,
+    int32_t input_norm, const void *input_weight, const float *input_rstd,
+    const void *gate, int64_t gate_stride, int32_t gate_kind,
+    const void *total, int64_t total_stride, int32_t residual_type,
+    const float *scale, const void *weight, int32_t weight_type,
+    const float *rstd, void *grad_in, int64_t grad_in_stride, void *grad_gate,
+    int64_t grad_gate_stride, void *grad_residual,
+    int64_t grad_residual_stride, void *grad_input_weight, void *grad_weight,
+    int32_t accumulate, void *temp, int64_t temp_bytes);
+
+/* One step of AdamW over lists of `count` tensors, in place: for every element
+ *   g = f * gradient,  m = beta1 * m + (1 - beta1) * g,  v = beta2 * v + (1 - beta2) * g^2
+ *   p = p - r * (m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + epsilon) + weight_decay * p)
+ * t = step[0] (int64, DEVICE memory, 1 for the first step; the caller counts it on),
+ * r = rate * schedule[0] (float32, DEVICE memory; NULL: 1), so that a captured step
+ * goes on counting when it is replayed.  norm (float32, DEVICE memory, as
+ * ilgpu_hip_gradient_norm leaves it; NULL: f = 1): f is max_norm / norm[0] where that
+ * is less than 1, else 1; where norm[0] is infinite or NaN nothing at all is changed.
+ * parameters[k], gradients[k] and copies[k] (copies NULL: none) have the same length
+ * and each its type, F32, F16 or BF16; copies receive p too, rounded to their own
+ * type.
+ * Moments in 32 bits (first_scales and second_scales NULL): first[k] and second[k]
+ * are F32 of the same length, zeros before the first step.
+ * Moments in 8 bits: first[k] and second[k] are U8 of the same length, and
+ * first_scales[k] and second_scales[k] F32 with one element for every 256 of it (the
+ * last may stand for fewer), the largest |m| and v among them; all zeros before the first step.  A code c
+ * of the first stands for s * q * |q| / 127^2 with q = c - 128, of the second for
+ * s * c^4 / 255^4, s the scale.  p is computed from m and v before they are rounded.
+ * They are rounded up or down so that they are right in the mean, which lets moments
+ * move that change by less than a code's distance in a step: with u a number in
+ * [0, 1) from a hash of (seed, t, k, index), the code below the value is raised by
+ * one where the value is more than u of the way to the next.  (Where the largest of a
+ * block is below 1e-27 the second moments lose digits, below the normal float32
+ * numbers a block is stored as zeros; a gradient that is not finite, without a norm,
+ * spoils the moments of its 256.)  m and v are made by products and sums rounded to
+ * float32 one by one, so that codes are the same wherever they are computed so.
+ * Nothing that is written overlaps anything else.  Tensors of length 0 are skipped. */
+typedef struct ilgpu_hip_adamw_options {
+  double rate;         /* not negative, finite */
+  double beta1, beta2; /* [0, 1) */
+  double epsilon;      /* a positive normal float32 */
+  double weight_decay; /* not negative, finite */
+  double max_norm;     /* not negative, not NaN; used with norm */
+  int64_t seed;        /* of 8-bit moments */
+} ilgpu_hip_adamw_options;
+int32_t ilgpu_hip_adamw(ilgpu_hip_stream_t stream,
+                        const ilgpu_hip_tensor *parameters,
+                        const ilgpu_hip_tensor *gradients,
+                        const ilgpu_hip_tensor *first,
+                        const ilgpu_hip_tensor *second,
+                        const ilgpu_hip_tensor *first_scales,
+                        const ilgpu_hip_tensor *second_scales,
+                        const ilgpu_hip_tensor *copies, int64_t count,
+                        const ilgpu_hip_adamw_options *options,
+                        const int64_t *step, const float *schedule,
+                        const float *norm);
+
+/* 8-bit moments as the numbers they stand for, into tensors of the same lengths
+ * (F32, F16 or BF16).  first, first_scales and first_targets may be NULL together,
+ * as may be the second's three; not all six. */
+int32_t ilgpu_hip_adamw_moments(ilgpu_hip_stream_t stream,
+                                const ilgpu_hip_tensor *first,
+                                const ilgpu_hip_tensor *first_scales,
+                                const ilgpu_hip_tensor *first_targets,
+                                const ilgpu_hip_tensor *second,
+                                const ilgpu_hip_tensor *second_scales,
+                                const ilgpu_hip_tensor *second_targets,
+                                int64_t count);
+
 #ifdef __cplusplus
 }
 #endif
