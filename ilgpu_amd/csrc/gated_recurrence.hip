@@ -59,11 +59,12 @@ __device__ __forceinline__ float apply(Map m, float h) {
 }
 
 // a and 1 - a of a gate, each to some units in its last place.
-template <bool SIGMOID> __device__ __forceinline__ void decay_of(float gate, float& a, float& left) {
+template <typename T, bool SIGMOID>
+__device__ __forceinline__ void decay_of(float gate, float& a, float& left) {
   if constexpr (SIGMOID) {
-    logistic(gate, a, left);
+    logistic<T>(gate, a, left);
   } else {
-    a = exp_of(gate);
+    a = exp_of<T>(gate);
     // Near 0, where the difference has lost its bits, 1 - exp by its series (off by 2e-8 at most).
     const float series =
         -gate * fmaf(gate * (1.0f / 2), fmaf(gate * (1.0f / 3), fmaf(gate * (1.0f / 4), fmaf(gate * (1.0f / 5), fmaf(
@@ -83,25 +84,39 @@ struct Sequences {
   }
 };
 
-// The sequence that begins, and that ends, in each row of a tile, or -1; called by the whole
-// block, ends with a barrier.  Rows [*from, *to) belong to sequences.
-template <int ROWS>
+// Where sequences begin and end in a tile: a bit for each row of a row group, in the order of the
+// scan, and the sequence for each row that has one.
+template <int GROUPS, int ROWS> struct Marks {
+  uint32_t begin_bits[GROUPS], end_bits[GROUPS];
+  int32_t begins[GROUPS * ROWS], ends[GROUPS * ROWS];
+};
+
+// Marks the rows of the tile from `first` on; called by the whole block.  Rows [*from, *to) belong to
+// sequences.  (Offsets that are none put marks in wrong rows of the tile, but in none outside.)
+template <bool BACK, int GROUPS, int ROWS>
 __device__ __forceinline__ void mark_rows(const Sequences& s, int64_t first, int64_t rows,
-                                          int32_t* begins, int32_t* ends, int64_t* from,
-                                          int64_t* to) {
+                                          Marks<GROUPS, ROWS>& marks, int64_t* from, int64_t* to) {
+  constexpr int kTileRows = GROUPS * ROWS;
+  if (threadIdx.x < GROUPS) marks.begin_bits[threadIdx.x] = marks.end_bits[threadIdx.x] = 0;
+  const auto mark = [&](uint32_t* bits, int32_t* sequences, int row, int64_t sequence) {
+    const int i = BACK ? kTileRows - 1 - row : row;
+    sequences[row] = (int32_t)sequence;
+    atomicOr(&bits[i / ROWS], 1u << (i % ROWS));
+  };
   if (s.offsets == nullptr) {
-    for (int i = threadIdx.x; i < ROWS; i += kBlock) {
-      const uint32_t row = (uint32_t)first + i;
-      const bool in = row < (uint64_t)rows;
-      begins[i] = in && row % s.length == 0 ? (int32_t)(row / s.length) : -1;
-      ends[i] = in && (row + 1) % s.length == 0 ? (int32_t)(row / s.length) : -1;
+    __syncthreads();
+    const uint32_t before = (uint32_t)first / s.length;
+    for (int64_t j = before + threadIdx.x; j <= s.count; j += kBlock) {
+      const int64_t row = j * s.length - first;
+      if (row > kTileRows) break;
+      if (row >= 0 && row < kTileRows && j < s.count) mark(marks.begin_bits, marks.begins, (int)row, j);
+      if (row > 0) mark(marks.end_bits, marks.ends, (int)row - 1, j - 1);
     }
     *from = 0;
     *to = rows;
     __syncthreads();
     return;
   }
-  for (int i = threadIdx.x; i < ROWS; i += kBlock) begins[i] = ends[i] = -1;
   // The first offset that is not below `first` lies in [at, at + left].
   int64_t at = 0, left = s.count + 1;
   while (left > kBlock) {
@@ -111,16 +126,17 @@ __device__ __forceinline__ void mark_rows(const Sequences& s, int64_t first, int
     if (below > 0) at += (below - 1) * step;
     left = step < end - at ? step : end - at;
   }
-  __syncthreads();
-  for (int64_t j = at + threadIdx.x; j <= s.count; j += kBlock) {
-    const int64_t o = s.offset(j), row = o - first;
-    if (row > ROWS) break;
-    if (row >= 0 && row < ROWS && j < s.count && s.offset(j + 1) > o) begins[row] = (int32_t)j;
-    if (row > 0 && j > 0 && s.offset(j - 1) < o) ends[row - 1] = (int32_t)(j - 1);
-  }
   const int64_t low = s.offset(0), high = s.offset(s.count);
   *from = low > 0 ? low : 0;
   *to = high < rows ? high : rows;
+  __syncthreads();
+  for (int64_t j = at + threadIdx.x; j <= s.count; j += kBlock) {
+    const int64_t o = s.offset(j), row = o - first;
+    if (row > kTileRows) break;
+    if (row >= 0 && row < kTileRows && j < s.count && s.offset(j + 1) > o)
+      mark(marks.begin_bits, marks.begins, (int)row, j);
+    if (row > 0 && j > 0 && s.offset(j - 1) < o) mark(marks.end_bits, marks.ends, (int)row - 1, j - 1);
+  }
   __syncthreads();
 }
 
@@ -206,8 +222,8 @@ __device__ __forceinline__ float look_back(const Scan& s, int64_t tile, uint32_t
   return h;
 }
 
-template <typename T, int W, int R, bool BACK, bool SIGMOID>
-__global__ __launch_bounds__(kBlock) void recurrence_kernel(Scan s) {
+template <typename T, int W, int R, bool BACK, bool SIGMOID, bool COMPLEMENT>
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void recurrence_kernel(Scan s) {
   constexpr int kGroups = groups_of<W>(), kTileRows = kGroups * R, kLanes = kTileChannels / W;
   constexpr int kWaveGroups = kGroups / kWaves;
   using V = typename Pack<T, W>::vec;
@@ -215,7 +231,7 @@ __global__ __launch_bounds__(kBlock) void recurrence_kernel(Scan s) {
   __shared__ Map maps[kGroups][kTileChannels];
   __shared__ Map wave_maps[kWaves][kTileChannels];
   __shared__ float wave_states[kWaves][kTileChannels];
-  __shared__ int32_t begins[kTileRows], ends[kTileRows];
+  __shared__ Marks<kGroups, R> marks;
   __shared__ uint32_t ticket;
 
   const uint32_t column = (uint32_t)((s.first_block + blockIdx.x) % s.columns_of_tiles);
@@ -225,7 +241,7 @@ __global__ __launch_bounds__(kBlock) void recurrence_kernel(Scan s) {
       ticket = __hip_atomic_fetch_add(s.tickets + column * (kTicketBytes / 4), 1u,
                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    tile = ticket;
+    tile = __builtin_amdgcn_readfirstlane(ticket);
     if (tile >= s.tiles) return;
   }
   const int64_t first = (BACK ? s.tiles - 1 - tile : tile) * kTileRows;
@@ -235,78 +251,107 @@ __global__ __launch_bounds__(kBlock) void recurrence_kernel(Scan s) {
   const int64_t c = (int64_t)column * kTileChannels + lane * W;
   const int64_t at = c + W <= s.channels ? c : s.channels - W;
   const int skip = (int)(c - at < W ? c - at : W);
-  // Its rows, in the order of the scan.
-  const auto row_in_tile = [&](int r) {
-    return BACK ? kTileRows - 1 - (group * R + r) : group * R + r;
-  };
-  const auto row_to_read = [&](int r) {
-    const int64_t row = first + row_in_tile(r);
-    return row < s.rows ? row : s.rows - 1;
-  };
+  // Its rows, in the order of the scan: the r-th is `origin` + r steps.
+  constexpr int kStep = BACK ? -1 : 1;
+  const int place = BACK ? kTileRows - 1 - group * R : group * R;  // of the first in the tile
+  const int64_t origin = first + place;
   V gate[R], in[R], grad[BACK ? R : 1], before[BACK ? R : 1];
+  if (first + kTileRows <= s.rows && (!BACK || first > 0)) {
+    const T* gates = static_cast<const T*>(s.gate) + origin * s.gate_stride + at;
+    const T* ins = static_cast<const T*>(s.in) + origin * s.in_stride + at;
+    const T* grads = static_cast<const T*>(s.grad_out) + origin * s.grad_out_stride + at;
+    const T* states = static_cast<const T*>(s.states) + (origin - 1) * s.states_stride + at;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int64_t row = row_to_read(r);
-    gate[r] = *reinterpret_cast<const P*>(static_cast<const T*>(s.gate) + row * s.gate_stride + at);
-    in[r] = *reinterpret_cast<const P*>(static_cast<const T*>(s.in) + row * s.in_stride + at);
-    if constexpr (BACK) {
-      grad[r] = *reinterpret_cast<const P*>(static_cast<const T*>(s.grad_out) +
-                                            row * s.grad_out_stride + at);
-      before[r] = *reinterpret_cast<const P*>(static_cast<const T*>(s.states) +
-                                              (row > 0 ? row - 1 : 0) * s.states_stride + at);
+    for (int r = 0; r < R; ++r) {
+      gate[r] = *reinterpret_cast<const P*>(gates + kStep * r * s.gate_stride);
+      in[r] = *reinterpret_cast<const P*>(ins + kStep * r * s.in_stride);
+      if constexpr (BACK) {
+        grad[r] = *reinterpret_cast<const P*>(grads + kStep * r * s.grad_out_stride);
+        before[r] = *reinterpret_cast<const P*>(states + kStep * r * s.states_stride);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      int64_t row = origin + kStep * r;
+      row = row < s.rows ? row : s.rows - 1;
+      gate[r] = *reinterpret_cast<const P*>(static_cast<const T*>(s.gate) + row * s.gate_stride + at);
+      in[r] = *reinterpret_cast<const P*>(static_cast<const T*>(s.in) + row * s.in_stride + at);
+      if constexpr (BACK) {
+        grad[r] = *reinterpret_cast<const P*>(static_cast<const T*>(s.grad_out) +
+                                              row * s.grad_out_stride + at);
+        before[r] = *reinterpret_cast<const P*>(static_cast<const T*>(s.states) +
+                                                (row > 0 ? row - 1 : 0) * s.states_stride + at);
+      }
     }
   }
   int64_t from, to;
-  mark_rows<kTileRows>(s.sequences, first, s.rows, begins, ends, &from, &to);
-  // Rows that forget what comes in, and rows of a sequence, a bit each.
-  uint32_t resets = 0, there = 0;
+  mark_rows<BACK>(s.sequences, first, s.rows, marks, &from, &to);
+  // A bit a row: rows of sequences, rows that forget what comes in, and rows whose state is left.
+  constexpr uint32_t kAll = R == 32 ? ~0u : (1u << R) - 1u;
+  uint32_t there = kAll;
+  if (first < from || first + kTileRows > to) {
+    there = 0;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int i = row_in_tile(r);
-    if (first + i >= from && first + i < to) there |= 1u << r;
-    if ((BACK ? ends : begins)[i] >= 0) resets |= 1u << r;
+    for (int r = 0; r < R; ++r)
+      if (origin + kStep * r >= from && origin + kStep * r < to) there |= 1u << r;
   }
-  resets &= there;
+  const uint32_t resets = (BACK ? marks.end_bits : marks.begin_bits)[group] & there;
+  const uint32_t lasts = (BACK ? marks.begin_bits : marks.end_bits)[group] & there;
+  const int32_t* reset_of = (BACK ? marks.ends : marks.begins) + place;
+  const int32_t* last_of = (BACK ? marks.begins : marks.ends) + place;
+  // Most waves have none of these, and go without what they ask for.
+  const bool special = __any((resets | lasts | (there ^ kAll)) != 0);
 
   float a[R][W], left[BACK ? R : 1][W], b[R][W];
-  Map own[W];
-#pragma unroll
-  for (int k = 0; k < W; ++k) own[k] = Map{1.0f, 0.0f};
 #pragma unroll
   for (int r = 0; r < R; ++r) {
 #pragma unroll
     for (int k = 0; k < W; ++k) {
       float l;
-      decay_of<SIGMOID>((float)gate[r][k], a[r][k], l);
+      decay_of<T, SIGMOID>((float)gate[r][k], a[r][k], l);
       if constexpr (BACK) {
         left[r][k] = l;
         b[r][k] = (float)grad[r][k];
       } else {
-        b[r][k] = s.complement ? l * (float)in[r][k] : (float)in[r][k];
+        b[r][k] = COMPLEMENT ? l * (float)in[r][k] : (float)in[r][k];
       }
     }
-    if (resets >> r & 1u) {  // what the sequence begins with is a part of b
-      const float* state = BACK ? s.grad_final : s.initial;
-      if (state != nullptr) {
-        state += (BACK ? ends : begins)[row_in_tile(r)] *
-                     (BACK ? s.grad_final_stride : s.initial_stride) + at;
+  }
+  Map own[W];
 #pragma unroll
-        for (int k = 0; k < W; ++k) b[r][k] = BACK ? b[r][k] + state[k] : fmaf(a[r][k], state[k], b[r][k]);
-      }
-    }
-    if (!(there >> r & 1u)) {
-#pragma unroll
-      for (int k = 0; k < W; ++k) {
-        a[r][k] = 1.0f;
-        b[r][k] = 0.0f;
-      }
-    }
+  for (int k = 0; k < W; ++k) own[k] = Map{1.0f, 0.0f};
+  const auto fold = [&](int r) {
 #pragma unroll
     for (int k = 0; k < W; ++k) {
-      const float h = resets >> r & 1u ? 0.0f : own[k].b;
-      own[k].b = BACK ? a[r][k] * (b[r][k] + h) : fmaf(a[r][k], h, b[r][k]);
+      own[k].b = BACK ? a[r][k] * (b[r][k] + own[k].b) : fmaf(a[r][k], own[k].b, b[r][k]);
       own[k].a *= a[r][k];
     }
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (special) {
+      asm volatile("");  // (a branch: as selects, all rows would pay for it)
+      if (resets >> r & 1u) {  // what the sequence begins with is a part of b
+        const float* state = BACK ? s.grad_final : s.initial;
+        if (state != nullptr) {
+          state += reset_of[kStep * r] * (BACK ? s.grad_final_stride : s.initial_stride) + at;
+#pragma unroll
+          for (int k = 0; k < W; ++k)
+            b[r][k] = BACK ? b[r][k] + state[k] : fmaf(a[r][k], state[k], b[r][k]);
+        }
+#pragma unroll
+        for (int k = 0; k < W; ++k) own[k].b = 0.0f;
+      }
+      if (!(there >> r & 1u)) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+          a[r][k] = 1.0f;
+          b[r][k] = 0.0f;
+        }
+      }
+    }
+    fold(r);
   }
   if (resets != 0) {
 #pragma unroll
@@ -343,9 +388,10 @@ __global__ __launch_bounds__(kBlock) void recurrence_kernel(Scan s) {
   for (int k = 0; k < W; ++k)
     h[k] = apply(maps[group][lane * W + k], wave_states[wave][lane * W + k]);
 
-  const auto store = [&](void* to_, int64_t stride, int64_t row, const float (&v)[W]) {
-    T* p = static_cast<T*>(to_) + row * stride + at;
-    if (skip == 0) {
+  const bool whole = s.channels % W == 0;
+  const auto store = [&](void* to_, int64_t stride, int r, const float (&v)[W]) {
+    T* p = static_cast<T*>(to_) + origin * stride + at + kStep * r * stride;
+    if (whole || skip == 0) {
       V packed;
 #pragma unroll
       for (int k = 0; k < W; ++k) packed[k] = (T)v[k];
@@ -356,41 +402,55 @@ __global__ __launch_bounds__(kBlock) void recurrence_kernel(Scan s) {
         if (k >= skip) p[k] = (T)v[k];
     }
   };
+  if (skip < W) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int i = row_in_tile(r);
-    const int64_t row = first + i;
-    if (!(there >> r & 1u)) continue;
-    if constexpr (!BACK) {
+    for (int r = 0; r < R; ++r) {
+      if (special) {
+        asm volatile("");
+        if (resets >> r & 1u) {
 #pragma unroll
-      for (int k = 0; k < W; ++k) h[k] = fmaf(a[r][k], resets >> r & 1u ? 0.0f : h[k], b[r][k]);
-      store(s.out, s.out_stride, row, h);
-    } else {
-      float reaches[W], of_gate[W], of_in[W], state[W];
-#pragma unroll
-      for (int k = 0; k < W; ++k) state[k] = (float)before[r][k];
-      if (begins[i] >= 0) {
-#pragma unroll
-        for (int k = 0; k < W; ++k)
-          state[k] = s.initial != nullptr ? s.initial[begins[i] * s.initial_stride + at + k] : 0.0f;
+          for (int k = 0; k < W; ++k) h[k] = 0.0f;
+        }
       }
+      const bool mine = !special || (there >> r & 1u) != 0;
+      if constexpr (!BACK) {
 #pragma unroll
-      for (int k = 0; k < W; ++k) {
-        reaches[k] = b[r][k] + (resets >> r & 1u ? 0.0f : h[k]);
-        h[k] = a[r][k] * reaches[k];
-        const float slope = SIGMOID ? a[r][k] * left[r][k] : a[r][k];
-        of_gate[k] = reaches[k] * (s.complement ? state[k] - (float)in[r][k] : state[k]) * slope;
-        of_in[k] = s.complement ? reaches[k] * left[r][k] : reaches[k];
+        for (int k = 0; k < W; ++k) h[k] = fmaf(a[r][k], h[k], b[r][k]);
+        if (mine) store(s.out, s.out_stride, r, h);
+      } else {
+        float of_gate[W], of_in[W], state[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) state[k] = (float)before[r][k];
+        if (special) {
+          asm volatile("");
+          if (lasts >> r & 1u) {
+#pragma unroll
+            for (int k = 0; k < W; ++k)
+              state[k] = s.initial != nullptr
+                             ? s.initial[last_of[kStep * r] * s.initial_stride + at + k] : 0.0f;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+          const float reaches = b[r][k] + h[k];
+          h[k] = a[r][k] * reaches;
+          of_in[k] = COMPLEMENT ? reaches * left[r][k] : reaches;
+          // (a G is the state that goes on; its slope has 1 - a for the other factor.)
+          const float of_decay = COMPLEMENT ? state[k] - (float)in[r][k] : state[k];
+          of_gate[k] = SIGMOID ? h[k] * left[r][k] * of_decay : h[k] * of_decay;
+        }
+        if (mine && s.out != nullptr) store(s.out, s.out_stride, r, of_gate);
+        if (mine && s.grad_in != nullptr) store(s.grad_in, s.grad_in_stride, r, of_in);
       }
-      if (s.out != nullptr) store(s.out, s.out_stride, row, of_gate);
-      if (s.grad_in != nullptr) store(s.grad_in, s.grad_in_stride, row, of_in);
-    }
-    const int32_t last = (BACK ? begins : ends)[i];
-    if (s.last != nullptr && last >= 0) {
-      float* p = s.last + last * s.last_stride + at;
+      if (special) {
+        asm volatile("");
+        if ((lasts >> r & 1u) != 0 && s.last != nullptr) {
+          float* p = s.last + last_of[kStep * r] * s.last_stride + at;
 #pragma unroll
-      for (int k = 0; k < W; ++k)
-        if (k >= skip) p[k] = h[k];
+          for (int k = 0; k < W; ++k)
+            if (k >= skip) p[k] = h[k];
+        }
+      }
     }
   }
   // Sequences without rows leave what they begin with.
@@ -423,7 +483,7 @@ __global__ __launch_bounds__(kBlock) void recurrence_step_kernel(Scan s) {
 #pragma unroll
     for (int k = 0; k < W; ++k) {
       float a, left;
-      decay_of<SIGMOID>(gate[k], a, left);
+      decay_of<T, SIGMOID>(gate[k], a, left);
       h[k] = fmaf(a, h[k], s.complement ? left * in[k] : in[k]);
     }
     store_floats<T, W>(static_cast<T*>(s.out) + row * s.out_stride + c, h, count);
@@ -449,7 +509,7 @@ inline unsigned blocks_for_elements(int64_t threads) {
 
 inline int64_t columns_of_tiles(int64_t channels) { return div_up(channels, kTileChannels); }
 
-template <typename T, int W, int R, bool BACK, bool SIGMOID>
+template <typename T, int W, int R, bool BACK, bool SIGMOID, bool COMPLEMENT>
 int32_t launch_scan_tiles(hipStream_t stream, Scan s, void* temp) {
   s.tiles = div_up(s.rows, (int64_t)groups_of<W>() * R);
   s.columns_of_tiles = (uint32_t)columns_of_tiles(s.channels);
@@ -467,7 +527,7 @@ int32_t launch_scan_tiles(hipStream_t stream, Scan s, void* temp) {
     const int64_t left = blocks - s.first_block;
     {
       ProfileScope scope(stream, BACK ? "recurrence_gradient" : "recurrence");
-      hipLaunchKernelGGL((recurrence_kernel<T, W, R, BACK, SIGMOID>),
+      hipLaunchKernelGGL((recurrence_kernel<T, W, R, BACK, SIGMOID, COMPLEMENT>),
                          dim3((unsigned)(left < kMostBlocks ? left : kMostBlocks)), dim3(kBlock), 0,
                          stream, s);
     }
@@ -476,7 +536,7 @@ int32_t launch_scan_tiles(hipStream_t stream, Scan s, void* temp) {
   return ILGPU_HIP_SUCCESS;
 }
 
-template <bool BACK, bool SIGMOID>
+template <bool BACK, bool SIGMOID, bool COMPLEMENT>
 int32_t launch_scan_of(hipStream_t stream, int32_t type, const Scan& s, void* temp) {
   return with_type(type, [&](auto t) -> int32_t {
     using T = decltype(t);
@@ -492,8 +552,8 @@ int32_t launch_scan_of(hipStream_t stream, int32_t type, const Scan& s, void* te
       return ILGPU_HIP_SUCCESS;
     }
     // (A row shorter than a vector: an element a thread.)
-    if (s.channels < W) return launch_scan_tiles<T, 1, R, BACK, SIGMOID>(stream, s, temp);
-    return launch_scan_tiles<T, W, R, BACK, SIGMOID>(stream, s, temp);
+    if (s.channels < W) return launch_scan_tiles<T, 1, R, BACK, SIGMOID, COMPLEMENT>(stream, s, temp);
+    return launch_scan_tiles<T, W, R, BACK, SIGMOID, COMPLEMENT>(stream, s, temp);
   });
 }
 
@@ -512,8 +572,11 @@ int32_t launch_scan(hipStream_t stream, int32_t type, int32_t decay, const Scan&
     ILGPU_HIP_CHECK(hipGetLastError());
     return ILGPU_HIP_SUCCESS;
   }
-  return decay == ILGPU_HIP_DECAY_SIGMOID ? launch_scan_of<BACK, true>(stream, type, s, temp)
-                                          : launch_scan_of<BACK, false>(stream, type, s, temp);
+  if (decay == ILGPU_HIP_DECAY_SIGMOID)
+    return s.complement ? launch_scan_of<BACK, true, true>(stream, type, s, temp)
+                        : launch_scan_of<BACK, true, false>(stream, type, s, temp);
+  return s.complement ? launch_scan_of<BACK, false, true>(stream, type, s, temp)
+                      : launch_scan_of<BACK, false, false>(stream, type, s, temp);
 }
 
 }  // namespace

@@ -5,24 +5,29 @@
 
 namespace ilgpu_hip {
 
-// exp(x) to about a unit in the last place: of x / ln 2 the part that the product rounds off is
-// put right behind the hardware's 2^x.
-__device__ __forceinline__ float exp_of(float x) {
-  constexpr float kLog2E = 1.44269504f, kLog2ELow = 1.92596299e-8f;  // log2(e) in two parts
-  x = x < -150.0f ? -150.0f : x;  // (a NaN stays one)
-  x = x > 150.0f ? 150.0f : x;
-  const float t = x * kLog2E;
-  const float rest = fmaf(x, kLog2ELow, fmaf(x, kLog2E, -t));
-  return __builtin_amdgcn_exp2f(t) * fmaf(rest, 0.693147181f, 1.0f);
+// 2^(x / ln 2) of an x that was a T.  The product's rounding is that of its size, x / ln 2 units in
+// the result's last place: of a float it is put right, of the 16-bit types, whose own last place
+// is thousands of times that, it is not.  FINITE: below 2^126, so that its reciprocal is a normal number.
+template <typename T, bool FINITE> __device__ __forceinline__ float power_of_e(float x) {
+  constexpr float kLog2E = 1.44269504f;
+  const float raw = x * kLog2E, t = FINITE && raw > 125.0f ? 125.0f : raw;  // (a NaN stays one)
+  const float e = __builtin_amdgcn_exp2f(t);
+  if constexpr (!std::is_same<T, float>::value) return e;
+  // (Where t was held back, or is infinite, the rest says nothing, and is held to 1.)
+  const float rest = __builtin_amdgcn_fmed3f(fmaf(x, kLog2E, -t), -1.0f, 1.0f);
+  return e * fmaf(rest, 0.693147181f, 1.0f);
 }
 
-// The logistic function of x and what is left of it to 1, each to some units in its last place: of
-// exp(-|x|), which does not overflow, the larger and the smaller of the two.
-__device__ __forceinline__ void logistic(float x, float& value, float& left) {
-  const float e = exp_of(-fabsf(x));
-  const float larger = __builtin_amdgcn_rcpf(1.0f + e), smaller = e * larger;
-  value = x >= 0.0f ? larger : smaller;
-  left = x >= 0.0f ? smaller : larger;
+// The logistic function of x and what is left of it to 1: 1 / (1 + e) and e / (1 + e) with
+// e = exp(-x), each with its own digits.
+template <typename T> __device__ __forceinline__ void logistic(float x, float& value, float& left) {
+  const float e = power_of_e<T, true>(-x);
+  value = __builtin_amdgcn_rcpf(1.0f + e);
+  left = e * value;
+}
+
+template <typename T> __device__ __forceinline__ float exp_of(float x) {
+  return power_of_e<T, false>(x);
 }
 
 }  // namespace ilgpu_hip

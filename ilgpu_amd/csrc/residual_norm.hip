@@ -17,23 +17,25 @@ namespace {
 constexpr int64_t kMaxBlocks = 1 << 22;
 constexpr int kLongBlock = kWholeBlock;
 
-// act(gate), and its slope.
-__device__ __forceinline__ float activation(float gate, int32_t kind) {
+// act(gate), and its slope.  Beyond kFar what is left is below the normal numbers: an infinite gate
+// is shut, or open, although infinity times 0 is no number.
+constexpr float kFar = 87.0f;
+template <typename T> __device__ __forceinline__ float activation(float gate, int32_t kind) {
   float s, left;
-  logistic(gate, s, left);
-  // (A gate of minus infinity is shut, although infinity times 0 is no number.)
-  return kind == ILGPU_HIP_GATE_SIGMOID ? s : s == 0.0f ? 0.0f : gate * s;
+  logistic<T>(gate, s, left);
+  return kind == ILGPU_HIP_GATE_SIGMOID ? s : gate < -kFar ? 0.0f : gate * s;
 }
+template <typename T>
 __device__ __forceinline__ float activation(float gate, int32_t kind, float& slope) {
   float s, left;
-  logistic(gate, s, left);
+  logistic<T>(gate, s, left);
   const float both = s * left;
   if (kind == ILGPU_HIP_GATE_SIGMOID) {
     slope = both;
     return s;
   }
-  slope = both == 0.0f ? s : fmaf(gate, both, s);
-  return s == 0.0f ? 0.0f : gate * s;
+  slope = fabsf(gate) > kFar ? s : fmaf(gate, both, s);
+  return gate < -kFar ? 0.0f : gate * s;
 }
 
 template <int W, int LANES, int V, typename T>
@@ -83,7 +85,7 @@ __global__ __launch_bounds__(row_block<LANES>()) void residual_norm_kernel(Resid
 #pragma unroll
       for (int k = 0; k < W; ++k) {
         x[v][k] = (float)next_x[v][k];
-        y[v][k] = a.gate != nullptr ? activation((float)next_gate[v][k], a.gate_kind) : 1.0f;
+        y[v][k] = a.gate != nullptr ? activation<T>((float)next_gate[v][k], a.gate_kind) : 1.0f;
       }
     float r[V][W];
 #pragma unroll
@@ -177,7 +179,7 @@ __global__ __launch_bounds__(kLongBlock) void residual_norm_long_kernel(Residual
         float gate[W];
         load_floats<T, W>(gate, row_of<T>(a.gate, row, a.gate_stride) + c, count);
 #pragma unroll
-        for (int k = 0; k < W; ++k) x[k] *= activation(gate[k], a.gate_kind);
+        for (int k = 0; k < W; ++k) x[k] *= activation<T>(gate[k], a.gate_kind);
       }
       float r[W];
 #pragma unroll
@@ -304,7 +306,7 @@ __global__ __launch_bounds__(BLOCK) void residual_norm_gradient_kernel(
 #pragma unroll
         for (int k = 0; k < W; ++k) {
           float slope;
-          const float open = activation(gate[v][k], a.gate_kind, slope);
+          const float open = activation<T>(gate[v][k], a.gate_kind, slope);
           gate[v][k] = d[v][k] * (x[v][k] * input_w[v][k]) * slope;
           d[v][k] *= open;
         }
@@ -399,7 +401,7 @@ template <typename T, typename TR, int W> struct LongRow {
 #pragma unroll
     for (int k = 0; k < W; ++k) {
       float slope;
-      const float open = activation(gate[k], a.gate_kind, slope);
+      const float open = activation<T>(gate[k], a.gate_kind, slope);
       of_gate[k] = d[k] * (x[k] * input_w[k]) * slope;
       d[k] *= open;
     }
