@@ -23,7 +23,7 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kWaves = kBlock / kWaveSize;
 constexpr int kTileChannels = kWaveSize;  // a wave's lanes walk back, a channel each
-constexpr int kWindow = 8;                // tiles that a look-back asks at a time
+constexpr int kWindow = 4;                // tiles that a look-back asks at a time
 constexpr uint32_t kMostPolls = 1 << 24;  // of a look-back: many seconds
 constexpr int64_t kMostBlocks = 1 << 22;  // of a launch
 
@@ -70,6 +70,25 @@ __device__ __forceinline__ void decay_of(float gate, float& a, float& left) {
         -gate * fmaf(gate * (1.0f / 2), fmaf(gate * (1.0f / 3), fmaf(gate * (1.0f / 4), fmaf(gate * (1.0f / 5), fmaf(
         gate * (1.0f / 6), fmaf(gate, 1.0f / 7, 1.0f), 1.0f), 1.0f), 1.0f), 1.0f), 1.0f);
     left = fabsf(gate) < 0.35f ? series : 1.0f - a;
+  }
+}
+
+// Hides where a vector comes from, so that what is made of it is made anew.
+template <typename V> __device__ __forceinline__ void keep(V& v) {
+  if constexpr (sizeof(V) == 16) {
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    Words w = __builtin_bit_cast(Words, v);
+    asm volatile("" : "+v"(w));
+    v = __builtin_bit_cast(V, w);
+  } else if constexpr (sizeof(V) == 4) {
+    uint32_t w = __builtin_bit_cast(uint32_t, v);
+    asm volatile("" : "+v"(w));
+    v = __builtin_bit_cast(V, w);
+  } else {
+    static_assert(sizeof(V) == 2, "a vector of 16 bytes or one element");
+    uint32_t w = __builtin_bit_cast(uint16_t, v);
+    asm volatile("" : "+v"(w));
+    v = __builtin_bit_cast(V, (uint16_t)w);
   }
 }
 
@@ -222,8 +241,11 @@ __device__ __forceinline__ float look_back(const Scan& s, int64_t tile, uint32_t
   return h;
 }
 
+#ifndef ILGPU_HIP_RECURRENCE_WAVES
+#define ILGPU_HIP_RECURRENCE_WAVES 2
+#endif
 template <typename T, int W, int R, bool BACK, bool SIGMOID, bool COMPLEMENT>
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) void recurrence_kernel(Scan s) {
+__global__ __launch_bounds__(kBlock, ILGPU_HIP_RECURRENCE_WAVES) void recurrence_kernel(Scan s) {
   constexpr int kGroups = groups_of<W>(), kTileRows = kGroups * R, kLanes = kTileChannels / W;
   constexpr int kWaveGroups = kGroups / kWaves;
   using V = typename Pack<T, W>::vec;
@@ -303,62 +325,80 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
   // Most waves have none of these, and go without what they ask for.
   const bool special = __any((resets | lasts | (there ^ kAll)) != 0);
 
-  float a[R][W], left[BACK ? R : 1][W], b[R][W];
+  // What sequences begin with, in the order of the scan.
+  const float* begin_state = BACK ? s.grad_final : s.initial;
+  const int64_t begin_stride = BACK ? s.grad_final_stride : s.initial_stride;
+  // Decays of the r-th row and what is left of them; its b (backwards: grad_out), of which what a sequence
+  // begins with is a part.
+  const auto decays = [&](int r, float (&a)[W], float (&left)[W]) {
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
+    for (int k = 0; k < W; ++k) decay_of<T, SIGMOID>((float)gate[r][k], a[k], left[k]);
+    if (!special) return;
+    asm volatile("");  // (a branch: as selects, all rows would pay for it)
+    if (!(there >> r & 1u)) {
 #pragma unroll
-    for (int k = 0; k < W; ++k) {
-      float l;
-      decay_of<T, SIGMOID>((float)gate[r][k], a[r][k], l);
-      if constexpr (BACK) {
-        left[r][k] = l;
-        b[r][k] = (float)grad[r][k];
-      } else {
-        b[r][k] = COMPLEMENT ? l * (float)in[r][k] : (float)in[r][k];
-      }
-    }
-  }
-  Map own[W];
-#pragma unroll
-  for (int k = 0; k < W; ++k) own[k] = Map{1.0f, 0.0f};
-  const auto fold = [&](int r) {
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-      own[k].b = BACK ? a[r][k] * (b[r][k] + own[k].b) : fmaf(a[r][k], own[k].b, b[r][k]);
-      own[k].a *= a[r][k];
+      for (int k = 0; k < W; ++k) a[k] = 1.0f;
     }
   };
+  const auto addends = [&](int r, const float (&a)[W], const float (&left)[W], float (&b)[W]) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      if (BACK) b[k] = (float)grad[BACK ? r : 0][k];
+      else b[k] = COMPLEMENT ? left[k] * (float)in[r][k] : (float)in[r][k];
+    }
+    if (!special) return;
+    asm volatile("");
+    if ((resets >> r & 1u) != 0 && begin_state != nullptr) {
+      float state[W];
+      load_floats<float, W>(state, begin_state + reset_of[kStep * r] * begin_stride + at, W);
+#pragma unroll
+      for (int k = 0; k < W; ++k) b[k] = BACK ? b[k] + state[k] : fmaf(a[k], state[k], b[k]);
+    }
+    if (!(there >> r & 1u)) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) b[k] = 0.0f;
+    }
+  };
+  // What comes in to the r-th row is forgotten where a sequence begins.
+  const auto forget = [&](int r, float (&h)[W]) {
+    if (!special) return;
+    asm volatile("");
+    if (resets >> r & 1u) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) h[k] = 0.0f;
+    }
+  };
+  // What is made of a row stays in registers until the state in front of the tile is known; backwards,
+  // where there is more of it, the decays are made again.  (b is not: what a sequence begins with may be
+  // written over by what it leaves, once this tile's map is known.)
+  constexpr int kHeld = BACK ? 1 : R;
+  float held_a[kHeld][W], b[R][W];
+  float own_a[W], h[W];
+#pragma unroll
+  for (int k = 0; k < W; ++k) {
+    own_a[k] = 1.0f;
+    h[k] = 0.0f;
+  }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    if (special) {
-      asm volatile("");  // (a branch: as selects, all rows would pay for it)
-      if (resets >> r & 1u) {  // what the sequence begins with is a part of b
-        const float* state = BACK ? s.grad_final : s.initial;
-        if (state != nullptr) {
-          state += reset_of[kStep * r] * (BACK ? s.grad_final_stride : s.initial_stride) + at;
+    float a[W], left[W];
+    decays(r, a, left);
+    addends(r, a, left, b[r]);
+    forget(r, h);
 #pragma unroll
-          for (int k = 0; k < W; ++k)
-            b[r][k] = BACK ? b[r][k] + state[k] : fmaf(a[r][k], state[k], b[r][k]);
-        }
-#pragma unroll
-        for (int k = 0; k < W; ++k) own[k].b = 0.0f;
-      }
-      if (!(there >> r & 1u)) {
-#pragma unroll
-        for (int k = 0; k < W; ++k) {
-          a[r][k] = 1.0f;
-          b[r][k] = 0.0f;
-        }
-      }
+    for (int k = 0; k < W; ++k) {
+      h[k] = BACK ? a[k] * (b[r][k] + h[k]) : fmaf(a[k], h[k], b[r][k]);
+      own_a[k] *= a[k];
+      if constexpr (!BACK) held_a[r][k] = a[k];
     }
-    fold(r);
-  }
-  if (resets != 0) {
-#pragma unroll
-    for (int k = 0; k < W; ++k) own[k].a = -0.0f;
+    if (BACK) __builtin_amdgcn_sched_barrier(0);  // (rows side by side take more registers)
   }
 #pragma unroll
-  for (int k = 0; k < W; ++k) maps[group][lane * W + k] = own[k];
+  for (int k = 0; k < W; ++k) maps[group][lane * W + k] = Map{resets != 0 ? -0.0f : own_a[k], h[k]};
+  if constexpr (BACK) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) keep(gate[r]);
+  }
   __syncthreads();
   // The maps in front of each group of a wave, then those in front of each wave.
   const int wave = threadIdx.x / kWaveSize, channel = threadIdx.x % kWaveSize;
@@ -375,15 +415,14 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
     Map all = wave_maps[0][channel];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) all = behind(wave_maps[w][channel], all);
-    float h = s.tickets != nullptr ? look_back(s, tile, column, all) : 0.0f;
+    float state = s.tickets != nullptr ? look_back(s, tile, column, all) : 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      wave_states[w][channel] = h;
-      h = apply(wave_maps[w][channel], h);
+      wave_states[w][channel] = state;
+      state = apply(wave_maps[w][channel], state);
     }
   }
   __syncthreads();
-  float h[W];
 #pragma unroll
   for (int k = 0; k < W; ++k)
     h[k] = apply(maps[group][lane * W + k], wave_states[wave][lane * W + k]);
@@ -395,7 +434,7 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
       V packed;
 #pragma unroll
       for (int k = 0; k < W; ++k) packed[k] = (T)v[k];
-      *reinterpret_cast<P*>(p) = packed;
+      __builtin_nontemporal_store(packed, reinterpret_cast<P*>(p));
     } else {
 #pragma unroll
       for (int k = 0; k < W; ++k)
@@ -405,19 +444,15 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
   if (skip < W) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (special) {
-        asm volatile("");
-        if (resets >> r & 1u) {
-#pragma unroll
-          for (int k = 0; k < W; ++k) h[k] = 0.0f;
-        }
-      }
       const bool mine = !special || (there >> r & 1u) != 0;
+      forget(r, h);
       if constexpr (!BACK) {
 #pragma unroll
-        for (int k = 0; k < W; ++k) h[k] = fmaf(a[r][k], h[k], b[r][k]);
+        for (int k = 0; k < W; ++k) h[k] = fmaf(held_a[r][k], h[k], b[r][k]);
         if (mine) store(s.out, s.out_stride, r, h);
       } else {
+        float a[W], left[W];
+        decays(r, a, left);
         float of_gate[W], of_in[W], state[W];
 #pragma unroll
         for (int k = 0; k < W; ++k) state[k] = (float)before[r][k];
@@ -433,15 +468,16 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
 #pragma unroll
         for (int k = 0; k < W; ++k) {
           const float reaches = b[r][k] + h[k];
-          h[k] = a[r][k] * reaches;
-          of_in[k] = COMPLEMENT ? reaches * left[r][k] : reaches;
+          h[k] = a[k] * reaches;
+          of_in[k] = COMPLEMENT ? reaches * left[k] : reaches;
           // (a G is the state that goes on; its slope has 1 - a for the other factor.)
           const float of_decay = COMPLEMENT ? state[k] - (float)in[r][k] : state[k];
-          of_gate[k] = SIGMOID ? h[k] * left[r][k] * of_decay : h[k] * of_decay;
+          of_gate[k] = SIGMOID ? h[k] * left[k] * of_decay : h[k] * of_decay;
         }
         if (mine && s.out != nullptr) store(s.out, s.out_stride, r, of_gate);
         if (mine && s.grad_in != nullptr) store(s.grad_in, s.grad_in_stride, r, of_in);
       }
+      if (BACK) __builtin_amdgcn_sched_barrier(0);
       if (special) {
         asm volatile("");
         if ((lasts >> r & 1u) != 0 && s.last != nullptr) {
@@ -455,13 +491,11 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(2))) voi
   }
   // Sequences without rows leave what they begin with.
   if (s.last == nullptr || s.sequences.offsets == nullptr) return;
-  const float* begin = BACK ? s.grad_final : s.initial;
-  const int64_t begin_stride = BACK ? s.grad_final_stride : s.initial_stride;
   for (int64_t i = tile * kBlock + threadIdx.x; i < s.sequences.count; i += s.tiles * kBlock) {
     if (s.sequences.offset(i + 1) > s.sequences.offset(i)) continue;
     for (int64_t k = (int64_t)column * kTileChannels;
          k < s.channels && k < (int64_t)(column + 1) * kTileChannels; ++k)
-      s.last[i * s.last_stride + k] = begin != nullptr ? begin[i * begin_stride + k] : 0.0f;
+      s.last[i * s.last_stride + k] = begin_state != nullptr ? begin_state[i * begin_stride + k] : 0.0f;
   }
 }
 
