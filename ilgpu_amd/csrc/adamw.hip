@@ -22,8 +22,12 @@ constexpr int kBlock = 256;
 constexpr int kW = 4;                         // elements of a thread side by side
 static_assert(kW * kWaveSize == kMomentBlock, "a wave has the moments of one scale");
 constexpr int kTurn = kBlock * kW;            // elements of a block at a time
-constexpr int kTurns = 4;
-constexpr int kChunk = kTurns * kTurn;
+// Turns of a chunk, all of whose loads are on their way together.
+constexpr int kShortTurns = 2, kLongTurns = 4;
+constexpr int64_t kLongFrom = 1 << 22;        // elements of a list from which 32 bits take long chunks
+constexpr int kBlocksPerCu = 40;              // of 8 bits: each makes a table of powers
+constexpr int kReadTurns = 4;
+constexpr int kReadChunk = kReadTurns * kTurn;
 constexpr int kTensors = 46;                  // per launch
 constexpr int64_t kMaxBlocks = 1 << 22;
 
@@ -138,7 +142,8 @@ __device__ __forceinline__ void store_any(void* p, int32_t type, int64_t at, con
 // What is the same for all elements of a step.
 struct Step {
   float factor, back;                      // of the gradients, one after the other
-  float rate, inverse1, inverse2;          // r; 1 / (1 - beta^t)
+  float rate, keep;                        // r / (1 - beta1^t), 1 - r * weight_decay
+  float inverse2;                          // 1 / (1 - beta2^t)
   bool finite;
 };
 __device__ __forceinline__ Step step_of(const StepNumbers& n) {
@@ -156,10 +161,11 @@ __device__ __forceinline__ Step step_of(const StepNumbers& n) {
       s.back = tiny ? 0x1p-120f : 1.0f;
     }
   }
-  s.rate = n.schedule != nullptr ? n.rate * n.schedule[0] : n.rate;
+  const float rate = n.schedule != nullptr ? n.rate * n.schedule[0] : n.rate;
   const double t = (double)n.step[0];
-  s.inverse1 = 1.0f / -expm1f((float)(t * n.log_beta1));
+  s.rate = rate / -expm1f((float)(t * n.log_beta1));
   s.inverse2 = 1.0f / -expm1f((float)(t * n.log_beta2));
+  s.keep = fmaf(-rate, n.weight_decay, 1.0f);
   return s;
 }
 
@@ -174,8 +180,7 @@ __device__ __forceinline__ float stepped(const StepNumbers& n, const Step& s, fl
     v = n.keep2 * v + n.new2 * (g * g);
   }
   const float root = __builtin_amdgcn_sqrtf(v * s.inverse2) + n.epsilon;
-  const float along = m * s.inverse1 * __builtin_amdgcn_rcpf(root);
-  return p - s.rate * fmaf(n.weight_decay, p, along);
+  return fmaf(s.keep, p, -s.rate * m * __builtin_amdgcn_rcpf(root));
 }
 
 // A hash of a 32-bit number: xor-shifts and products with odd numbers (the first bits of the fractions of
@@ -229,34 +234,50 @@ __device__ __forceinline__ void fill_powers(Powers& powers) {
 
 // The code of a value that is not negative: the last whose value is not above it, or the next one
 // if `chance` / 2^16 of the way to it is less than the rest.  The share of the scale is a quotient rounded to
-// float32, everything behind it float64, in which its products with the powers are as good as
-// exact.  (The quotient by the reciprocal and one correction, which is right where the
-// reciprocal is the nearest.)
-constexpr float kSmallest = 0x1p-126f;
-__device__ __forceinline__ float share_of(float value, float scale, float inverse) {
-  const float q = value * inverse;
-  return fmaf(fmaf(-q, scale, value), inverse, q);
-}
-template <int POWER> __device__ __forceinline__ double power_of(float code) {
-  const double square = (double)(code * code);  // (exact in float32)
-  return POWER == 2 ? square : square * square;
-}
-template <int POWER> __device__ __forceinline__ uint32_t code_of(float share, uint32_t chance) {
-  constexpr float kLevels = POWER == 2 ? 127.0f : 255.0f;
-  const double z = (double)share * (POWER == 2 ? 127.0 * 127.0 : 255.0 * 255.0 * 255.0 * 255.0);
-  const double u = (double)chance * 0x1p-16;
-  float low = floorf(POWER == 2 ? __builtin_amdgcn_sqrtf((float)z)
-                                : __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)z)));
-  double below = power_of<POWER>(low), way = z - below;
-  double span = power_of<POWER>(low + 1.0f) - below;
-  if (way < 0.0 || way >= span) {  // (the root's roundings: rare)
-    low += way < 0.0 ? -1.0f : 1.0f;
-    below = power_of<POWER>(low);
-    way = z - below;
-    span = power_of<POWER>(low + 1.0f) - below;
+// float32, everything behind it exact (float64, in which the products with powers are as good as that).
+template <int POWER> struct Code {
+  static constexpr float kLevels = POWER == 2 ? 127.0f : 255.0f;
+  static constexpr double kAll = POWER == 2 ? 127.0 * 127.0 : 255.0 * 255.0 * 255.0 * 255.0;
+  static __device__ __forceinline__ double power(float code) {
+    const double square = (double)(code * code);  // (exact in float32)
+    return POWER == 2 ? square : square * square;
   }
-  return (uint32_t)fminf(low + (way > u * span ? 1.0f : 0.0f), kLevels);
-}
+  static __device__ __forceinline__ float root(float z) {
+    z = __builtin_amdgcn_sqrtf(z);
+    return POWER == 2 ? z : __builtin_amdgcn_sqrtf(z);
+  }
+  static __device__ float exactly(float value, float scale, uint32_t chance) {
+    const double z = (double)(value / scale) * kAll;
+    float low = floorf(root((float)z));
+    double below = power(low), way = z - below, span = power(low + 1.0f) - below;
+    if (way < 0.0 || way >= span) {  // (the root's roundings)
+      low += way < 0.0 ? -1.0f : 1.0f;
+      below = power(low);
+      way = z - below;
+      span = power(low + 1.0f) - below;
+    }
+    return fminf(low + (way > (double)chance * 0x1p-16 * span ? 1.0f : 0.0f), kLevels);
+  }
+  // The same in float32; `sure` becomes false where its roundings, of at most 6 units of z, might decide,
+  // or where the root's might: there only the first or last chance tells the code above from the one
+  // below that is raised.  (90 million moments with both in float64 378 us, bound by its operations.)
+  static __device__ __forceinline__ float nearly(float value, float inverse, uint32_t chance, bool& sure) {
+    const float z = value * inverse, low = floorf(root(z));  // inverse: (float)kAll / scale
+    const float step = fmaf(2.0f, low, 1.0f), square = low * low;
+    float way, span;
+    if constexpr (POWER == 2) {
+      way = fmaf(-low, low, z);
+      span = step;
+    } else {
+      way = fmaf(-square, square, z);
+      span = step * fmaf(2.0f, square, step);
+    }
+    const float rest = fmaf(-0x1p-16f * (float)chance, span, way);
+    sure = sure && fabsf(rest) > z * 4e-7f && chance - 1u < 65534u;
+    return low + (rest > 0.0f ? 1.0f : 0.0f);
+  }
+};
+constexpr float kSmallest = 0x1p-126f;
 
 typedef uint32_t WordAt1 __attribute__((aligned(1)));
 __device__ __forceinline__ uint32_t load_codes(const void* p, int64_t at, int count) {
@@ -279,11 +300,14 @@ __device__ __forceinline__ void store_codes(void* p, int64_t at, uint32_t w, int
     if (k < count) to[k] = (uint8_t)(w >> (8 * k));
 }
 
-template <bool EIGHT>
-__global__ __launch_bounds__(kBlock) void adamw_kernel(StepTable table, StepNumbers numbers) {
+template <bool EIGHT, int TURNS>
+__global__ __launch_bounds__(kBlock, EIGHT ? 8 : 4) void adamw_kernel(StepTable table, StepNumbers numbers) {
   __shared__ Powers powers;
   if (EIGHT) fill_powers(powers);
+  constexpr int kTurns = TURNS, kChunk = TURNS * kTurn;
   const uint32_t chunks = table.chunks_end[table.count - 1];
+  Step s;
+  bool known = false;
   for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const int t = tensor_of(table, chunk);
     const int64_t first = (int64_t)(chunk - (t > 0 ? table.chunks_end[t - 1] : 0)) * kChunk;
@@ -320,7 +344,8 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(StepTable table, StepNumb
         unit2[u] = there ? table.second_scale[t][block] * kSecondUnit : 0.0f;
       }
     }
-    const Step s = step_of(numbers);
+    if (!known) s = step_of(numbers);  // while the first chunk is on its way
+    known = true;
     if (!s.finite) return;
     uint32_t key = 0;
     if (EIGHT) {
@@ -364,16 +389,22 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(StepTable table, StepNumb
         }
       }
       const float scale1 = wave_largest(largest1), scale2 = wave_largest(largest2);
-      const float inverse1 = 1.0f / scale1, inverse2 = 1.0f / scale2;
+      // (A scale below the normal numbers is none: all codes are those of zero.)
+      const float inverse1 = scale1 < kSmallest ? 0.0f : (float)Code<2>::kAll * __builtin_amdgcn_rcpf(scale1);
+      const float inverse2 = scale2 < kSmallest ? 0.0f : (float)Code<4>::kAll * __builtin_amdgcn_rcpf(scale2);
       uint32_t codes1 = 0, codes2 = 0;
 #pragma unroll
       for (int k = 0; k < kW; ++k) {
         const uint32_t chance = mixed((uint32_t)(at + k) * 0x9e3779b9u + key);
-        const float share1 = share_of(fabsf(moment1[k]), scale1, inverse1);
-        const float share2 = share_of(moment2[k], scale2, inverse2);
-        const uint32_t q = scale1 < kSmallest ? 0u : code_of<2>(share1, chance & 0xffffu);
-        codes1 |= (moment1[k] < 0.0f ? 128u - q : 128u + q) << (8 * k);
-        codes2 |= (scale2 < kSmallest ? 0u : code_of<4>(share2, chance >> 16)) << (8 * k);
+        bool sure = true;
+        float code1 = Code<2>::nearly(fabsf(moment1[k]), inverse1, chance & 0xffffu, sure);
+        float code2 = Code<4>::nearly(moment2[k], inverse2, chance >> 16, sure);
+        if (__any(!sure)) {  // (of a hundred waves one)
+          code1 = scale1 < kSmallest ? 0.0f : Code<2>::exactly(fabsf(moment1[k]), scale1, chance & 0xffffu);
+          code2 = scale2 < kSmallest ? 0.0f : Code<4>::exactly(moment2[k], scale2, chance >> 16);
+        }
+        codes1 = __builtin_amdgcn_cvt_pk_u8_f32(128.0f + copysignf(code1, moment1[k]), k, codes1);
+        codes2 = __builtin_amdgcn_cvt_pk_u8_f32(code2, k, codes2);
       }
       if (count > 0) {
         store_codes(table.first[t], at, codes1, count);
@@ -407,18 +438,18 @@ __global__ __launch_bounds__(kBlock) void adamw_moments_kernel(ReadTable table) 
   const uint32_t chunks = table.chunks_end[table.count - 1];
   for (uint32_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
     const int t = tensor_of(table, chunk);
-    const int64_t first = (int64_t)(chunk - (t > 0 ? table.chunks_end[t - 1] : 0)) * kChunk;
-    uint32_t codes[kTurns];
-    float unit[kTurns];
+    const int64_t first = (int64_t)(chunk - (t > 0 ? table.chunks_end[t - 1] : 0)) * kReadChunk;
+    uint32_t codes[kReadTurns];
+    float unit[kReadTurns];
 #pragma unroll
-    for (int u = 0; u < kTurns; ++u) {
+    for (int u = 0; u < kReadTurns; ++u) {
       const int64_t at = first + u * kTurn + threadIdx.x * kW, left = table.length[t] - at;
       codes[u] = load_codes(table.codes[t], at, left < kW ? (int)left : kW);
       unit[u] = left > 0 ? table.scales[t][at / kMomentBlock] * (SECOND ? kSecondUnit : kFirstUnit)
                          : 0.0f;
     }
 #pragma unroll
-    for (int u = 0; u < kTurns; ++u) {
+    for (int u = 0; u < kReadTurns; ++u) {
       const int64_t at = first + u * kTurn + threadIdx.x * kW, left = table.length[t] - at;
       if (left <= 0) break;
       float v[kW];
@@ -453,6 +484,9 @@ int32_t launch_adamw(hipStream_t stream, const AdamwArgs& a) {
   numbers.seed_low = (uint32_t)(uint64_t)o.seed;
   numbers.seed_high = (uint32_t)((uint64_t)o.seed >> 32);
   const bool eight = a.first_scales != nullptr;
+  int64_t elements = 0;
+  for (int64_t k = 0; k < a.count; ++k) elements += a.parameters[k].length;
+  const bool long_chunks = !eight && elements >= kLongFrom;
   StepTable table;
   for (int64_t next = 0; next < a.count;) {
     int used = 0;
@@ -460,7 +494,7 @@ int32_t launch_adamw(hipStream_t stream, const AdamwArgs& a) {
     for (; next < a.count && used < kTensors; ++next) {
       const int64_t length = a.parameters[next].length;
       if (length == 0) continue;
-      chunks += div_up(length, kChunk);  // (at most 2^28 and one per tensor)
+      chunks += div_up(length, (long_chunks ? kLongTurns : kShortTurns) * kTurn);  // (at most 2^28 and one per tensor)
       table.parameter[used] = a.parameters[next].data;
       table.gradient[used] = a.gradients[next].data;
       table.first[used] = a.first[next].data;
@@ -479,9 +513,13 @@ int32_t launch_adamw(hipStream_t stream, const AdamwArgs& a) {
     table.count = used;
     {
       ProfileScope scope(stream, eight ? "adamw_8bit" : "adamw");
-      const dim3 grid((unsigned)(chunks < kMaxBlocks ? chunks : kMaxBlocks));
-      if (eight) hipLaunchKernelGGL((adamw_kernel<true>), grid, dim3(kBlock), 0, stream, table, numbers);
-      else hipLaunchKernelGGL((adamw_kernel<false>), grid, dim3(kBlock), 0, stream, table, numbers);
+      // (With 8 bits a block that goes on to further chunks has its table of powers for all.)
+      const int64_t most = eight ? (int64_t)device_cu_count() * kBlocksPerCu : kMaxBlocks;
+      const dim3 grid((unsigned)(chunks < most ? chunks : most));
+      const auto kernel = eight ? adamw_kernel<true, kShortTurns>
+                                : long_chunks ? adamw_kernel<false, kLongTurns>
+                                              : adamw_kernel<false, kShortTurns>;
+      hipLaunchKernelGGL(kernel, grid, dim3(kBlock), 0, stream, table, numbers);
     }
     ILGPU_HIP_CHECK(hipGetLastError());
   }
@@ -497,7 +535,7 @@ int32_t launch_adamw_moments(hipStream_t stream, const ilgpu_hip_tensor* codes,
     int64_t chunks = 0;
     for (; next < count && used < kReadTensors; ++next) {
       if (codes[next].length == 0) continue;
-      chunks += div_up(codes[next].length, kChunk);
+      chunks += div_up(codes[next].length, kReadChunk);
       table.codes[used] = codes[next].data;
       table.scales[used] = static_cast<const float*>(scales[next].data);
       table.target[used] = targets[next].data;

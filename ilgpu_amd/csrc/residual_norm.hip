@@ -222,14 +222,22 @@ __global__ __launch_bounds__(kLongBlock) void residual_norm_long_kernel(Residual
 // A wave or block goes over rows like the forward pass and adds up what its columns give to the
 // weights' gradients on the way; a second kernel adds up the blocks' sums in their order.
 constexpr int kGradientBlock = 512;
-constexpr int kGradientWavesPerCu = 12;
+constexpr int kGradientWavesPerCu = 16;
 constexpr int kMaxSplitsPerCu = 4;
 constexpr int kRowsPerSplit = 4;
-// Of a row that a block has: 512 threads leave each 256 registers.
+// Up to 512 vectors a row, two blocks share a compute unit with 128 registers a thread, so that one loads
+// while the other waits for its sums; longer rows have a block for themselves.
 constexpr int kWideBlock = 512;
 
+// Waves of a SIMD: as many as leave the registers that a thread asks for.  (16384 x 4096 bfloat16, a block
+// of 512 threads a row: 209 us with 128 registers and two blocks a compute unit, 247 with 136 and one;
+// with the stream in float32, which 128 registers spill, 152 against 204 with 8192 rows.)
+template <typename T, typename TR, int LANES, int V> constexpr int gradient_waves() {
+  if (sizeof(T) == 4) return LANES <= kWaveSize && V > 1 ? 3 : 4;
+  return V > 1 ? 2 : LANES <= kWaveSize || sizeof(TR) == 4 ? 3 : 4;
+}
 template <typename T, typename TR, int W, int LANES, int V, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void residual_norm_gradient_kernel(
+__global__ __launch_bounds__(BLOCK, (gradient_waves<T, TR, LANES, V>())) void residual_norm_gradient_kernel(
     ResidualNormGradientArgs a, float* __restrict__ partials) {
   constexpr int kRows = LANES <= kWaveSize ? BLOCK / LANES : 1;  // at a time
   constexpr int kJoins = LANES <= kWaveSize ? BLOCK / kWaveSize : 1;
@@ -523,7 +531,9 @@ template <typename F> int32_t with_residual_types(int32_t type, int32_t residual
 
 int32_t launch_residual_norm(hipStream_t stream, const ResidualNormArgs& a) {
   if (a.rows == 0) return ILGPU_HIP_SUCCESS;
-  constexpr int kWavesPerCu = 64;
+  // (Waves wanted a compute unit, 32768 x 2048 bfloat16, the stream in float32, us: 32 188, 64 184, 128 177,
+  // 512 173: four rows in a block one after the other, whose weights come from the caches each time.)
+  constexpr int kWavesPerCu = 512;
   return with_residual_types(a.type, a.residual_type, [&](auto t, auto tr) -> int32_t {
     using T = decltype(t);
     using TR = decltype(tr);
@@ -636,17 +646,23 @@ int32_t launch_residual_norm_gradient(hipStream_t stream, const ResidualNormGrad
     };
     using std::integral_constant;
     return with_shape<T>(
-        a.columns, kWideBlock,
+        a.columns, sizeof(T) == 4 ? kWholeBlock : kWideBlock,
         [&](auto w, auto lanes, auto v, int row_threads) -> int32_t {
           constexpr int kLanes = decltype(lanes)::value, kV = decltype(v)::value;
+          const auto block = [&](auto size) { return in_registers(w, lanes, v, size, row_threads); };
           if constexpr (kLanes <= kWaveSize) {
             return in_registers(w, lanes, v, integral_constant<int, kGradientBlock>(), kGradientBlock);
-          } else if constexpr (kV <= 2) {
-            if (row_threads <= kWideBlock)
-              return in_registers(w, lanes, v, integral_constant<int, kWideBlock>(), row_threads);
-            return of_long_rows();
+          } else if constexpr (sizeof(T) == 4) {
+            if constexpr (kV > 2) {
+              return of_long_rows();
+            } else {
+              if constexpr (kV == 1)
+                if (row_threads <= kWideBlock) return block(integral_constant<int, kWideBlock>());
+              return block(integral_constant<int, kWholeBlock>());
+            }
           } else {
-            return of_long_rows();
+            if (row_threads > kWideBlock) return of_long_rows();
+            return block(integral_constant<int, kWideBlock>());
           }
         },
         of_long_rows);
