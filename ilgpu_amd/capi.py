@@ -806,8 +806,11 @@ def _same_shape(first: DeviceMatrix, **others) -> None:
             raise ArgumentOutOfRangeError(ERROR_OUT_OF_RANGE, what)
 
 
+_NO_MATRIX = (None, 0)
+
+
 def _matrix(m: Optional[DeviceMatrix]):
-    return (None, 0) if m is None else (m.ptr, m.row_stride)
+    return _NO_MATRIX if m is None else (m.ptr, m.row_stride)
 
 
 def _states(m: Optional[DeviceMatrix], sequences: int, channels: int, what: str):
@@ -888,13 +891,14 @@ def gated_recurrence_gradient(grad_out: DeviceMatrix, gate: DeviceMatrix, inp: D
         temp_ptr, temp_bytes))
 
 
-def _weights(columns: int, otherwise: int, **vectors):
-    """The type of the vectors that are there, and a pointer for each."""
-    there = [a for a in vectors.values() if a is not None]
-    kind = there[0].type_code if there else otherwise
-    if any(a.type_code != kind for a in there):
+def _weight_type(otherwise: int, *vectors) -> int:
+    """The type of the vectors that are there."""
+    there = [a.type_code for a in vectors if a is not None]
+    if not there:
+        return otherwise
+    if there.count(there[0]) != len(there):
         raise NotSupportedError(ERROR_NOT_SUPPORTED, "types differ")
-    return (kind, *(_column_vector(a, columns, what) for what, a in vectors.items()))
+    return there[0]
 
 
 def residual_norm(inp: DeviceMatrix, residual: Optional[DeviceMatrix],
@@ -909,21 +913,29 @@ def residual_norm(inp: DeviceMatrix, residual: Optional[DeviceMatrix],
     squares + epsilon), input_rstd the same of inp.  inp is normalised with input_norm, which
     an input_weight or input_rstd stands for.  input_rstd and rstd (float32) receive what the
     gradients need."""
+    rows, columns, kind = inp.rows, inp.columns, inp.type_code
     if input_norm is None:
         input_norm = input_weight is not None or input_rstd is not None
-    _same_shape(inp, residual=residual, total=total, out=out, gate=gate)
-    _same_type(inp, gate, out)
-    stream_type = next((m.type_code for m in (residual, total) if m is not None), inp.type_code)
-    if total is not None and total.type_code != stream_type:
+    for m in (residual, total, out, gate):
+        if m is not None and (m.rows != rows or m.columns != columns):
+            _same_shape(inp, residual=residual, total=total, out=out, gate=gate)
+    some = residual if residual is not None else total
+    stream_type = kind if some is None else some.type_code
+    if (gate is not None and gate.type_code != kind) or (
+            out is not None and out.type_code != kind) or (
+            total is not None and total.type_code != stream_type):
         raise NotSupportedError(ERROR_NOT_SUPPORTED, "types differ")
-    kind, weight_ptr, input_ptr = _weights(inp.columns, inp.type_code, weight=weight,
-                                           input_weight=input_weight)
+    vector = weight if weight is not None else input_weight
+    weight_type = kind if vector is None else vector.type_code
+    if input_weight is not None and input_weight.type_code != weight_type:
+        raise NotSupportedError(ERROR_NOT_SUPPORTED, "types differ")
     check((_lib or lib()).ilgpu_hip_residual_norm(
-        _stream_ptr(stream), inp.ptr, inp.row_stride, inp.rows, inp.columns, inp.type_code,
-        1 if input_norm else 0, input_ptr, *_matrix(gate), gate_kind, *_matrix(residual),
-        stream_type, _float(scale), weight_ptr, kind, _float(epsilon), *_matrix(total),
-        *_matrix(out), _statistic(input_rstd, inp.rows, "input_rstd"),
-        _statistic(rstd, inp.rows, "rstd")))
+        _stream_ptr(stream), inp.ptr, inp.row_stride, rows, columns, kind,
+        1 if input_norm else 0, _column_vector(input_weight, columns, "input_weight"),
+        *_matrix(gate), gate_kind, *_matrix(residual), stream_type, _float(scale),
+        _column_vector(weight, columns, "weight"), weight_type, _float(epsilon), *_matrix(total),
+        *_matrix(out), _statistic(input_rstd, rows, "input_rstd"),
+        _statistic(rstd, rows, "rstd")))
 
 
 def residual_norm_gradient_temp_bytes(rows: int, columns: int) -> int:
@@ -956,18 +968,20 @@ def residual_norm_gradient(grad_out: Optional[DeviceMatrix], grad_total: Optiona
     stream_type = of_stream[0].type_code if of_stream else inp.type_code
     if any(m.type_code != stream_type for m in of_stream):
         raise NotSupportedError(ERROR_NOT_SUPPORTED, "types differ")
-    kind, weight_ptr, input_ptr, grad_weight_ptr, grad_input_ptr = _weights(
-        inp.columns, inp.type_code, weight=weight, input_weight=input_weight,
-        grad_weight=grad_weight, grad_input_weight=grad_input_weight)
+    columns = inp.columns
     if temp is None:
-        temp = _scratch(residual_norm_gradient_temp_bytes(inp.rows, inp.columns), stream)
+        temp = _scratch(residual_norm_gradient_temp_bytes(inp.rows, columns), stream)
     check((_lib or lib()).ilgpu_hip_residual_norm_gradient(
         _stream_ptr(stream), *_matrix(grad_out), *_matrix(grad_total), inp.ptr, inp.row_stride,
-        inp.rows, inp.columns, inp.type_code, 1 if input_norm else 0, input_ptr,
+        inp.rows, columns, inp.type_code, 1 if input_norm else 0,
+        _column_vector(input_weight, columns, "input_weight"),
         _statistic(input_rstd, inp.rows, "input_rstd"), *_matrix(gate), gate_kind,
-        *_matrix(total), stream_type, _float(scale), weight_ptr, kind,
+        *_matrix(total), stream_type, _float(scale), _column_vector(weight, columns, "weight"),
+        _weight_type(inp.type_code, weight, input_weight, grad_weight, grad_input_weight),
         _statistic(rstd, inp.rows, "rstd"), *_matrix(grad_in), *_matrix(grad_gate),
-        *_matrix(grad_residual), grad_input_ptr, grad_weight_ptr, 1 if accumulate else 0,
+        *_matrix(grad_residual),
+        _column_vector(grad_input_weight, columns, "grad_input_weight"),
+        _column_vector(grad_weight, columns, "grad_weight"), 1 if accumulate else 0,
         temp.ptr, temp.nbytes))
 
 
@@ -992,17 +1006,21 @@ def adamw(parameters, gradients, first, second, step: DeviceArray, *, rate: floa
     ADAMW_MOMENT_BLOCK elements begun), uint8; zeros before the first step.  copies receive the
     parameters in their own types."""
     parameters = _tensor_list(parameters)
-    count = len(parameters)
-    kept = [_table(t, count, what) for t, what in (
-        (gradients, "gradients"), (first, "first"), (second, "second"),
-        (first_scales, "first_scales"), (second_scales, "second_scales"), (copies, "copies"))]
+    count = len(parameters.arrays)
+    # (The lists are kept until the call has read their tables.)
+    gradients, first, second = _tensor_list(gradients), _tensor_list(first), _tensor_list(second)
+    _need(len(gradients.arrays) == len(first.arrays) == len(second.arrays) == count,
+          "lists of different lengths")
+    first_scales, first_table = _table(first_scales, count, "first_scales")
+    second_scales, second_table = _table(second_scales, count, "second_scales")
+    copies, copies_table = _table(copies, count, "copies")
     if step.type_code != I64:
         raise NotSupportedError(ERROR_NOT_SUPPORTED, "step is int64")
     _need(_dense(step).length >= 1, "step")
     options = _AdamwOptions(rate, betas[0], betas[1], epsilon, weight_decay, max_norm, seed)
     check((_lib or lib()).ilgpu_hip_adamw(
-        _stream_ptr(stream), parameters.table, *(table for _, table in kept), count,
-        ctypes.byref(options), step.ptr, _statistic(schedule, 1, "schedule"),
+        _stream_ptr(stream), parameters.table, gradients.table, first.table, second.table,
+        first_table, second_table, copies_table, count, ctypes.byref(options), step.ptr, _statistic(schedule, 1, "schedule"),
         _statistic(norm, 1, "norm")))
 
 
