@@ -9,6 +9,14 @@
 // it begins at the state that the tile before it has published or at one some tiles further back, it goes
 // through the same operations on the same numbers, so every run gives the same bits.
 //
+// Bound by latency in front of the memory: of a tile's 11 us, loads, the fold, the look-back and
+// the stores follow one another, and two (backwards three) tiles share a compute unit.  65536 x 2048
+// bfloat16 208 us, 3.9 TB/s; 168 without the look-back's wait, which is all that is known to be left.
+// Gradients of 31744 x 4096 389 us, 4.0 TB/s.  (Rows of a thread, us, 16 / 8 / 4 / 2: forwards 392 / 229 / 269 / 384 of the first
+// form, backwards 8 / 4 / 2: 614 / 465 / 524: shorter tiles walk back more often than they fill the
+// waits.  Blocks that go on from tile to tile, the next one's loads in front of the stores: 280 and 440.
+// Polls as seldom as every 2048 cycles: no difference.)
+//
 // A sequence's first row is a reset: its map forgets what comes in, whatever that is (a NaN
 // times 0 would still be one).  A reset is marked by A = -0, which no product of
 // decays gives.  Backwards, with P[t] = a[t] G[t] for the state, G[t] = grad_out[t] + P[t+1] is the same scan
@@ -29,13 +37,7 @@ constexpr int64_t kMostBlocks = 1 << 22;  // of a launch
 
 // Rows of a thread; row groups of a tile; rows of a tile.
 template <int W> constexpr int groups_of() { return kBlock * W / kTileChannels; }
-#ifndef ILGPU_HIP_RECURRENCE_ROWS
-#define ILGPU_HIP_RECURRENCE_ROWS 8
-#endif
-#ifndef ILGPU_HIP_RECURRENCE_BACK_ROWS
-#define ILGPU_HIP_RECURRENCE_BACK_ROWS 4
-#endif
-constexpr int kRows = ILGPU_HIP_RECURRENCE_ROWS, kBackRows = ILGPU_HIP_RECURRENCE_BACK_ROWS;
+constexpr int kRows = 8, kBackRows = 4;
 constexpr int kFewestRows = kRows < kBackRows ? kRows : kBackRows;
 
 constexpr int64_t kTicketBytes = 128;  // of a column of tiles: a line of its own
@@ -241,11 +243,8 @@ __device__ __forceinline__ float look_back(const Scan& s, int64_t tile, uint32_t
   return h;
 }
 
-#ifndef ILGPU_HIP_RECURRENCE_WAVES
-#define ILGPU_HIP_RECURRENCE_WAVES 2
-#endif
 template <typename T, int W, int R, bool BACK, bool SIGMOID, bool COMPLEMENT>
-__global__ __launch_bounds__(kBlock, ILGPU_HIP_RECURRENCE_WAVES) void recurrence_kernel(Scan s) {
+__global__ __launch_bounds__(kBlock, 2) void recurrence_kernel(Scan s) {
   constexpr int kGroups = groups_of<W>(), kTileRows = kGroups * R, kLanes = kTileChannels / W;
   constexpr int kWaveGroups = kGroups / kWaves;
   using V = typename Pack<T, W>::vec;
