@@ -11,7 +11,7 @@
 //
 // Bound by latency in front of the memory: of a tile's 11 us, loads, the fold, the look-back and
 // the stores follow one another, and two (backwards three) tiles share a compute unit.  65536 x 2048
-// bfloat16 208 us, 3.9 TB/s; 168 without the look-back's wait, which is all that is known to be left.
+// bfloat16 208 us, 3.9 TB/s; 161 without the look-back's wait, which is all that is known to be left.
 // Gradients of 31744 x 4096 389 us, 4.0 TB/s.  (Rows of a thread, us, 16 / 8 / 4 / 2: forwards 392 / 229 / 269 / 384 of the first
 // form, backwards 8 / 4 / 2: 614 / 465 / 524: shorter tiles walk back more often than they fill the
 // waits.  Blocks that go on from tile to tile, the next one's loads in front of the stores: 280 and 440.

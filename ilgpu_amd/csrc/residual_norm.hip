@@ -648,24 +648,24 @@ int32_t launch_residual_norm_gradient(hipStream_t stream, const ResidualNormGrad
       return ILGPU_HIP_SUCCESS;
     };
     using std::integral_constant;
+    // A vector a thread in up to 1024 threads where a thread's registers hold the next row beside it; with a
+    // wider stream two vectors in up to 512.  (8192 rows bfloat16 by one vector and by two, us: 5120 columns
+    // 163 and 189, 8192 213 and 241; with the stream in float32, whose second row spills, 6144 321 and 278.)
+    constexpr bool kOneVector = sizeof(T) == sizeof(TR);
     return with_shape<T>(
-        a.columns, sizeof(T) == 4 ? kWholeBlock : kWideBlock,
+        a.columns, kOneVector ? kWholeBlock : kWideBlock,
         [&](auto w, auto lanes, auto v, int row_threads) -> int32_t {
           constexpr int kLanes = decltype(lanes)::value, kV = decltype(v)::value;
           const auto block = [&](auto size) { return in_registers(w, lanes, v, size, row_threads); };
           if constexpr (kLanes <= kWaveSize) {
             return in_registers(w, lanes, v, integral_constant<int, kGradientBlock>(), kGradientBlock);
-          } else if constexpr (sizeof(T) == 4) {
-            if constexpr (kV > 2) {
-              return of_long_rows();
-            } else {
-              if constexpr (kV == 1)
-                if (row_threads <= kWideBlock) return block(integral_constant<int, kWideBlock>());
-              return block(integral_constant<int, kWholeBlock>());
-            }
+          } else if constexpr (kV > 2 || (kV == 2 && kOneVector && sizeof(T) == 2)) {
+            return of_long_rows();
           } else {
-            if (row_threads > kWideBlock) return of_long_rows();
-            return block(integral_constant<int, kWideBlock>());
+            if constexpr (kV == 1 || sizeof(T) == 2)
+              if (row_threads <= kWideBlock) return block(integral_constant<int, kWideBlock>());
+            if constexpr (kOneVector) return block(integral_constant<int, kWholeBlock>());
+            else return of_long_rows();
           }
         },
         of_long_rows);
