@@ -32,12 +32,13 @@ constexpr int kBlock = 256;
 constexpr int kWaves = kBlock / kWaveSize;
 constexpr int kTileChannels = kWaveSize;  // a wave's lanes walk back, a channel each
 constexpr int kWindow = 4;                // tiles that a look-back asks at a time
+constexpr int kWideWindow = 16;           // and of few columns of tiles
 constexpr uint32_t kMostPolls = 1 << 24;  // of a look-back: many seconds
 constexpr int64_t kMostBlocks = 1 << 22;  // of a launch
 
 // Rows of a thread; row groups of a tile; rows of a tile.
 template <int W> constexpr int groups_of() { return kBlock * W / kTileChannels; }
-constexpr int kRows = 8, kBackRows = 4;
+constexpr int kRows = 8, kBackRows = 4, kLongBackRows = 8;
 constexpr int kFewestRows = kRows < kBackRows ? kRows : kBackRows;
 
 constexpr int64_t kTicketBytes = 128;  // of a column of tiles: a line of its own
@@ -178,6 +179,7 @@ struct Scan {
   uint64_t* words;
   int64_t tiles;            // of rows
   uint32_t columns_of_tiles;
+  bool wide;                // what a look-back asks at a time
   int64_t first_block;      // of this launch
 };
 
@@ -198,9 +200,43 @@ __device__ __forceinline__ float value_of(uint64_t w) {
   return __builtin_bit_cast(float, (uint32_t)w);
 }
 
+// The state in front of a tile that is not the first, from up to WINDOW tiles in front.  (A wait ends
+// all the same, with a NaN, if the words are another call's, to which the temp was given at the same time.)
+template <int WINDOW>
+__device__ __forceinline__ float walk_back(const Scan& s, int64_t tile, uint32_t column) {
+  float h = __builtin_nanf("");
+  for (uint32_t polls = 0; polls < kMostPolls; ++polls) {
+    uint64_t low[WINDOW], high[WINDOW];
+#pragma unroll
+    for (int d = 0; d < WINDOW; ++d) {
+      const int64_t front = tile - 1 - d;
+      const uint64_t* w = words_of(s, front > 0 ? front : 0, column);
+      low[d] = get_word(w);
+      high[d] = get_word(w + 1);
+    }
+    int found = -1;  // the nearest tile whose state is known, all maps behind it being there
+    bool whole = true;
+#pragma unroll
+    for (int d = 0; d < WINDOW; ++d) {
+      if (whole && found < 0 && low[d] >> 32 == 2) found = d;
+      whole = whole && low[d] >> 32 == 1 && high[d] >> 32 == 1;
+    }
+    if (__all(found >= 0)) {
+#pragma unroll
+      for (int d = WINDOW - 1; d >= 0; --d) {
+        if (d == found) h = value_of(low[d]);
+        else if (d < found) h = apply(Map{value_of(high[d]), value_of(low[d])}, h);
+      }
+      break;
+    }
+    __builtin_amdgcn_s_sleep(1);
+  }
+  return h;
+}
+
 // The state in front of a tile, a channel a lane, by one wave.  The tiles in front have drawn
-// their tickets before this one, so they run and publish, and no wait is long.  (It ends all the same, with a
-// NaN, if the words are another call's, to which the temp was given at the same time.)
+// their tickets before this one, so they run and publish, and no wait is long.
+template <int WIDE>
 __device__ __forceinline__ float look_back(const Scan& s, int64_t tile, uint32_t column, Map own) {
   uint64_t* mine = words_of(s, tile, column);
   float h = 0.0f;
@@ -211,33 +247,7 @@ __device__ __forceinline__ float look_back(const Scan& s, int64_t tile, uint32_t
       put_word(mine + 1, 1, own.a);
       put_word(mine, 1, own.b);
     }
-    h = __builtin_nanf("");
-    for (uint32_t polls = 0; polls < kMostPolls; ++polls) {
-      uint64_t low[kWindow], high[kWindow];
-#pragma unroll
-      for (int d = 0; d < kWindow; ++d) {
-        const int64_t front = tile - 1 - d;
-        const uint64_t* w = words_of(s, front > 0 ? front : 0, column);
-        low[d] = get_word(w);
-        high[d] = get_word(w + 1);
-      }
-      int found = -1;  // the nearest tile whose state is known, all maps behind it being there
-      bool whole = true;
-#pragma unroll
-      for (int d = 0; d < kWindow; ++d) {
-        if (whole && found < 0 && low[d] >> 32 == 2) found = d;
-        whole = whole && low[d] >> 32 == 1 && high[d] >> 32 == 1;
-      }
-      if (__all(found >= 0)) {
-#pragma unroll
-        for (int d = kWindow - 1; d >= 0; --d) {
-          if (d == found) h = value_of(low[d]);
-          else if (d < found) h = apply(Map{value_of(high[d]), value_of(low[d])}, h);
-        }
-        break;
-      }
-      __builtin_amdgcn_s_sleep(1);
-    }
+    h = s.wide ? walk_back<WIDE>(s, tile, column) : walk_back<kWindow>(s, tile, column);
   }
   put_word(mine, 2, apply(own, h));
   return h;
@@ -247,6 +257,8 @@ template <typename T, int W, int R, bool BACK, bool SIGMOID, bool COMPLEMENT>
 __global__ __launch_bounds__(kBlock, 2) void recurrence_kernel(Scan s) {
   constexpr int kGroups = groups_of<W>(), kTileRows = kGroups * R, kLanes = kTileChannels / W;
   constexpr int kWaveGroups = kGroups / kWaves;
+  // (Backwards there are no registers for 16.)
+  constexpr int kWide = BACK ? kWideWindow / 2 : kWideWindow;
   using V = typename Pack<T, W>::vec;
   using P = typename Pack<T, W>::type;
   __shared__ Map maps[kGroups][kTileChannels];
@@ -414,7 +426,7 @@ __global__ __launch_bounds__(kBlock, 2) void recurrence_kernel(Scan s) {
     Map all = wave_maps[0][channel];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) all = behind(wave_maps[w][channel], all);
-    float state = s.tickets != nullptr ? look_back(s, tile, column, all) : 0.0f;
+    float state = s.tickets != nullptr ? look_back<kWide>(s, tile, column, all) : 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       wave_states[w][channel] = state;
@@ -540,6 +552,16 @@ inline unsigned blocks_for_elements(int64_t threads) {
   return (unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks);
 }
 
+// Few columns of tiles that all run at once wait for the state to come through them: a look-back that
+// asks more tiles at a time takes fewer turns.  (Window 4 and 16, us: 131072 x 64 101 and 62, 32768 x 512 36 and 31;
+// but 65536 x 2048 208 and 213, 2000 x 512 11.2 and 11.9; backwards 4 and 8: 65536 x 64 101 and 75.)
+constexpr int kFewColumns = 8;
+// Backwards, three tiles of four rows a thread or two of eight share a compute unit.  Eight rows are taken
+// where they make one turn of a grid that four would not, and where the chain of tiles is long but one turn still holds
+// it (us, 4 and 8: 8192 x 1024 28.6 and 26.7, 16384 x 512 32.7 and 27.7, 65536 x 64 75 and 50; but
+// 4096 x 1024 18.3 and 20.7, 16384 x 768 41 and 45).
+constexpr int64_t kManyTiles = 128;
+
 inline int64_t columns_of_tiles(int64_t channels) { return div_up(channels, kTileChannels); }
 
 template <typename T, int W, int R, bool BACK, bool SIGMOID, bool COMPLEMENT>
@@ -556,6 +578,7 @@ int32_t launch_scan_tiles(hipStream_t stream, Scan s, void* temp) {
     if (rc != ILGPU_HIP_SUCCESS) return rc;
   }
   const int64_t blocks = s.tiles * s.columns_of_tiles;
+  s.wide = s.columns_of_tiles <= kFewColumns && s.tiles > kWideWindow;
   for (s.first_block = 0; s.first_block < blocks; s.first_block += kMostBlocks) {
     const int64_t left = blocks - s.first_block;
     {
@@ -586,6 +609,13 @@ int32_t launch_scan_of(hipStream_t stream, int32_t type, const Scan& s, void* te
     }
     // (A row shorter than a vector: an element a thread.)
     if (s.channels < W) return launch_scan_tiles<T, 1, R, BACK, SIGMOID, COMPLEMENT>(stream, s, temp);
+    if constexpr (BACK) {
+      const int64_t tiles = div_up(s.rows, (int64_t)groups_of<W>() * R);
+      const int64_t blocks = tiles * columns_of_tiles(s.channels);
+      if (blocks <= 4 * device_cu_count() &&
+          (blocks > 3 * device_cu_count() || tiles >= kManyTiles))
+        return launch_scan_tiles<T, W, kLongBackRows, BACK, SIGMOID, COMPLEMENT>(stream, s, temp);
+    }
     return launch_scan_tiles<T, W, R, BACK, SIGMOID, COMPLEMENT>(stream, s, temp);
   });
 }

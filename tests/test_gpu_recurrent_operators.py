@@ -489,6 +489,37 @@ def test_recurrence_gradient_of_sequences(dtype, channels, way):
         assert torch.equal(state, got[2])
 
 
+# Many tiles of rows behind one another, and grids for which the gradients' tiles are longer.
+@pytest.mark.parametrize("cuts", [None, [3, 3, 4000, 4001, 4001, 6400, 8170]])
+@pytest.mark.parametrize("dtype,rows,channels", [("float32", 8321, 70), ("bfloat16", 16_700, 24),
+                                                 ("float16", 16_500, 130), ("bfloat16", 8193, 799)])
+def test_recurrence_and_gradient_of_many_tiles(dtype, rows, channels, cuts):
+    import torch
+    from ilgpu_amd import capi
+    g = _rng(rows, channels)
+    kind, complement = ("sigmoid", True) if cuts is None else ("exponential", False)
+    bounds = [0, rows] if cuts is None else cuts
+    sequences = len(bounds) - 1
+    offsets = None if cuts is None else torch.tensor(cuts, device="cuda")
+    gate, x, grad = (_gates(g, rows, channels, kind, _t(dtype)), _normal(g, rows, channels, dtype=_t(dtype)),
+                     _normal(g, rows, channels, dtype=_t(dtype)))
+    initial, grad_final = (torch.randn(sequences, channels, generator=g, device="cuda") for _ in range(2))
+    out, _ = _check_recurrence(gate, x, kind, complement, sequences, offsets, initial)
+    got = _gradient(capi, grad, gate, x, out, kind, complement, sequences, offsets, initial, grad_final)
+    _check_gradient(got, grad, gate, x, out, kind, complement, bounds, initial, grad_final)
+    again = _gradient(capi, grad, gate, x, out, kind, complement, sequences, offsets, initial, grad_final)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    # over what is read
+    read, state = [grad.clone(), gate.clone()], grad_final.clone()
+    capi.gated_recurrence_gradient(
+        *(_matrix(t) for t in (read[0], read[1], x, out, read[0], read[1])), sequences=sequences,
+        offsets=_array(offsets), initial=_matrix(initial), grad_final=_matrix(state),
+        grad_initial=_matrix(state), decay=getattr(capi, "DECAY_" + kind.upper()), complement=complement)
+    used = slice(bounds[0], bounds[-1])
+    assert torch.equal(read[0][used], got[0][used]) and torch.equal(read[1][used], got[1][used])
+    assert torch.equal(state, got[2])
+
+
 def test_recurrence_gradient_against_differences():
     # In float32 with steps of 1/64: a difference is off by its curvature, of which a central one
     # keeps the third derivative, and by the roundings of the loss's terms over the step.
