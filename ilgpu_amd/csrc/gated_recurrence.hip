@@ -11,8 +11,8 @@
 //
 // Bound by latency in front of the memory: of a tile's 11 us, loads, the fold, the look-back and
 // the stores follow one another, and two (backwards three) tiles share a compute unit.  65536 x 2048
-// bfloat16 208 us, 3.9 TB/s; 161 without the look-back's wait, which is all that is known to be left.
-// Gradients of 31744 x 4096 389 us, 4.0 TB/s.  (Rows of a thread, us, 16 / 8 / 4 / 2: forwards 392 / 229 / 269 / 384 of the first
+// bfloat16 210 us, 3.8 TB/s; 161 without the look-back's wait, which is all that is known to be left.
+// Gradients of 31744 x 4096 390 us, 4.0 TB/s.  (Rows of a thread, us, 16 / 8 / 4 / 2: forwards 392 / 229 / 269 / 384 of the first
 // form, backwards 8 / 4 / 2: 614 / 465 / 524: shorter tiles walk back more often than they fill the
 // waits.  Blocks that go on from tile to tile, the next one's loads in front of the stores: 280 and 440.
 // Polls as seldom as every 2048 cycles: no difference.)
@@ -41,24 +41,38 @@ template <int W> constexpr int groups_of() { return kBlock * W / kTileChannels; 
 constexpr int kRows = 8, kBackRows = 4, kLongBackRows = 8;
 constexpr int kFewestRows = kRows < kBackRows ? kRows : kBackRows;
 
+constexpr float kSmallestNormal = 0x1p-126f;
+
 constexpr int64_t kTicketBytes = 128;  // of a column of tiles: a line of its own
 constexpr int64_t kStateBytes = kTileChannels * 16;
 
+// h -> 2^e a h + b, 1 <= a < 2 (or 0, infinity, a NaN; -0: a reset).  The decays of some rows
+// leave float32 together where each of them and the state do not: infinity times a state of 0, or 0 times an
+// infinite one, would be a NaN.  2^e goes to the state, which rounds nothing but results below the
+// normal numbers.
 struct Map {
   float a, b;
+  int32_t e;
 };
 __device__ __forceinline__ bool is_reset(float a) {
   return __builtin_bit_cast(uint32_t, a) == 0x80000000u;
 }
-// The map that does `first`, then `then`.
-__device__ __forceinline__ Map behind(Map then, Map first) {
-  Map m;
-  m.a = is_reset(then.a) || is_reset(first.a) ? -0.0f : then.a * first.a;
-  m.b = is_reset(then.a) ? then.b : fmaf(then.a, first.b, then.b);
-  return m;
+// 2^e a is multiplied by `factor`, 1/2 <= a < 1 behind it.
+__device__ __forceinline__ void multiply(float& a, int32_t& e, float factor) {
+  const float product = a * factor;
+  a = __builtin_amdgcn_frexp_mantf(product);
+  e += __builtin_amdgcn_frexp_expf(product);
 }
 __device__ __forceinline__ float apply(Map m, float h) {
-  return is_reset(m.a) ? m.b : fmaf(m.a, h, m.b);
+  return is_reset(m.a) ? m.b : fmaf(m.a, __builtin_ldexpf(h, m.e), m.b);
+}
+// The map that does `first`, then `then`.
+__device__ __forceinline__ Map behind(Map then, Map first) {
+  Map m{then.a, apply(then, first.b), then.e + first.e};
+  multiply(m.a, m.e, first.a);
+  m.a = is_reset(then.a) || is_reset(first.a) ? -0.0f : 2.0f * m.a;
+  --m.e;
+  return m;
 }
 
 // a and 1 - a of a gate, each to some units in its last place.
@@ -183,8 +197,8 @@ struct Scan {
   int64_t first_block;      // of this launch
 };
 
-// What a tile leaves for those behind it, two words a channel: {B, 1} and {A, 1} of its map, then
-// {state behind it, 2} in the first.
+// What a tile leaves for those behind it, two words a channel: {B, 1} and {A, 1 and its exponent} of
+// its map, then {state behind it, 2} in the first, at once if it is a reset.
 __device__ __forceinline__ uint64_t* words_of(const Scan& s, int64_t tile, uint32_t column) {
   return s.words + (tile * s.columns_of_tiles + column) * (kStateBytes / 8) +
          2 * (threadIdx.x & (kWaveSize - 1));
@@ -199,6 +213,8 @@ __device__ __forceinline__ uint64_t get_word(const uint64_t* w) {
 __device__ __forceinline__ float value_of(uint64_t w) {
   return __builtin_bit_cast(float, (uint32_t)w);
 }
+// (Of a tile's rows together less than 2^20, either way.)
+__device__ __forceinline__ int32_t exponent_of(uint64_t w) { return (int32_t)(w >> 32) >> 1; }
 
 // The state in front of a tile that is not the first, from up to WINDOW tiles in front.  (A wait ends
 // all the same, with a NaN, if the words are another call's, to which the temp was given at the same time.)
@@ -219,13 +235,14 @@ __device__ __forceinline__ float walk_back(const Scan& s, int64_t tile, uint32_t
 #pragma unroll
     for (int d = 0; d < WINDOW; ++d) {
       if (whole && found < 0 && low[d] >> 32 == 2) found = d;
-      whole = whole && low[d] >> 32 == 1 && high[d] >> 32 == 1;
+      whole = whole && low[d] >> 32 == 1 && high[d] >> 32 != 0;
     }
     if (__all(found >= 0)) {
 #pragma unroll
       for (int d = WINDOW - 1; d >= 0; --d) {
-        if (d == found) h = value_of(low[d]);
-        else if (d < found) h = apply(Map{value_of(high[d]), value_of(low[d])}, h);
+        // (Tiles that end in a reset publish no map; what d > found makes is not used.)
+        h = d == found ? value_of(low[d])
+                       : fmaf(value_of(high[d]), __builtin_ldexpf(h, exponent_of(high[d])), value_of(low[d]));
       }
       break;
     }
@@ -244,7 +261,7 @@ __device__ __forceinline__ float look_back(const Scan& s, int64_t tile, uint32_t
     if (is_reset(own.a)) {
       put_word(mine, 2, own.b);
     } else {
-      put_word(mine + 1, 1, own.a);
+      put_word(mine + 1, (uint32_t)own.e << 1 | 1, own.a);
       put_word(mine, 1, own.b);
     }
     h = s.wide ? walk_back<WIDE>(s, tile, column) : walk_back<kWindow>(s, tile, column);
@@ -261,7 +278,10 @@ __global__ __launch_bounds__(kBlock, 2) void recurrence_kernel(Scan s) {
   constexpr int kWide = BACK ? kWideWindow / 2 : kWideWindow;
   using V = typename Pack<T, W>::vec;
   using P = typename Pack<T, W>::type;
-  __shared__ Map maps[kGroups][kTileChannels];
+  // In LDS the k-th channels of all lanes lie side by side, and a row group begins a group's lanes further:
+  // 64 lanes that read or write a word each meet 64 banks.  The scan goes by these places.  (Channels in their
+  // order, us: gradients of 31744 x 4096 397 instead of 390.)
+  __shared__ Map maps[kGroups][kTileChannels + kLanes];
   __shared__ Map wave_maps[kWaves][kTileChannels];
   __shared__ float wave_states[kWaves][kTileChannels];
   __shared__ Marks<kGroups, R> marks;
@@ -384,7 +404,7 @@ __global__ __launch_bounds__(kBlock, 2) void recurrence_kernel(Scan s) {
   // written over by what it leaves, once this tile's map is known.)
   constexpr int kHeld = BACK ? 1 : R;
   float held_a[kHeld][W], b[R][W];
-  float own_a[W], h[W];
+  float own_a[W], h[W], largest = 0.0f;
 #pragma unroll
   for (int k = 0; k < W; ++k) {
     own_a[k] = 1.0f;
@@ -400,12 +420,47 @@ __global__ __launch_bounds__(kBlock, 2) void recurrence_kernel(Scan s) {
     for (int k = 0; k < W; ++k) {
       h[k] = BACK ? a[k] * (b[r][k] + h[k]) : fmaf(a[k], h[k], b[r][k]);
       own_a[k] *= a[k];
+      if (!SIGMOID) largest = fmaxf(largest, a[k]);
       if constexpr (!BACK) held_a[r][k] = a[k];
     }
     if (BACK) __builtin_amdgcn_sched_barrier(0);  // (rows side by side take more registers)
   }
+  // Decays of up to 1 whose product is a normal number have not left float32 on the way.  (With the exponent
+  // apart in every row, us: 65536 x 2048 211.1 instead of 209.8, gradients of 8192 x 1024 27.0 instead of 26.6.)
+  bool left_range = largest > 1.0f;
 #pragma unroll
-  for (int k = 0; k < W; ++k) maps[group][lane * W + k] = Map{resets != 0 ? -0.0f : own_a[k], h[k]};
+  for (int k = 0; k < W; ++k) {
+    left_range = left_range || !(own_a[k] >= kSmallestNormal);
+    maps[group][k * kLanes + lane].b = h[k];
+  }
+  const auto put_decay = [&](int k, float a, int32_t e) {  // 2^e a, 1/2 <= a < 1
+    Map& m = maps[group][k * kLanes + lane];
+    m.a = resets != 0 ? -0.0f : 2.0f * a;
+    m.e = e - 1;
+  };
+  if (__any(left_range && resets == 0)) {
+    int32_t own_e[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      own_a[k] = 0.5f;
+      own_e[k] = 1;
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float a[W], left[W];
+      if constexpr (BACK) keep(gate[r]);
+      decays(r, a, left);
+#pragma unroll
+      for (int k = 0; k < W; ++k) multiply(own_a[k], own_e[k], a[k]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int k = 0; k < W; ++k) put_decay(k, own_a[k], own_e[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < W; ++k)
+      put_decay(k, __builtin_amdgcn_frexp_mantf(own_a[k]), __builtin_amdgcn_frexp_expf(own_a[k]));
+  }
   if constexpr (BACK) {
 #pragma unroll
     for (int r = 0; r < R; ++r) keep(gate[r]);
@@ -413,7 +468,7 @@ __global__ __launch_bounds__(kBlock, 2) void recurrence_kernel(Scan s) {
   __syncthreads();
   // The maps in front of each group of a wave, then those in front of each wave.
   const int wave = threadIdx.x / kWaveSize, channel = threadIdx.x % kWaveSize;
-  Map front{1.0f, 0.0f};
+  Map front{1.0f, 0.0f, 0};
 #pragma unroll
   for (int g = 0; g < kWaveGroups; ++g) {
     const Map here = maps[wave * kWaveGroups + g][channel];
@@ -436,7 +491,7 @@ __global__ __launch_bounds__(kBlock, 2) void recurrence_kernel(Scan s) {
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < W; ++k)
-    h[k] = apply(maps[group][lane * W + k], wave_states[wave][lane * W + k]);
+    h[k] = apply(maps[group][k * kLanes + lane], wave_states[wave][k * kLanes + lane]);
 
   const bool whole = s.channels % W == 0;
   const auto store = [&](void* to_, int64_t stride, int r, const float (&v)[W]) {
@@ -553,12 +608,12 @@ inline unsigned blocks_for_elements(int64_t threads) {
 }
 
 // Few columns of tiles that all run at once wait for the state to come through them: a look-back that
-// asks more tiles at a time takes fewer turns.  (Window 4 and 16, us: 131072 x 64 101 and 62, 32768 x 512 36 and 31;
+// asks more tiles at a time takes fewer turns.  (Window 4 and 16, us: 131072 x 64 101 and 59, 32768 x 512 36 and 31;
 // but 65536 x 2048 208 and 213, 2000 x 512 11.2 and 11.9; backwards 4 and 8: 65536 x 64 101 and 75.)
 constexpr int kFewColumns = 8;
 // Backwards, three tiles of four rows a thread or two of eight share a compute unit.  Eight rows are taken
 // where they make one turn of a grid that four would not, and where the chain of tiles is long but one turn still holds
-// it (us, 4 and 8: 8192 x 1024 28.6 and 26.7, 16384 x 512 32.7 and 27.7, 65536 x 64 75 and 50; but
+// it (us, 4 and 8: 8192 x 1024 28.6 and 26.7, 16384 x 512 32.7 and 27.7, 65536 x 64 75 and 43; but
 // 4096 x 1024 18.3 and 20.7, 16384 x 768 41 and 45).
 constexpr int64_t kManyTiles = 128;
 

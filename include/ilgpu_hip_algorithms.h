@@ -569,6 +569,10 @@ int32_t ilgpu_hip_clip_gradients(ilgpu_hip_stream_t stream,
  * sequence and behind the last are not written.  offsets ascend from 0 or more to
  * at most rows; others give unspecified results, but no access outside the
  * matrices.
+ * Decays and states are float32: exp(gate) of a gate above 88.7 is infinite, of one
+ * below -87.3 it may be zero, and a state that decays above 1 take beyond the
+ * largest float32 is infinite or a NaN from there on.  The decays of many rows may
+ * leave float32 together, as long as the states do not.
  * One row for each sequence (offsets NULL, sequences == rows) is the step from
  * token to token; it needs no temp.
  * out may be gate or in itself, final_state may be initial itself (same base and

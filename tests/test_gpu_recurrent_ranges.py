@@ -1,0 +1,104 @@
+"""The gated recurrence, the residual norm and the AdamW step at the ends of their ranges, against
+their formulas in float64.
+
+Inputs and tolerances are those of test_gpu_recurrent_operators, which says where they come from;
+u = 2^-24 here too.
+"""
+import pytest
+
+from tests.test_gpu_recurrent_operators import (
+    KINDS, TYPES, U, _array, _check_gradient, _check_recurrence, _close, _gradient, _matrix, _normal,
+    _rng, _run, _t)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- decays whose product over some rows leaves float32 ------------------------------------
+# Rows whose gates add up to more than 88.7 grow beyond float32 together, whatever comes in.
+@pytest.mark.parametrize("backwards", [False, True])
+@pytest.mark.parametrize("dtype,rows,channels", [("float32", 700, 70), ("float16", 900, 136),
+                                                 ("bfloat16", 900, 136), ("bfloat16", 300, 3),
+                                                 ("bfloat16", 17_000, 24)])
+def test_growing_decays_leave_nothing_where_nothing_comes_in(dtype, rows, channels, backwards):
+    import torch
+    from ilgpu_amd import capi
+    g = _rng(rows, channels, backwards)
+    gate = (0.3 + 2.0 * torch.rand(rows, channels, generator=g, device="cuda")).to(_t(dtype))
+    given = torch.zeros(rows, channels, dtype=_t(dtype), device="cuda")
+    # (every third channel has a number at the end of the scan, which does not pass any rows)
+    given[0 if backwards else rows - 1, ::3] = 1.5
+    zeros, out, grads = torch.zeros_like(given), torch.empty_like(given), torch.empty_like(given)
+    last = torch.empty(1, channels, device="cuda")
+    if backwards:
+        capi.gated_recurrence_gradient(
+            *(_matrix(t) for t in (given, gate, zeros, zeros, out, grads)),
+            grad_initial=_matrix(last), decay=capi.DECAY_EXPONENTIAL)
+        assert torch.equal(grads, given) and bool((out == 0).all())
+        want = given[0].double() * gate[0].double().exp()
+        _close(last[0], want, 24 * U * want)
+    else:
+        _run(capi, gate, given, out, "exponential", False, final=last)
+        assert torch.equal(out, given) and torch.equal(last[0], given[-1].float())
+
+
+def _growth(rows, dtype):
+    """Gates of 512 rows that leave a state as it is and of `rows` through which it grows by e^0 to
+    e^150, a channel each, and what grows to 1e30."""
+    import torch
+    total = torch.linspace(0.0, 150.0, 76, dtype=torch.float64, device="cuda")
+    gate = (total / rows).to(dtype)
+    gates = torch.cat((torch.zeros(512, 76, dtype=dtype, device="cuda"), gate.expand(rows, 76)))
+    return gates, (1e30 * torch.exp(-rows * gate.double())).float()[None]
+
+
+# A tile has 256 rows at most, which is all of the growth, or more of it than float32 holds.
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows", [100, 256, 1200])
+def test_states_that_grow_or_fall_through_all_of_float32(rows, dtype):
+    import torch
+    from ilgpu_amd import capi
+    gates, start = _growth(rows, _t(dtype))
+    large, none = torch.full_like(start, 1e30), torch.zeros_like(gates)
+    _check_recurrence(gates, none, "exponential", False, 1, None, start)
+    _, final = _check_recurrence(-gates, none, "exponential", False, 1, None, large)
+    assert bool((final > 0).all())
+    # up and down again, with something added in all rows
+    _check_recurrence(torch.cat((gates, -gates)), torch.cat((none, none + 1.0)), "exponential", False, 1, None,
+                      start)
+    # and backwards; states of zero, so that the gates' gradients are
+    for way, grad_final in ((gates.flip(0), start), (-gates.flip(0), large)):
+        got = _gradient(capi, none, way, none, none, "exponential", False, 1, None, None, grad_final)
+        _check_gradient(got, none, way, none, none, "exponential", False, [0, len(gates)], None, grad_final)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_an_infinite_state_stays_infinite_however_long(dtype, kind):
+    import torch
+    from ilgpu_amd import capi
+    rows, channels = 2500, 72
+    gate = torch.full((rows, channels), -3.0, dtype=_t(dtype), device="cuda")
+    x = _normal(_rng(rows, 11), rows, channels, dtype=_t(dtype))
+    x[0, ::2] = float("inf")
+    x[0, 1::4] = -float("inf")
+    out = torch.empty_like(x)
+    _run(capi, gate, x, out, kind, False)
+    assert bool((out[:, ::2] == float("inf")).all()) and bool((out[:, 1::4] == -float("inf")).all())
+    assert bool(torch.isfinite(out[:, 3::4]).all())
+
+
+def test_growing_decays_give_the_same_bits_again():
+    import torch
+    from ilgpu_amd import capi
+    g = _rng(12)
+    gate, x = (0.05 * torch.randn(20_011, 136, generator=g, device="cuda")).bfloat16(), \
+        _normal(g, 20_011, 136, dtype=torch.bfloat16)
+    runs = []
+    for _ in range(4):
+        out, of_gate, of_x = (torch.empty_like(x) for _ in range(3))
+        _run(capi, gate, x, out, "exponential", False)
+        capi.gated_recurrence_gradient(*(_matrix(t) for t in (x, gate, x, x, of_gate, of_x)),
+                                       decay=capi.DECAY_EXPONENTIAL)
+        runs.append([t.view(torch.uint8).clone() for t in (out, of_gate, of_x)])
+    for run in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(run, runs[0]))
