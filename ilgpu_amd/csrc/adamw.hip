@@ -282,7 +282,9 @@ template <int POWER> struct Code {
     return low + (rest > 0.0f ? 1.0f : 0.0f);
   }
 };
-constexpr float kSmallest = 0x1p-126f;
+// Scales below the first are none: all codes are those of zero.  The reciprocals of those above the second
+// are below the normal numbers, and the instruction may give 0 for them: their codes are made exactly.
+constexpr float kSmallest = 0x1p-126f, kLargest = 0x1p126f;
 
 typedef uint32_t WordAt1 __attribute__((aligned(1)));
 __device__ __forceinline__ uint32_t load_codes(const void* p, int64_t at, int count) {
@@ -394,14 +396,13 @@ __global__ __launch_bounds__(kBlock, EIGHT ? 8 : 4) void adamw_kernel(StepTable 
         }
       }
       const float scale1 = wave_largest(largest1), scale2 = wave_largest(largest2);
-      // (A scale below the normal numbers is none: all codes are those of zero.)
       const float inverse1 = scale1 < kSmallest ? 0.0f : (float)Code<2>::kAll * __builtin_amdgcn_rcpf(scale1);
       const float inverse2 = scale2 < kSmallest ? 0.0f : (float)Code<4>::kAll * __builtin_amdgcn_rcpf(scale2);
       uint32_t codes1 = 0, codes2 = 0;
 #pragma unroll
       for (int k = 0; k < kW; ++k) {
         const uint32_t chance = mixed((uint32_t)(at + k) * 0x9e3779b9u + key);
-        bool sure = true;
+        bool sure = scale1 <= kLargest && scale2 <= kLargest;
         float code1 = Code<2>::nearly(fabsf(moment1[k]), inverse1, chance & 0xffffu, sure);
         float code2 = Code<4>::nearly(moment2[k], inverse2, chance >> 16, sure);
         if (__any(!sure)) {  // (of a hundred waves one)

@@ -7,8 +7,8 @@ u = 2^-24 here too.
 import pytest
 
 from tests.test_gpu_recurrent_operators import (
-    KINDS, TYPES, U, _array, _check_gradient, _check_recurrence, _close, _gradient, _matrix, _normal,
-    _rng, _run, _t)
+    KINDS, TYPES, U, _adam_state, _adamw, _array, _check_adamw, _check_gradient,
+    _check_recurrence, _clone, _close, _gradient, _matrix, _normal, _rng, _run, _t)
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +102,19 @@ def test_growing_decays_give_the_same_bits_again():
         runs.append([t.view(torch.uint8).clone() for t in (out, of_gate, of_x)])
     for run in runs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(run, runs[0]))
+
+
+# ---- AdamW's codes ---------------------------------------------------------------------
+def test_moments_in_8_bits_near_the_largest_float32():
+    # Squares of 1.3e19 to 1.8e19 are floats, and the half of them is above 2^126, whose
+    # reciprocal is below the normal numbers; beside them a block with smaller ones.
+    import torch
+    from ilgpu_amd import capi
+    s = _adam_state(_rng(21), [1024], ("float32", "float32", None), True, fresh=True)
+    s["g"][0] = s["g"][0].sign() * torch.linspace(1e17, 1.8e19, 1024, device="cuda")
+    s["g"][0][512:768] = torch.linspace(1.0, 1.8e19, 256, device="cuda")
+    before = _clone(s)
+    _adamw(capi, s, betas=(0.9, 0.5))
+    _check_adamw(s, before, betas=(0.9, 0.5))
+    assert bool((s["v"][0].view(4, 256).max(1).values == 255).all())
+    assert bool(((s["m"][0].long() - 128).abs().view(4, 256).max(1).values == 127).all())
