@@ -263,9 +263,12 @@ template <int POWER> struct Code {
     }
     return fminf(low + (way > (double)chance * 0x1p-16 * span ? 1.0f : 0.0f), kLevels);
   }
-  // The same in float32; `sure` becomes false where its roundings, of at most 6 units of z, might decide,
-  // or where the root's might: there only the first or last chance tells the code above from the one
-  // below that is raised.  (90 million moments with both in float64 378 us, bound by its operations.)
+  // The same in float32; `sure` becomes false where its roundings might decide: z is off by 5 units of 2^-24 of
+  // it at most (the reciprocal by 2, the two products and the quotient of the exact way by one each), the rest by
+  // less than another.  Or where the root's might (another 12 units of z): `low` is then next to a code's value
+  // and one too large or too small, and the code is the same, one that is raised or the next that is not, unless
+  // chance / 2^16 of the way between two codes, z / 64 at least, is less than those 17 units: below 5, or that far
+  // from 2^16.  (90 million moments with both in float64 378 us, bound by its operations.)
   static __device__ __forceinline__ float nearly(float value, float inverse, uint32_t chance, bool& sure) {
     const float z = value * inverse, low = floorf(root(z));  // inverse: (float)kAll / scale
     const float step = fmaf(2.0f, low, 1.0f), square = low * low;
@@ -278,7 +281,7 @@ template <int POWER> struct Code {
       span = step * fmaf(2.0f, square, step);
     }
     const float rest = fmaf(-0x1p-16f * (float)chance, span, way);
-    sure = sure && fabsf(rest) > z * 4e-7f && chance - 1u < 65534u;
+    sure = sure && fabsf(rest) > z * 4e-7f && chance - 5u < 65527u;
     return low + (rest > 0.0f ? 1.0f : 0.0f);
   }
 };
@@ -405,7 +408,7 @@ __global__ __launch_bounds__(kBlock, EIGHT ? 8 : 4) void adamw_kernel(StepTable 
         bool sure = scale1 <= kLargest && scale2 <= kLargest;
         float code1 = Code<2>::nearly(fabsf(moment1[k]), inverse1, chance & 0xffffu, sure);
         float code2 = Code<4>::nearly(moment2[k], inverse2, chance >> 16, sure);
-        if (__any(!sure)) {  // (of a hundred waves one)
+        if (__any(!sure)) {  // (of a hundred waves three)
           code1 = scale1 < kSmallest ? 0.0f : Code<2>::exactly(fabsf(moment1[k]), scale1, chance & 0xffffu);
           code2 = scale2 < kSmallest ? 0.0f : Code<4>::exactly(moment2[k], scale2, chance >> 16);
         }

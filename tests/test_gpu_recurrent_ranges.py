@@ -7,8 +7,8 @@ u = 2^-24 here too.
 import pytest
 
 from tests.test_gpu_recurrent_operators import (
-    KINDS, TYPES, U, _adam_state, _adamw, _array, _check_adamw, _check_gradient,
-    _check_recurrence, _clone, _close, _gradient, _matrix, _normal, _rng, _run, _t)
+    BLOCK, KINDS, TYPES, U, WORD, _adam_state, _adamw, _array, _check_adamw, _check_gradient,
+    _check_recurrence, _clone, _close, _gradient, _matrix, _mixed, _normal, _rng, _run, _t)
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +118,55 @@ def test_moments_in_8_bits_near_the_largest_float32():
     _check_adamw(s, before, betas=(0.9, 0.5))
     assert bool((s["v"][0].view(4, 256).max(1).values == 255).all())
     assert bool(((s["m"][0].long() - 128).abs().view(4, 256).max(1).values == 127).all())
+
+
+def _codes(shares, power, levels, chance):
+    """The codes of shares of a scale, exactly: float64 holds a float32 times levels^power to a unit of 2^-53."""
+    import torch
+    z = shares.double() * float(levels) ** power
+    low = z.pow(1.0 / power).floor()
+    low = torch.where(low ** power > z, low - 1, low)
+    low = torch.where((low + 1) ** power <= z, low + 1, low)
+    way, span = z - low ** power, (low + 1) ** power - low ** power
+    return (low + (way * 65536 > chance * span)).clamp(max=levels)
+
+
+@pytest.mark.parametrize("second", [False, True])
+def test_codes_beside_what_a_code_stands_for(second):
+    # Values some units from a code's, at the first and last chances: the code above is raised from the one
+    # or the other side.  Without what was before (beta 0) the moments are the gradient and its square.
+    import torch
+    from ilgpu_amd import capi
+    power, levels = (4, 255) if second else (2, 127)
+    n, t = 1 << 25, 1
+    index = torch.arange(n, device="cuda")
+    g = _rng(22, second)
+    s = _adam_state(g, [n], ("float32", "float32", None), True, fresh=True)
+    s["step"][0] = t
+    compared = 0
+    for seed in range(77, 87):
+        key = _mixed(((seed & WORD) + t * 0x3C6EF373) & WORD)
+        key = _mixed((key + (seed >> 32 & WORD)) & WORD)
+        word = _mixed((index * 0x9E3779B9 + key) & WORD)
+        chance = word >> 16 if second else word & 0xFFFF
+        at = (((chance > 0) & (chance < 6)) | (chance > 65530)).nonzero()[:, 0]
+        at = at[(at % BLOCK) != 0]
+        largest = 1.0 + torch.rand(n // BLOCK, generator=g, device="cuda")
+        scale = (largest * largest if second else largest)[at // BLOCK]
+        code = torch.randint(levels // 2, levels, (at.numel(),), generator=g, device="cuda").double()
+        value = ((code / levels) ** power * scale.double()).float()
+        near = value.view(torch.int32) + torch.randint(-9, 10, (at.numel(),), generator=g, device="cuda").int()
+        s["g"][0].zero_()
+        s["g"][0][::BLOCK] = largest
+        s["g"][0][at] = near.view(torch.float32).sqrt() if second else near.view(torch.float32)
+        for k in ("m", "v", "ms", "vs"):
+            s[k][0].zero_()
+        _adamw(capi, s, betas=(0.0, 0.0), seed=seed)
+        assert torch.equal(s["vs" if second else "ms"][0][at // BLOCK], scale)
+        got = (s["v"][0][at].long() if second else s["m"][0][at].long() - 128).double()
+        values = s["g"][0][at] * s["g"][0][at] if second else s["g"][0][at]
+        shares = (values.cpu() / scale.cpu()).cuda()      # (rounded to float32 to the nearest)
+        want = _codes(shares, power, levels, chance[at].double())
+        assert torch.equal(got, want), (seed, int((got != want).sum()))
+        compared += at.numel()
+    assert compared > 30_000
