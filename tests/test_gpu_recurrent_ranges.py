@@ -170,3 +170,34 @@ def test_codes_beside_what_a_code_stands_for(second):
         assert torch.equal(got, want), (seed, int((got != want).sum()))
         compared += at.numel()
     assert compared > 30_000
+
+
+# ---- the exponential of float32 gates ------------------------------------------------------
+def _decays(gates, kind):
+    """Decays and what is left of them to 1, each alone: a state of 1 a row on, and an input of 1."""
+    import torch
+    from ilgpu_amd import capi
+    x = gates.reshape(-1, 64)
+    zero, one = torch.zeros_like(x), torch.ones_like(x)
+    a, left = torch.empty_like(x), torch.empty_like(x)
+    _run(capi, x, zero, a, kind, False, len(x), None, one)
+    _run(capi, x, one, left, kind, True, len(x))
+    return a.flatten(), left.flatten()
+
+
+def test_decays_of_large_float32_gates_keep_their_digits():
+    # The exponential is off by 4 u: the instruction's unit in the last place (2 u), the two roundings of what
+    # the product's rest makes of it; the rest itself is off by a thousandth of u.  The logistic function
+    # adds a sum, a reciprocal (2 u) and a product; 1 - exp is -1 and more of the exponential.
+    import torch
+    gates = torch.linspace(0.5, 87.0, 64 * 4096, device="cuda")
+    for sign in (1, -1):
+        x = sign * gates
+        e = torch.exp(x.double())
+        a, left = _decays(x, "exponential")
+        _close(a, e, 4 * U * e)
+        if sign > 0:
+            _close(left, 1 - e, 5 * U * e)
+        a, left = _decays(x, "sigmoid")
+        for got, exact in ((a, torch.sigmoid(x.double())), (left, torch.sigmoid(-x.double()))):
+            _close(got, exact, 12 * U * exact)
