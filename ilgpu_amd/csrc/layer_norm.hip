@@ -18,8 +18,6 @@ namespace ilgpu_hip {
 
 namespace {
 
-constexpr int64_t kMaxBlocks = 1 << 22;
-
 // Whether a row's mean is more than two deviations from zero. Below that its roundings are as
 // small as those of the deviations' own sums; beyond it a third sum finds the `rest` of the
 // mean: 32768 x 4096 bfloat16 100 us where all rows are far, 98 where none is.  (Added up in every
@@ -351,8 +349,8 @@ int32_t launch_layer_norm(hipStream_t stream, const LayerNormArgs& a) {
               blocks < most ? blocks : most, threads);
         },
         [&] {
-          return launch(layer_norm_long_kernel<T, TW>, a.rows < kMaxBlocks ? a.rows : kMaxBlocks,
-                        kLongBlock);
+          return launch(layer_norm_long_kernel<T, TW>,
+                        a.rows < kMaxLongBlocks ? a.rows : kMaxLongBlocks, kLongBlock);
         });
   });
 }
@@ -433,7 +431,7 @@ int32_t launch_layer_norm_gradient(hipStream_t stream, const LayerNormGradientAr
           if (grad_in != nullptr) {
             ProfileScope scope(stream, "layer_norm_grad_in");
             hipLaunchKernelGGL((layer_norm_long_grad_in_kernel<T, TW>),
-                               dim3((unsigned)(a.rows < kMaxBlocks ? a.rows : kMaxBlocks)),
+                               dim3((unsigned)(a.rows < kMaxLongBlocks ? a.rows : kMaxLongBlocks)),
                                dim3(kLongBlock), 0, stream, grad_out, a.grad_out_stride, in,
                                a.in_stride, a.rows, a.columns, weight, a.mean, a.rstd, grad_in,
                                a.grad_in_stride);

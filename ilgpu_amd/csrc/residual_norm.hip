@@ -15,7 +15,6 @@ namespace ilgpu_hip {
 
 namespace {
 
-constexpr int64_t kMaxBlocks = 1 << 22;
 constexpr int kLongBlock = kWholeBlock;
 
 // act(gate), and its slope.  Beyond kFar what is left is below the normal numbers: an infinite gate
@@ -558,8 +557,8 @@ int32_t launch_residual_norm(hipStream_t stream, const ResidualNormArgs& a) {
               blocks < most ? blocks : most, threads);
         },
         [&] {
-          return launch(residual_norm_long_kernel<T, TR>, a.rows < kMaxBlocks ? a.rows : kMaxBlocks,
-                        kLongBlock);
+          return launch(residual_norm_long_kernel<T, TR>,
+                        a.rows < kMaxLongBlocks ? a.rows : kMaxLongBlocks, kLongBlock);
         });
   });
 }
@@ -619,7 +618,7 @@ int32_t launch_residual_norm_gradient(hipStream_t stream, const ResidualNormGrad
       int64_t splits = partial_rows(a.rows) < kLongSplits ? partial_rows(a.rows) : kLongSplits;
       // (A grid holds less than 2^32 threads.)
       while (splits > 1 && across * splits * kBlock >= INT64_C(1) << 32) splits /= 2;
-      const int64_t blocks = a.rows < kMaxBlocks ? a.rows : kMaxBlocks;
+      const int64_t blocks = a.rows < kMaxLongBlocks ? a.rows : kMaxLongBlocks;
       float* means = partials + 2 * partial_rows(a.rows) * a.columns;
       {
         ProfileScope scope(stream, "residual_norm_means");

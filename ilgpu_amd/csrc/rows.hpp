@@ -40,6 +40,9 @@ template <int LANES> __device__ __forceinline__ float lanes_sum(float v) {
 // LANES is the number of lanes of a wave that share a row (8, 16, 32, 64), or kWholeBlock: all
 // threads of a block do, as many as the row's length asks for.
 constexpr int kWholeBlock = 1024;
+// Blocks of a launch of such: a grid holds less than 2^32 threads along an axis.  They go on to further rows.
+constexpr int64_t kMaxLongBlocks = 1 << 20;
+static_assert(kMaxLongBlocks * kWholeBlock < INT64_C(1) << 32, "threads of a grid");
 template <int LANES> __device__ __forceinline__ int row_lanes() {
   return LANES == kWholeBlock ? blockDim.x : LANES;
 }

@@ -201,3 +201,20 @@ def test_decays_of_large_float32_gates_keep_their_digits():
         a, left = _decays(x, "sigmoid")
         for got, exact in ((a, torch.sigmoid(x.double())), (left, torch.sigmoid(-x.double()))):
             _close(got, exact, 12 * U * exact)
+
+
+# ---- more rows than a grid of the largest blocks has ------------------------------------------
+def test_norm_gradient_of_very_many_long_rows():
+    # One row in the place of all.  Sums of ones are exact; with a weight of 1 of both norms the
+    # input's statistics take part too: the gradient of total is grad_out - mean(grad_out * h) * h = 0.
+    import torch
+    from ilgpu_amd import capi
+    rows, columns = (1 << 22) + 3, 8200
+    one = torch.ones(1, columns, dtype=torch.bfloat16, device="cuda").expand(rows, columns)
+    rstd = torch.ones(rows, device="cuda")
+    rstd[-3:] = 0.0
+    of_weight, of_input = (torch.full((columns,), 77.0, device="cuda") for _ in range(2))
+    capi.residual_norm_gradient(_matrix(one), None, _matrix(one), _matrix(one), None, _array(rstd),
+                                grad_weight=_array(of_weight), input_rstd=_array(rstd),
+                                grad_input_weight=_array(of_input))
+    assert bool((of_weight == 1 << 22).all()) and bool((of_input == 0).all())
