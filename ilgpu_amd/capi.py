@@ -958,9 +958,10 @@ def residual_norm_gradient(grad_out: Optional[DeviceMatrix], grad_total: Optiona
                            accumulate: bool = False, stream=None) -> None:
     """The gradients of residual_norm from those of out (None: not used) and of total (None:
     not used), and from total, rstd and input_rstd as it left them; those passed as None are
-    not computed.  With accumulate grad_weight and grad_input_weight are added to."""
+    not computed.  With an input norm, which an input_weight stands for here too, input_rstd
+    is needed.  With accumulate grad_weight and grad_input_weight are added to."""
     if input_norm is None:
-        input_norm = input_rstd is not None
+        input_norm = input_weight is not None or input_rstd is not None
     _same_shape(inp, grad_out=grad_out, grad_total=grad_total, total=total, grad_in=grad_in,
                 grad_residual=grad_residual, gate=gate, grad_gate=grad_gate)
     _same_type(inp, grad_out, gate, grad_in, grad_gate)
