@@ -41,25 +41,40 @@ namespace ILGPU.Algorithms.Hip
     }
 
     /// <summary>What a block's output passes through on its way into the residual stream:
-    /// a norm, a gate and a scale.</summary>
+    /// a norm, a gate and a scale.  default passes it on as it is.</summary>
     public struct HipBlockOutput<T, TWeight>
         where T : unmanaged
         where TWeight : unmanaged
     {
+        private float? scale;
+        private HipGateKind? kind;
+
         public HipBlockOutput(float scale)
         {
             Normalized = false;
             Weight = default;
             Gate = default;
-            Kind = HipGateKind.Silu;
-            Scale = scale;
+            kind = null;
+            this.scale = scale;
         }
 
         public bool Normalized;
         public ArrayView<TWeight> Weight;
         public HipMatrixView<T> Gate;
-        public HipGateKind Kind;
-        public float Scale;
+
+        /// <summary>Silu where nothing was set.</summary>
+        public HipGateKind Kind
+        {
+            get => kind ?? HipGateKind.Silu;
+            set => kind = value;
+        }
+
+        /// <summary>1 where nothing was set.</summary>
+        public float Scale
+        {
+            get => scale ?? 1.0f;
+            set => scale = value;
+        }
     }
 
     /// <summary>Where the gradients of ResidualNorm go; those left as default are not

@@ -1,5 +1,8 @@
 """Host-only checks of what the bindings of the recurrent operators make of arguments that are left
 out."""
+import os
+import re
+
 import numpy as np
 import pytest
 
@@ -19,3 +22,18 @@ def test_an_input_weight_stands_for_an_input_norm_in_the_gradients_too():
         capi.residual_norm_gradient(**args, input_norm=True)
     none = capi.DeviceMatrix(host_array(0, f32), 0, 4)
     capi.residual_norm_gradient(**{**args, "grad_total": none, "inp": none, "grad_in": none})
+
+
+def test_a_default_block_output_of_the_csharp_layer_is_passed_on_as_it_is():
+    # A struct is all zeros unless its constructor is called: what has another value where nothing was set
+    # is no plain field.  The C ABI's scale is 1, and the other layers' gate is silu.
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csharp",
+                        "ILGPU.Algorithms.Hip", "HipRecurrentModelExtensions.cs")
+    text = open(path).read()
+    struct = text[text.index("public struct HipBlockOutput"):]
+    struct = struct[:struct.index("\n    }\n")]
+    assert re.search(r"private float\? scale;", struct) and re.search(r"private HipGateKind\? kind;", struct)
+    for kind, name, value in (("float", "Scale", "scale ?? 1.0f"), ("HipGateKind", "Kind", "kind ?? HipGateKind.Silu")):
+        assert not re.search(rf"public {kind} {name};", struct)
+        body = re.search(rf"public {kind} {name}\s*{{(.*?)\n        }}", struct, flags=re.S)[1]
+        assert f"get => {value};" in body and "set => " in body
