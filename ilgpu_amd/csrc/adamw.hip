@@ -503,7 +503,7 @@ int32_t launch_adamw(hipStream_t stream, const AdamwArgs& a) {
     for (; next < a.count && used < kTensors; ++next) {
       const int64_t length = a.parameters[next].length;
       if (length == 0) continue;
-      chunks += div_up(length, (long_chunks ? kLongTurns : kShortTurns) * kTurn);  // (at most 2^28 and one per tensor)
+      chunks += div_up(length, (long_chunks ? kLongTurns : kShortTurns) * kTurn);  // (at most 2^29 and one per tensor)
       table.parameter[used] = a.parameters[next].data;
       table.gradient[used] = a.gradients[next].data;
       table.first[used] = a.first[next].data;

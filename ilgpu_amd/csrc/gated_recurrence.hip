@@ -609,12 +609,12 @@ inline unsigned blocks_for_elements(int64_t threads) {
 
 // Few columns of tiles that all run at once wait for the state to come through them: a look-back that
 // asks more tiles at a time takes fewer turns.  (Window 4 and 16, us: 131072 x 64 101 and 59, 32768 x 512 36 and 31;
-// but 65536 x 2048 208 and 213, 2000 x 512 11.2 and 11.9; backwards 4 and 8: 65536 x 64 101 and 75.)
+// but 65536 x 2048 208 and 213, 2000 x 512 11.2 and 11.9; backwards 4 and 8: 65536 x 64 101 and 75; all bfloat16.)
 constexpr int kFewColumns = 8;
 // Backwards, three tiles of four rows a thread or two of eight share a compute unit.  Eight rows are taken
 // where they make one turn of a grid that four would not, and where the chain of tiles is long but one turn still holds
 // it (us, 4 and 8: 8192 x 1024 28.6 and 26.7, 16384 x 512 32.7 and 27.7, 65536 x 64 75 and 43; but
-// 4096 x 1024 18.3 and 20.7, 16384 x 768 41 and 45).
+// 4096 x 1024 18.3 and 20.7, 16384 x 768 41 and 45; all bfloat16).
 constexpr int64_t kManyTiles = 128;
 
 inline int64_t columns_of_tiles(int64_t channels) { return div_up(channels, kTileChannels); }

@@ -53,7 +53,7 @@ template <typename T> __device__ __forceinline__ T* row_of(void* p, int64_t row,
   return static_cast<T*>(p) + row * stride;
 }
 
-// A float per row of the block, alternating between rows: what one row's sums are put into is
+// Two sums of a row, a float for each wave, alternating between rows: what one row's sums are put into is
 // read by others until the sums of the row behind it.
 using Slots = float[2][2][kMostWaves];
 
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(row_block<LANES>()) void residual_norm_kernel(Resid
   }
 }
 
-// W elements of a vector from column c on, `otherwise` where there is none.
+// W weights from column c on, 1 where there are none.
 template <typename T, int W>
 __device__ __forceinline__ void long_weights(float (&w)[W], const void* p, bool wide, int64_t c,
                                              int64_t count) {
