@@ -71,20 +71,26 @@ def test_states_that_grow_or_fall_through_all_of_float32(rows, dtype):
         _check_gradient(got, none, way, none, none, "exponential", False, [0, len(gates)], None, grad_final)
 
 
+# (Of gates of -20 the decays of eight rows, a thread's, are below float32 together.)
+@pytest.mark.parametrize("gate", [-3.0, -20.0])
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dtype", TYPES)
-def test_an_infinite_state_stays_infinite_however_long(dtype, kind):
+def test_an_infinite_state_stays_infinite_however_long(dtype, kind, gate):
     import torch
     from ilgpu_amd import capi
     rows, channels = 2500, 72
-    gate = torch.full((rows, channels), -3.0, dtype=_t(dtype), device="cuda")
+    gates = torch.full((rows, channels), gate, dtype=_t(dtype), device="cuda")
     x = _normal(_rng(rows, 11), rows, channels, dtype=_t(dtype))
     x[0, ::2] = float("inf")
     x[0, 1::4] = -float("inf")
-    out = torch.empty_like(x)
-    _run(capi, gate, x, out, kind, False)
-    assert bool((out[:, ::2] == float("inf")).all()) and bool((out[:, 1::4] == -float("inf")).all())
-    assert bool(torch.isfinite(out[:, 3::4]).all())
+    back = x.flip(0).contiguous()
+    out, grads = torch.empty_like(x), torch.empty_like(x)
+    _run(capi, gates, x, out, kind, False)
+    capi.gated_recurrence_gradient(*(_matrix(t) for t in (back, gates, x, x, None, grads)),
+                                   decay=getattr(capi, "DECAY_" + kind.upper()))
+    for got in (out, grads):
+        assert bool((got[:, ::2] == float("inf")).all()) and bool((got[:, 1::4] == -float("inf")).all())
+        assert bool(torch.isfinite(got[:, 3::4]).all())
 
 
 def test_growing_decays_give_the_same_bits_again():
@@ -218,3 +224,23 @@ def test_norm_gradient_of_very_many_long_rows():
                                 grad_weight=_array(of_weight), input_rstd=_array(rstd),
                                 grad_input_weight=_array(of_input))
     assert bool((of_weight == 1 << 22).all()) and bool((of_input == 0).all())
+
+
+# ---- more tiles than a launch has blocks ---------------------------------------------------
+# 2^22 blocks a launch; of one channel a tile has 32 rows, backwards 16.  A state of 1 has to come through
+# all of them unchanged.
+@pytest.mark.parametrize("backwards", [False, True])
+def test_a_state_passes_through_more_tiles_than_a_launch_has(backwards):
+    import torch
+    from ilgpu_amd import capi
+    rows = (1 << 27) // (2 if backwards else 1) + 77
+    gate = torch.zeros(1, 1, dtype=torch.bfloat16, device="cuda").expand(rows, 1)
+    given = torch.zeros(rows, 1, dtype=torch.bfloat16, device="cuda")
+    given[-1 if backwards else 0] = 1.0
+    out, last = torch.zeros_like(given), torch.empty(1, 1, device="cuda")
+    if backwards:
+        capi.gated_recurrence_gradient(*(_matrix(t) for t in (given, gate, gate, gate, None, out)),
+                                       grad_initial=_matrix(last), decay=capi.DECAY_EXPONENTIAL)
+    else:
+        _run(capi, gate, given, out, "exponential", False, final=last)
+    assert bool((out == 1.0).all()) and float(last) == 1.0
